@@ -1,0 +1,131 @@
+// Pieces that the attention operators share: rows spread over groups of lanes, conversions between element types.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "attention_kernels.hpp"
+#include "attention_plan.hpp"
+#include "launch.cuh"
+
+namespace rocshmem {
+namespace kernels {
+namespace attn {
+
+struct e4m3 {
+  uint8_t v;
+};
+
+// Eight consecutive elements of a row in 32 bits. 16-bit and fp32 rows move 16 bytes an access, e4m3 rows eight.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<float> {
+  float4 a, b;
+};
+template <>
+struct Raw8<__nv_bfloat16> {
+  uint4 a;
+};
+template <>
+struct Raw8<__half> {
+  uint4 a;
+};
+template <>
+struct Raw8<e4m3> {
+  uint2 a;
+};
+
+// Elements [8 at, 8 at + 8) of the row at `p`.
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const T *p, int at = 0) {
+  return *reinterpret_cast<const Raw8<T> *>(p + 8 * at);
+}
+
+__device__ __forceinline__ void unpack8(const Raw8<float> &r, float (&x)[8]) {
+  x[0] = r.a.x, x[1] = r.a.y, x[2] = r.a.z, x[3] = r.a.w, x[4] = r.b.x, x[5] = r.b.y, x[6] = r.b.z, x[7] = r.b.w;
+}
+__device__ __forceinline__ void unpack8(const Raw8<__nv_bfloat16> &r, float (&x)[8]) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack8(const Raw8<__half> &r, float (&x)[8]) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void unpack8(const Raw8<e4m3> &r, float (&x)[8]) {
+  const uint32_t w[2] = {r.a.x, r.a.y};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i / 2] >> (16 * (i % 2))), __NV_E4M3);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+  }
+}
+
+// One rounding to the nearest value of the type, ties to even.
+__device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
+  float4 *v = reinterpret_cast<float4 *>(p);
+  v[0] = make_float4(x[0], x[1], x[2], x[3]);
+  v[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16 *p, const float (&x)[8]) {
+  uint4 o;
+  uint32_t *w = reinterpret_cast<uint32_t *>(&o);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t *>(&h);
+  }
+  *reinterpret_cast<uint4 *>(p) = o;
+}
+__device__ __forceinline__ void store8(__half *p, const float (&x)[8]) {
+  uint4 o;
+  uint32_t *w = reinterpret_cast<uint32_t *>(&o);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t *>(&h);
+  }
+  *reinterpret_cast<uint4 *>(p) = o;
+}
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ void store1(float *p, float x) { *p = x; }
+__device__ __forceinline__ void store1(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+__device__ __forceinline__ void store1(__half *p, float x) { *p = __float2half_rn(x); }
+
+// Sum over the `LANES` neighbouring lanes (a power of two) that hold one row.
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <int LANES>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Lanes that hold a row of `dim` elements, eight each: 8, 16 or 32 (those past the row's end hold zeros).
+inline int row_lanes(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
+
+}  // namespace attn
+}  // namespace kernels
+}  // namespace rocshmem

@@ -1,0 +1,66 @@
+// Arithmetic of paged attention that the host launcher, the kernels and a CPU test share: how a batch of sequences is
+// cut into tiles of keys, how the tiles are dealt to blocks, and where a row of the cache lies.
+//
+// The tiles of all (sequence, unit) pairs stand in one line: sequence by sequence, within it unit by unit (a unit is a
+// key head and up to 8 * NT of its query heads), within that tile by tile. Block c takes the tiles [c * per_block,
+// (c + 1) * per_block) of the line, whatever pairs they belong to. A pair that lies in one block is finished there; one
+// that several blocks share leaves a partial result in each of them. A block has at most two such pairs, the first and
+// the last of its range, so two places per block hold all partial results whatever the lengths are.
+#pragma once
+
+#include <cstdint>
+
+#ifdef __CUDACC__
+#define ATTN_HD __host__ __device__ __forceinline__
+#else
+#define ATTN_HD inline
+#endif
+
+namespace rocshmem {
+namespace kernels {
+namespace attn {
+
+// The positions [first, end) that a sequence's new token sees. Lengths below zero count as zero, those past the end of
+// the block table as its end; window > 0 leaves the last `window` positions.
+struct Span {
+  int first, end;
+};
+ATTN_HD Span visible(int length, int capacity, int window) {
+  const int end = length < 0 ? 0 : (length > capacity ? capacity : length);
+  return Span{window > 0 && end > window ? end - window : 0, end};
+}
+
+ATTN_HD int tiles_of(Span s, int tile_keys) { return (s.end - s.first + tile_keys - 1) / tile_keys; }
+
+// Tiles that a block takes: an equal share, but not fewer than `least` (a block's fixed costs).
+ATTN_HD long long per_block(long long total, int blocks, int least) {
+  const long long share = (total + blocks - 1) / blocks;
+  return share < least ? least : share;
+}
+
+// The blocks that share a pair whose tiles are [begin, begin + n), n > 0.
+struct Owners {
+  long long first, last;
+};
+ATTN_HD Owners owners(long long begin, int n, long long per) { return Owners{begin / per, (begin + n - 1) / per}; }
+
+// Which of block c's two places holds its partial result of a pair that blocks `o` share: 0 for a pair that an earlier
+// block began, 1 for one that a later block ends.
+ATTN_HD int place(Owners o, long long c) { return c > o.first ? 0 : 1; }
+
+// Row (of `dim` elements) of position `pos` in a cache [pages, kv_heads, page_size, dim], or -1 where the position is
+// not visible or its page is no page of the cache. page_size = 1 << shift.
+ATTN_HD int page_row(int page, int num_pages, int pos, int shift, int kv_heads, int head) {
+  if (page < 0 || page >= num_pages) return -1;
+  return ((page * kv_heads + head) << shift) + (pos & ((1 << shift) - 1));
+}
+
+// The same for a flat slot (page * page_size + offset), or -1 for a slot outside the cache.
+ATTN_HD long long slot_row(long long slot, long long num_slots, int shift, int kv_heads, int head) {
+  if (slot < 0 || slot >= num_slots) return -1;
+  return (((slot >> shift) * kv_heads + head) << shift) + (slot & ((1ll << shift) - 1));
+}
+
+}  // namespace attn
+}  // namespace kernels
+}  // namespace rocshmem

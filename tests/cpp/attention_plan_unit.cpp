@@ -1,0 +1,103 @@
+// The arithmetic of paged attention's split (attention_plan.hpp) on the CPU: every tile of every pair is taken by exactly
+// one block, in order; partial results of one pair lie in places of their own; rows of pages that do not exist are refused.
+#include <cstdio>
+#include <cstdlib>
+#include <map>
+#include <random>
+#include <set>
+#include <utility>
+#include <vector>
+
+#include "kernels/attention_plan.hpp"
+
+using namespace rocshmem::kernels::attn;
+
+#define CHECK(cond)                                                     \
+  do {                                                                  \
+    if (!(cond)) {                                                      \
+      std::fprintf(stderr, "%s:%d: %s\n", __FILE__, __LINE__, #cond);   \
+      std::exit(1);                                                     \
+    }                                                                   \
+  } while (0)
+
+namespace {
+
+void check_spans() {
+  CHECK(visible(-3, 100, 0).end == 0);
+  CHECK(visible(-3, 100, 0).first == 0);
+  CHECK(visible(500, 100, 0).end == 100);
+  CHECK(visible(50, 100, 20).first == 30 && visible(50, 100, 20).end == 50);
+  CHECK(visible(20, 100, 20).first == 0);
+  CHECK(visible(5, 100, 20).first == 0);
+  CHECK(tiles_of(visible(0, 100, 0), 64) == 0);
+  CHECK(tiles_of(visible(1, 100, 0), 64) == 1);
+  CHECK(tiles_of(visible(64, 100, 0), 64) == 1);
+  CHECK(tiles_of(visible(65, 100, 0), 64) == 2);
+  CHECK(tiles_of(visible(0x7fffff00, 0x7fffff00, 0), 128) == 0x7fffff00 / 128);
+}
+
+void check_rows() {
+  CHECK(page_row(-1, 8, 5, 4, 2, 1) == -1);
+  CHECK(page_row(8, 8, 5, 4, 2, 1) == -1);
+  CHECK(page_row(-2147483647 - 1, 8, 5, 4, 2, 1) == -1);
+  CHECK(page_row(2147483647, 8, 5, 4, 2, 1) == -1);
+  CHECK(page_row(7, 8, 16 + 5, 4, 2, 1) == ((7 * 2 + 1) << 4) + 5);
+  CHECK(page_row(3, 4, 9, 0, 1, 0) == 3);
+  CHECK(slot_row(-1, 64, 4, 2, 1) == -1);
+  CHECK(slot_row(64, 64, 4, 2, 1) == -1);
+  CHECK(slot_row(1ll << 40, 64, 4, 2, 1) == -1);
+  CHECK(slot_row(63, 64, 4, 2, 1) == ((3 * 2 + 1) << 4) + 15);
+  // Row numbers past 32 bits, with 2^28 pages of 16 slots and two heads.
+  CHECK(slot_row((1ll << 32) - 1, 1ll << 32, 4, 2, 1) == (((1ll << 28) - 1) * 2 + 1) * 16 + 15);
+}
+
+void check_split(const std::vector<int> &lengths, int capacity, int window, int units, int blocks, int least, int tile) {
+  std::vector<long long> bases;
+  long long total = 0;
+  for (int n : lengths) {
+    bases.push_back(total);
+    total += static_cast<long long>(tiles_of(visible(n, capacity, window), tile)) * units;
+  }
+  const long long per = per_block(total, blocks, least);
+  CHECK(per >= least && per * blocks >= total);
+  std::set<std::pair<long long, int>> places;
+  for (size_t b = 0; b < lengths.size(); ++b) {
+    const int n = tiles_of(visible(lengths[b], capacity, window), tile);
+    for (int u = 0; u < units && n > 0; ++u) {
+      const long long begin = bases[b] + static_cast<long long>(u) * n;
+      const Owners own = owners(begin, n, per);
+      CHECK(own.first >= 0 && own.first <= own.last && own.last < blocks);
+      // The tiles that the owners' ranges hold of this pair are all of them.
+      long long seen = 0;
+      for (long long c = own.first; c <= own.last; ++c) {
+        const long long lo = c * per > begin ? c * per : begin;
+        const long long hi = (c + 1) * per < begin + n ? (c + 1) * per : begin + n;
+        CHECK(hi > lo);
+        seen += hi - lo;
+        if (own.first == own.last) continue;
+        // What the block itself goes by: it begins the pair (place 1) or finds it begun (place 0).
+        CHECK(place(own, c) == (lo == begin ? 1 : 0));
+        CHECK(places.insert({c, place(own, c)}).second);
+      }
+      CHECK(seen == n);
+    }
+  }
+}
+
+}  // namespace
+
+int main() {
+  check_spans();
+  check_rows();
+  std::mt19937 rng(5);
+  for (int round = 0; round < 3000; ++round) {
+    std::vector<int> lengths(1 + rng() % 40);
+    const int most = 1 << (rng() % 14);
+    for (int &n : lengths) n = rng() % 5 == 0 ? 0 : static_cast<int>(rng() % (most + 2)) - 1;
+    const int window = rng() % 3 == 0 ? 1 + rng() % most : 0;
+    check_split(lengths, most, window, 1 + rng() % 9, 1 + rng() % 300, 1 + rng() % 4, rng() % 2 ? 64 : 128);
+  }
+  check_split({1000000, 0, 1}, 1 << 20, 0, 1, 296, 2, 64);
+  std::puts("ok");
+  return 0;
+}
