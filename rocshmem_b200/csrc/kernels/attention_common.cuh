@@ -123,6 +123,11 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
   return v;
 }
 
+template <int V>
+struct Int {
+  static constexpr int value = V;
+};
+
 // Lanes that hold a row of `dim` elements, eight each: 8, 16 or 32 (those past the row's end hold zeros).
 inline int row_lanes(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
 

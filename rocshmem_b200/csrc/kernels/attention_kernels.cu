@@ -79,12 +79,11 @@ template <typename T, typename W, int LANES, int ROWS>
 __global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRope<T, W> a, T *q_out, T *k_out) {
   const int lane = threadIdx.x % LANES;
   const int heads = a.q_heads + a.k_heads;
-  const int chunks = (heads + ROWS - 1) / ROWS;
-  const long long items = static_cast<long long>(a.tokens) * chunks;
+  const unsigned chunks = (heads + ROWS - 1) / ROWS, items = a.tokens * chunks;
   // All lanes of a warp take part in every shuffle: groups past the last item work on it again and store nothing.
-  const long long mine = static_cast<long long>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
-  const long long item = mine < items ? mine : items - 1;
-  const int t = static_cast<int>(item / chunks), h0 = static_cast<int>(item % chunks) * ROWS;
+  const unsigned mine = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  const unsigned item = min(mine, items - 1), t = item / chunks;
+  const int h0 = (item - t * chunks) * ROWS;
   const bool in_row = 8 * lane < a.dim;
   const long long pos = load_index(a.positions, a.wide_positions, t);
   const bool live = pos >= 0, known = pos < a.table_rows;
@@ -151,20 +150,19 @@ __global__ void __launch_bounds__(kThreads) norm_rope_backward_kernel(NormRope<T
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   constexpr int kGroups = kThreads / LANES;
   const int heads = a.q_heads + a.k_heads;
-  const int chunks = (heads + ROWS - 1) / ROWS;
-  const long long items = static_cast<long long>(a.tokens) * chunks;
+  const unsigned chunks = (heads + ROWS - 1) / ROWS, items = a.tokens * chunks;
   const bool in_row = 8 * lane < a.dim, rotated = 8 * lane < a.rotary;
   float wq[8] = {}, wk[8] = {}, dwq[8] = {}, dwk[8] = {};
   if (in_row) {
     unpack8(load8(a.q_weight, lane), wq);
     unpack8(load8(a.k_weight, lane), wk);
   }
-  const long long step = static_cast<long long>(gridDim.x) * kGroups;
+  const unsigned step = gridDim.x * kGroups;
   // The same number of rounds for all groups of a block, for the shuffles.
-  for (long long base = static_cast<long long>(blockIdx.x) * kGroups; base < items; base += step) {
+  for (unsigned base = blockIdx.x * kGroups; base < items; base += step) {
     const bool has = base + group < items;
-    const long long item = has ? base + group : items - 1;
-    const int t = static_cast<int>(item / chunks), h0 = static_cast<int>(item % chunks) * ROWS;
+    const unsigned item = has ? base + group : items - 1, t = item / chunks;
+    const int h0 = (item - t * chunks) * ROWS;
     const long long pos = load_index(a.positions, a.wide_positions, t);
     const bool live = pos >= 0, known = pos < a.table_rows;
     Raw8<T> raw[ROWS], graw[ROWS];
@@ -272,7 +270,19 @@ struct Cache {
   int kv_heads, shift, dim;
 };
 
-// Rows are numbered (token, k or v, head); a group takes ROWS rows that lie a grid apart, their loads first.
+// The head and the first of its tokens that a group of lanes has.
+struct Row {
+  long long token;
+  int head;
+  bool is_v;
+};
+__device__ __forceinline__ Row row_of(unsigned group, int tokens_each, int kv_heads) {
+  const unsigned each = 2 * kv_heads, chunk = group / each, h = group - chunk * each;
+  return Row{static_cast<long long>(chunk) * tokens_each, static_cast<int>(h < kv_heads ? h : h - kv_heads), h >= kv_heads};
+}
+
+// A group of lanes takes one head's row (of k or of v) of ROWS neighbouring tokens, their loads first. Neighbouring groups
+// take the token's other heads: reads are contiguous across a block, and a head's rows go to neighbouring places of its page.
 //
 // e4m3: with m the largest magnitude of the row, codes are x * (448 / m) and the factor m / 448. m is held above 2^-110,
 // below which 448 / m would overflow. The largest magnitude is that of the bits, so that a NaN or infinity becomes m, and
@@ -284,31 +294,25 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(Cache<C> c, const T 
   constexpr bool kQuantize = sizeof(C) == 1;
   const int lane = threadIdx.x % LANES;
   const bool in_row = 8 * lane < c.dim;
-  const long long rows = static_cast<long long>(tokens) * 2 * c.kv_heads;
-  const long long step = static_cast<long long>(gridDim.x) * (kThreads / LANES);
-  const long long first = static_cast<long long>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
+  const Row w = row_of(blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES, ROWS, c.kv_heads);
+  const T *from = (w.is_v ? v + w.head * v_head : k + w.head * k_head) + w.token * (w.is_v ? v_token : k_token);
+  const long long step = w.is_v ? v_token : k_token;
   Raw8<T> raw[ROWS];
   long long to[ROWS];
-  bool is_v[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    const long long row = first + r * step;
     to[r] = -1;
-    is_v[r] = false;
     raw[r] = Raw8<T>{};
-    if (row < rows) {
-      const int t = static_cast<int>(row / (2 * c.kv_heads)), w = static_cast<int>(row % (2 * c.kv_heads));
-      is_v[r] = w >= c.kv_heads;
-      const int h = is_v[r] ? w - c.kv_heads : w;
-      to[r] = slot_row(load_index(slots, wide_slots, t), c.slots, c.shift, c.kv_heads, h);
-      if (to[r] >= 0 && in_row) raw[r] = load8(is_v[r] ? v + t * v_token + h * v_head : k + t * k_token + h * k_head, lane);
+    if (w.token + r < tokens) {
+      if (in_row) raw[r] = load8(from + r * step, lane);
+      to[r] = slot_row(load_index(slots, wide_slots, static_cast<int>(w.token) + r), c.slots, c.shift, c.kv_heads, w.head);
     }
   }
+  C *base = w.is_v ? c.v : c.k;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     float x[8];
     unpack8(raw[r], x);
-    C *base = is_v[r] ? c.v : c.k;
     if constexpr (kQuantize) {
       uint32_t top = 0;
 #pragma unroll
@@ -320,17 +324,17 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(Cache<C> c, const T 
       if (to[r] >= 0) {
         if (in_row) {
           uint2 o;
-          uint32_t *w = reinterpret_cast<uint32_t *>(&o);
+          uint32_t *codes = reinterpret_cast<uint32_t *>(&o);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float2 a = make_float2(x[4 * i] * inv, x[4 * i + 1] * inv);
             const float2 b = make_float2(x[4 * i + 2] * inv, x[4 * i + 3] * inv);
-            w[i] = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
+            codes[i] = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
                    static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3)) << 16;
           }
           *reinterpret_cast<uint2 *>(base + to[r] * c.dim + 8 * lane) = o;
         }
-        if (lane == 0) (is_v[r] ? c.v_scale : c.k_scale)[to[r]] = m * (1.0f / 448.0f);
+        if (lane == 0) (w.is_v ? c.v_scale : c.k_scale)[to[r]] = m * (1.0f / 448.0f);
       }
     } else {
       if (to[r] >= 0 && in_row) store8(base + to[r] * c.dim + 8 * lane, x);
@@ -343,57 +347,67 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(Cache<C> c, T *k_out,
                                                            int wide_slots, int tokens) {
   const int lane = threadIdx.x % LANES;
   const bool in_row = 8 * lane < c.dim;
-  const long long rows = static_cast<long long>(tokens) * 2 * c.kv_heads;
-  const long long step = static_cast<long long>(gridDim.x) * (kThreads / LANES);
-  const long long first = static_cast<long long>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
+  const Row w = row_of(blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES, ROWS, c.kv_heads);
+  const C *base = w.is_v ? c.v : c.k;
+  T *out = (w.is_v ? v_out : k_out) + (w.token * c.kv_heads + w.head) * c.dim + 8 * lane;
+  const long long step = static_cast<long long>(c.kv_heads) * c.dim;
+  if (!in_row) return;
   Raw8<C> raw[ROWS];
   float factor[ROWS];
-  T *to[ROWS];
+  long long from[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    const long long row = first + r * step;
+    from[r] = w.token + r < tokens ? slot_row(load_index(slots, wide_slots, static_cast<int>(w.token) + r), c.slots, c.shift,
+                                              c.kv_heads, w.head) : -1;
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
     raw[r] = Raw8<C>{};
     factor[r] = 0.f;
-    to[r] = nullptr;
-    if (row < rows && in_row) {
-      const int t = static_cast<int>(row / (2 * c.kv_heads)), w = static_cast<int>(row % (2 * c.kv_heads));
-      const bool is_v = w >= c.kv_heads;
-      const int h = is_v ? w - c.kv_heads : w;
-      to[r] = (is_v ? v_out : k_out) + (static_cast<long long>(t) * c.kv_heads + h) * c.dim + 8 * lane;
-      const long long from = slot_row(load_index(slots, wide_slots, t), c.slots, c.shift, c.kv_heads, h);
-      if (from >= 0) {
-        raw[r] = load8((is_v ? c.v : c.k) + from * c.dim, lane);
-        if constexpr (sizeof(C) == 1) factor[r] = (is_v ? c.v_scale : c.k_scale)[from];
-      }
+    if (from[r] >= 0) {
+      raw[r] = load8(base + from[r] * c.dim, lane);
+      if constexpr (sizeof(C) == 1) factor[r] = (w.is_v ? c.v_scale : c.k_scale)[from[r]];
     }
   }
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    if (to[r] == nullptr) continue;
+    if (w.token + r >= tokens) return;
     float x[8];
     unpack8(raw[r], x);
     if constexpr (sizeof(C) == 1) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] *= factor[r];
     }
-    store8(to[r], x);
+    store8(out + r * step, x);
   }
 }
 
 // ---- the join of partial results ---------------------------------------------------------------------------------
 
-// out = sum w_i o_i / sum w_i with w_i = exp(lse_i - max). A part whose lse is -inf has seen nothing and is not read.
+// out = sum w_i o_i / sum w_i with w_i = exp(lse_i - max). A part whose lse is -inf has seen nothing and
+// does not count, whatever its rows hold.
 template <typename T, typename O, int LANES>
 __global__ void __launch_bounds__(kThreads) join_kernel(const T *outs, const float *lses, long long out_part,
                                                         long long lse_part, int parts, long long rows, int dim, O *out,
                                                         float *lse) {
-  constexpr int kAhead = 4;  // parts whose loads are in flight
+  constexpr int kAhead = sizeof(T) == 4 ? 4 : 8;  // parts whose loads are in flight
   const int lane = threadIdx.x % LANES;
   const long long row = static_cast<long long>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
   if (row >= rows) return;
   const bool in_row = 8 * lane < dim;
+  const T *from = outs + row * dim;
+  Raw8<T> raw[kAhead];
+  auto fetch = [&](int p0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      raw[i] = Raw8<T>{};
+      if (p0 + i < parts && in_row) raw[i] = load8(from + (p0 + i) * out_part, lane);
+    }
+  };
+  fetch(0);  // on their way while the maximum is found
   float top = -INFINITY;
   bool bad = false;
+#pragma unroll 4
   for (int p = 0; p < parts; ++p) {
     const float l = lses[p * lse_part + row];
     bad |= l != l;
@@ -401,24 +415,21 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const T *outs, const flo
   }
   const float base = top == -INFINITY ? 0.f : top;
   float acc[8] = {}, total = 0.f;
-  for (int p0 = 0; p0 < parts; p0 += kAhead) {
-    Raw8<T> raw[kAhead];
-    float w[kAhead];
+  for (int p0 = 0;;) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int p = p0 + i;
-      raw[i] = Raw8<T>{};
-      w[i] = p < parts ? expf(lses[p * lse_part + row] - base) : 0.f;
-      if (w[i] != 0.f && in_row) raw[i] = load8(outs + p * out_part + row * dim, lane);
-    }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+      if (p0 + i >= parts) break;
+      const float l = lses[(p0 + i) * lse_part + row], w = expf(l - base);
+      total += w;
+      if (l == -INFINITY) continue;
       float x[8];
       unpack8(raw[i], x);
-      total += w[i];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = fmaf(w[i], x[e], acc[e]);
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, x[e], acc[e]);
     }
+    p0 += kAhead;
+    if (p0 >= parts) break;
+    fetch(p0);
   }
   const float inv = total > 0.f || bad ? 1.f / total : 0.f;
   float x[8];
@@ -445,10 +456,6 @@ int with_type(int code, F f) {
   }
 }
 
-template <int V>
-struct Int {
-  static constexpr int value = V;
-};
 template <typename F>
 int with_lanes(int dim, F f) {
   switch (row_lanes(dim)) {
@@ -460,10 +467,10 @@ int with_lanes(int dim, F f) {
 
 bool bad_rows(int dim) { return dim < 8 || dim > 256 || dim % 8; }
 
-// Blocks of a launch with one group of lanes for each of `items`; 0 when that is more than a grid takes.
+// Blocks of a launch with one group of lanes for each of `items`; 0 when the kernels could not number the groups in 32 bits.
 unsigned blocks_for(long long items, int lanes) {
   const long long per = kThreads / lanes, n = (items + per - 1) / per;
-  return n > 0x7fffffffll ? 0u : static_cast<unsigned>(n);
+  return n * per > 0x7fffffffll ? 0u : static_cast<unsigned>(n);
 }
 
 int backward_blocks() { return device_sm_count() * 2; }
@@ -557,6 +564,7 @@ int qk_norm_rope_backward(const NormRopeArgs &a, const void *gq, const void *gk,
       const long long items = static_cast<long long>(a.tokens) * ((heads + kRows - 1) / kRows);
       const long long per = kThreads / kLanes;
       const int blocks = static_cast<int>(std::min<long long>(backward_blocks(), (items + per - 1) / per));
+      if (items > 0x7fffffffll - static_cast<long long>(blocks) * per) return cudaErrorInvalidValue;
       if (blocks > 0) {
         norm_rope_backward_kernel<T, W, kLanes, kRows><<<blocks, kThreads, kThreads / kLanes * 2 * a.dim * sizeof(float), s>>>(
             norm_rope_args<T, W>(a), static_cast<const T *>(gq), static_cast<const T *>(gk), static_cast<T *>(dq),
@@ -586,7 +594,7 @@ int kv_cache_write(const KvCacheArgs &c, const void *k, const void *v, long long
         const long long rows = static_cast<long long>(tokens) * 2 * c.kv_heads;
         auto launch = [&](auto n) -> int {
           constexpr int kRows = decltype(n)::value;
-          const unsigned blocks = blocks_for((rows + kRows - 1) / kRows, kLanes);
+          const unsigned blocks = blocks_for((static_cast<long long>(tokens) + kRows - 1) / kRows * 2 * c.kv_heads, kLanes);
           if (!blocks) return cudaErrorInvalidValue;
           kv_write_kernel<T, C, kLanes, kRows><<<blocks, kThreads, 0, s>>>(
               cache, static_cast<const T *>(k), static_cast<const T *>(v), k_token, k_head, v_token, v_head, slots,
@@ -613,7 +621,7 @@ int kv_cache_read(const KvCacheArgs &c, void *k_out, void *v_out, const void *sl
         const long long rows = static_cast<long long>(tokens) * 2 * c.kv_heads;
         auto launch = [&](auto n) -> int {
           constexpr int kRows = decltype(n)::value;
-          const unsigned blocks = blocks_for((rows + kRows - 1) / kRows, kLanes);
+          const unsigned blocks = blocks_for((static_cast<long long>(tokens) + kRows - 1) / kRows * 2 * c.kv_heads, kLanes);
           if (!blocks) return cudaErrorInvalidValue;
           kv_read_kernel<T, C, kLanes, kRows><<<blocks, kThreads, 0, s>>>(cache, static_cast<T *>(k_out),
                                                                          static_cast<T *>(v_out), slots, wide_slots, tokens);

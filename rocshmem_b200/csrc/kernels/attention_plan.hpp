@@ -2,10 +2,10 @@
 // cut into tiles of keys, how the tiles are dealt to blocks, and where a row of the cache lies.
 //
 // The tiles of all (sequence, unit) pairs stand in one line: sequence by sequence, within it unit by unit (a unit is a
-// key head and up to 8 * NT of its query heads), within that tile by tile. Block c takes the tiles [c * per_block,
-// (c + 1) * per_block) of the line, whatever pairs they belong to. A pair that lies in one block is finished there; one
-// that several blocks share leaves a partial result in each of them. A block has at most two such pairs, the first and
-// the last of its range, so two places per block hold all partial results whatever the lengths are.
+// key head and up to 8 * NT of its query heads), within that tile by tile. Warp c of the grid takes the share [c * per,
+// (c + 1) * per) of the line, whatever pairs its tiles belong to. A pair that lies in one share is finished there; one that
+// lies in several leaves a partial result in each of them. A share has at most two such pairs, its first and its last, so
+// two places a share hold all partial results whatever the lengths are.
 #pragma once
 
 #include <cstdint>
@@ -32,20 +32,20 @@ ATTN_HD Span visible(int length, int capacity, int window) {
 
 ATTN_HD int tiles_of(Span s, int tile_keys) { return (s.end - s.first + tile_keys - 1) / tile_keys; }
 
-// Tiles that a block takes: an equal share, but not fewer than `least` (a block's fixed costs).
-ATTN_HD long long per_block(long long total, int blocks, int least) {
-  const long long share = (total + blocks - 1) / blocks;
-  return share < least ? least : share;
+// Tiles of a share: an equal part of the line, but not fewer than `least` (a share's fixed costs).
+ATTN_HD long long per_share(long long total, int shares, int least) {
+  const long long per = (total + shares - 1) / shares;
+  return per < least ? least : per;
 }
 
-// The blocks that share a pair whose tiles are [begin, begin + n), n > 0.
+// The shares that a pair lies in whose tiles are [begin, begin + n), n > 0.
 struct Owners {
   long long first, last;
 };
 ATTN_HD Owners owners(long long begin, int n, long long per) { return Owners{begin / per, (begin + n - 1) / per}; }
 
-// Which of block c's two places holds its partial result of a pair that blocks `o` share: 0 for a pair that an earlier
-// block began, 1 for one that a later block ends.
+// Which of share c's two places holds its partial result of a pair that lies in shares `o`: 0 for a pair that an earlier
+// share began, 1 for one that a later share ends.
 ATTN_HD int place(Owners o, long long c) { return c > o.first ? 0 : 1; }
 
 // Row (of `dim` elements) of position `pos` in a cache [pages, kv_heads, page_size, dim], or -1 where the position is

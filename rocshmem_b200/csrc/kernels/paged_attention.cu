@@ -14,11 +14,11 @@
 // The accumulator layout of S^T differs from the operand layout of P^T by a transposition of 8 x 8 blocks (movmatrix).
 // Both products have a head's values in the same lanes, so rescaling O by the change of the maximum needs no exchange.
 //
-// Each warp streams keys of its own through a ring of stages (cp.async; rows behind the end, of bad pages and before the
-// window arrive as zeros and score -inf), with a running maximum and sum of its own: no barrier until the pair is done. Then the
-// block's four warps are joined through shared memory. Blocks take equal shares of the line of all tiles (attention_plan.hpp); a pair that several
-// blocks share leaves unnormalised partial results, which join_kernel adds in the order of the blocks: results
-// do not depend on which block is done first.
+// Blocks are single warps that work on their own. The line of all tiles (attention_plan.hpp) is dealt to them in equal shares; a
+// warp streams its tiles through a ring of stages (cp.async; rows behind the end, of bad pages and before the window
+// arrive as zeros and score -inf) with a running maximum and sum, and its loads run ahead from one pair into the next. There is no
+// barrier. A pair that lies in several shares leaves unnormalised partial results, which paged_join_kernel adds in the order of the
+// shares: results do not depend on which warp is done first.
 //
 // e4m3 caches: codes become fp16 exactly (cvt), a key's factor multiplies its score, a value's factor its probability.
 #include "attention_common.cuh"
@@ -31,8 +31,6 @@ namespace kernels {
 namespace attn {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kPagedThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Probabilities are at most 1. Where they are rounded to fp16 they are scaled by 2^14 first, so that one down to 2^-28 of
 // the largest keeps all its bits and none above 2^-39 is lost from a long sum; the factor is in the sum as well and cancels.
@@ -90,12 +88,28 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
 }
-// Two e4m3 codes in the low or high half of `w` as two fp16 values (exact).
-__device__ __forceinline__ uint32_t e4m3_lo(uint32_t w) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
+template <bool BF16>
+__device__ __forceinline__ void unpack2(uint32_t w, float &lo, float &hi) {
+  if (BF16) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    lo = f.x, hi = f.y;
+  }
 }
-__device__ __forceinline__ uint32_t e4m3_hi(uint32_t w) { return e4m3_lo(w >> 16); }
+// Four e4m3 codes as two pairs of fp16 values (exact).
+__device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
+}
+// c tanh(x / c) in base 2, with to = 2 log2(e) / c and back = c log2(e): tanh y = 1 - 2 / (exp(2y) + 1). Off by 2^-22 of c, which
+// is what counts in an exponent; tanhf, exact near zero too, cost a fifth of the kernel's time.
+__device__ __forceinline__ float cap2(float x, float to, float back) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(exp2_fast(x * to) + 1.f));
+  return fmaf(-2.f * back, r, back);
+}
 
 // Shared memory and tile sizes of one instantiation. Rows are padded so that the accesses of a fragment fall into
 // different banks: 16 bytes for 16-bit rows (ldmatrix), for e4m3 32 bytes a key row (8 bytes a lane from four rows) and 16 a value row
@@ -103,26 +117,22 @@ __device__ __forceinline__ uint32_t e4m3_hi(uint32_t w) { return e4m3_lo(w >> 16
 template <int D, int NT, int MODE>
 struct Shape {
   static constexpr int kElem = MODE == MODE_E4M3 ? 1 : 2;
-  static constexpr int kKeys = D * kElem <= 128 ? 32 : 16;  // keys a warp takes a step
-  static constexpr int kTileKeys = kWarps * kKeys;
+  static constexpr int kKeys = MODE == MODE_E4M3 && D <= 128 ? 32 : 16;  // keys a warp takes a step
   static constexpr int kRowBytes = D * kElem;
   static constexpr int kPitchK = kRowBytes + (MODE == MODE_E4M3 ? (D == 96 ? 0 : 32) : 16);
   static constexpr int kPitchV = kRowBytes + 16;
   static constexpr int kScales = MODE == MODE_E4M3 ? 2 * kKeys * 4 : 0;
-  static constexpr int kStage = kKeys * (kPitchK + kPitchV) + kScales;  // one warp's stage
+  static constexpr int kStage = kKeys * (kPitchK + kPitchV) + kScales + 16;  // one warp's stage; its last word: which rows are seen
   static constexpr int kHeads = 8 * NT;
-  // Joining the warps: their maxima and sums, and their accumulators a half of the rows of O^T at a time.
-  static constexpr int kStats = 3 * kWarps * kHeads;
-  static constexpr int kMerge = (kStats + kWarps * (D / 2) * kHeads) * 4;
-  static constexpr int kFixed = kMerge + 16 * kWarps * 4 + 64;
-  // Two blocks an SM if three stages or more fit for both, else one block; at most six stages.
-  static constexpr int kFitTwo = (113 * 1024 - kFixed) / (kWarps * kStage);
-  static constexpr int kFitOne = (226 * 1024 - kFixed) / (kWarps * kStage);
-  static constexpr int kBlocks = kFitTwo >= 3 ? 2 : 1;
-  static constexpr int kFit = kBlocks == 2 ? kFitTwo : kFitOne;
+  static constexpr int kFrags = D / 16 * NT;               // of O^T, four values a lane
+  static constexpr int kPart = kFrags * 128 + 2 * kHeads;  // floats of a partial result: O^T, maxima (base 2), sums
+  // As many blocks as registers allow, with as many stages as then fit: bytes on their way, and warps to issue between them.
+  static constexpr int kBlocks = D == 256 ? (MODE == MODE_E4M3 ? 8 : 6) : D == 128 || (NT == 2 && D == 96) ? 8
+                                 : NT == 1 && D == 64 && MODE == MODE_E4M3 ? 16 : 12;
+  static constexpr int kFit = (227 * 1024 / kBlocks - 1024) / kStage;
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
-  static constexpr int kSmem = kFixed + kStages * kWarps * kStage;
-  static_assert(kStages >= 3 && kStages <= 16 && kPitchK % 16 == 0 && kPitchV % 16 == 0 && kStage % 16 == 0, "alignment");
+  static constexpr int kSmem = kStages * kStage;
+  static_assert(kStages >= 2 && kPitchK % 16 == 0 && kPitchV % 16 == 0 && kStage % 16 == 0, "alignment");
 };
 
 struct Params {
@@ -138,12 +148,12 @@ struct Params {
   void *out;
   float *lse;
   int q_bf16, out_f32;
-  float *partial;     // [blocks][2][kHeads][D + 2]: unnormalised O, then maximum (base 2) and sum
-  long long *bases;   // [batch + 2]: a sequence's first tile; then the total, then tiles per block
+  float *partial;     // [shares][2][kPart]
+  long long *bases;   // [batch + 1]: a sequence's first tile; then the tiles of a share
   int blocks, least;
 };
 
-// Walks the tiles of a block's range in order.
+// Walks the tiles of a warp's share in order.
 struct Cursor {
   int b, unit, tile, n, first, end;
   int left;  // tiles that remain, this one included
@@ -172,133 +182,144 @@ __device__ __forceinline__ void advance(Cursor &c, const Params &p, int tile_key
   } while (c.n == 0);
 }
 
+// Which element of its head row r (0 - 15) of block d of O^T is. e4m3: see where the value rows are read.
+template <int D, int MODE>
+__device__ __forceinline__ int element(int d, int r) {
+  if (MODE != MODE_E4M3) return 16 * d + r;
+  const int of_lane = 2 * d + r / 8, group = r % 8;
+  return D <= 128 ? group * (D / 8) + of_lane : of_lane / 16 * 128 + group * 16 + of_lane % 16;
+}
+
+__device__ __forceinline__ void store_out(const Params &p, long long at, float x) {
+  if (p.out_f32) static_cast<float *>(p.out)[at] = x;
+  else if (p.q_bf16) store1(static_cast<__nv_bfloat16 *>(p.out) + at, x);
+  else store1(static_cast<__half *>(p.out) + at, x);
+}
+
 template <int D, int NT, int MODE>
-__global__ void __launch_bounds__(kPagedThreads, Shape<D, NT, MODE>::kBlocks) paged_kernel(const Params p) {
+__global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(const Params p) {
   using S = Shape<D, NT, MODE>;
   constexpr bool kBf16 = MODE == MODE_BF16;
   constexpr int kKeys = S::kKeys, MT = kKeys / 16, DK = D / 16;
-  extern __shared__ __align__(16) char smem[];
-  float *stats = reinterpret_cast<float *>(smem + S::kStages * kWarps * S::kStage);
-  float *merge = stats + S::kStats;
-  uint32_t *masks = reinterpret_cast<uint32_t *>(merge + kWarps * (D / 2) * S::kHeads);  // [stage][warp]
-  long long *scan = reinterpret_cast<long long *>(masks + 16 * kWarps);                  // 8 words
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
+  extern __shared__ __align__(16) char ring[];
+  const int lane = threadIdx.x, g = lane / 4, t = lane % 4;
   const int units = p.kv_heads * p.chunks;
 
-  // ---- this block's range of the line of tiles ----
-  // Threads take neighbouring sequences, `per_thread` each; a scan over the threads gives each one its first tile.
-  const int per_thread = (p.batch + kPagedThreads - 1) / kPagedThreads;
-  const int b_lo = min(tid * per_thread, p.batch), b_hi = min(b_lo + per_thread, p.batch);
+  // ---- the line of tiles ----
+  // Lanes take neighbouring sequences, `per_lane` each; a scan over the lanes gives each one its first tile.
+  const int per_lane = (p.batch + 31) / 32, b_lo = min(lane * per_lane, p.batch), b_hi = min(b_lo + per_lane, p.batch);
+  auto tiles_at = [&](int b) { return static_cast<long long>(tiles_of(visible(p.lengths[b], p.capacity, p.window), kKeys)) * units; };
   long long mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += tiles_of(visible(p.lengths[b], p.capacity, p.window), S::kTileKeys);
-  mine *= units;
+  for (int b = b_lo; b < b_hi; ++b) mine += tiles_at(b);
   long long upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long v = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += v;
   }
-  if (lane == 31) scan[warp] = upto;
-  __syncthreads();
-  long long total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) upto += scan[w];
-    total += scan[w];
-  }
-  const long long per = per_block(total, p.blocks, p.least);
+  const long long total = __shfl_sync(0xffffffffu, upto, 31), per = per_share(total, p.blocks, p.least);
+  // The join may be set up from here on; it waits for the end of this grid before it reads.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // The lane whose sequences hold the share's first tile finds the sequence. Block 0 writes down all first tiles for the
+  // join; a sequence that sees nothing gets its result here.
   const long long t0 = per * blockIdx.x, t1 = min(total, t0 + per);
-  // The thread whose sequences hold tile t0 finds the sequence; block 0 writes down all first tiles for the join, and a
-  // sequence that sees nothing gets its result here.
-  {
+  const bool holds = t0 < t1 && t0 >= upto - mine && t0 < upto;
+  int first_b = 0;
+  long long into = 0;
+  if (holds || blockIdx.x == 0) {
     long long at = upto - mine;
     for (int b = b_lo; b < b_hi; ++b) {
-      const int n = tiles_of(visible(p.lengths[b], p.capacity, p.window), S::kTileKeys);
-      if (t0 < t1 && t0 >= at && t0 < at + static_cast<long long>(n) * units) {
-        scan[4] = b;
-        scan[5] = t0 - at;
+      const long long n = tiles_at(b);
+      if (t0 >= at && t0 < at + n) {
+        first_b = b;
+        into = t0 - at;
       }
       if (blockIdx.x == 0) p.bases[b] = at;
-      at += static_cast<long long>(n) * units;
+      at += n;
     }
-    if (blockIdx.x == 0 && tid == 0) {
-      p.bases[p.batch] = total;
-      p.bases[p.batch + 1] = per;
-    }
+    if (blockIdx.x == 0 && lane == 0) p.bases[p.batch] = per;
   }
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
     const Span s = visible(p.lengths[b], p.capacity, p.window);
     if (s.end > s.first) continue;
-    for (int i = tid; i < p.heads * D; i += kPagedThreads) {
-      const long long at = static_cast<long long>(b) * p.heads * D + i;
-      if (p.out_f32) static_cast<float *>(p.out)[at] = 0.f;
-      else static_cast<uint16_t *>(p.out)[at] = 0;
-    }
+    for (int i = lane; i < p.heads * D; i += 32) store_out(p, static_cast<long long>(b) * p.heads * D + i, 0.f);
     if (p.lse != nullptr) {
-      for (int i = tid; i < p.heads; i += kPagedThreads) p.lse[static_cast<long long>(b) * p.heads + i] = -INFINITY;
+      for (int i = lane; i < p.heads; i += 32) p.lse[static_cast<long long>(b) * p.heads + i] = -INFINITY;
     }
   }
-  __syncthreads();
-  if (t0 >= t1) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    return;
-  }
+  if (t0 >= t1) return;
+  const int from = __ffs(__ballot_sync(0xffffffffu, holds)) - 1;
   Cursor cur;
-  cur.b = static_cast<int>(scan[4]);
-  enter(cur, p, S::kTileKeys);
-  cur.unit = static_cast<int>(scan[5] / cur.n);
-  cur.tile = static_cast<int>(scan[5] % cur.n);
+  cur.b = __shfl_sync(0xffffffffu, first_b, from);
+  into = __shfl_sync(0xffffffffu, into, from);
+  enter(cur, p, kKeys);
+  cur.unit = static_cast<int>(into / cur.n);
+  cur.tile = static_cast<int>(into - static_cast<long long>(cur.unit) * cur.n);
   cur.left = static_cast<int>(t1 - t0);
   Cursor ahead = cur;
 
   // ---- loads: `ahead` runs kStages - 1 tiles before `cur`; a tile's page is looked up one step before its rows are ----
-  char *const stages = smem + warp * S::kStage;  // a stage of all four warps is kWarps * kStage bytes
-  auto look_up = [&](const Cursor &c) -> int {
-    if (c.left <= 0) return -1;
-    const int pos = c.first + c.tile * S::kTileKeys + warp * kKeys + lane;
-    if ((kKeys < 32 && lane >= kKeys) || pos >= c.end) return -1;
-    return page_row(p.table[c.b * p.table_stride + (pos >> p.shift)], p.pages, pos, p.shift, p.kv_heads, c.unit / p.chunks);
+  const uint32_t stages = smem_addr(ring);
+  struct Next {
+    int page, pos, head;  // of the lane's key; pos < 0: none
   };
-  auto load = [&](int stage, int row) {
-    char *k_s = stages + stage * kWarps * S::kStage, *v_s = k_s + kKeys * S::kPitchK;
+  auto look_up = [&](const Cursor &c) -> Next {
+    const int pos = c.first + c.tile * kKeys + lane;
+    if (c.left <= 0 || (kKeys < 32 && lane >= kKeys) || pos >= c.end) return Next{0, -1, 0};
+    return Next{p.table[c.b * p.table_stride + (pos >> p.shift)], pos, c.unit / p.chunks};
+  };
+  // A row is kChunks pieces of 16 bytes. Where whole rows make up a warp's copy, a lane has the same piece of every
+  // kEach-th row, and all its addresses are one register and constants.
+  constexpr unsigned kChunks = S::kRowBytes / 16, kCopies = kKeys * kChunks / 32;
+  static_assert(kKeys * kChunks % 32 == 0, "whole warps");
+  constexpr bool kEven = 32 % kChunks == 0;
+  constexpr unsigned kEach = kEven ? 32 / kChunks : 1;
+  const unsigned my_row = kEven ? lane / kChunks : 0, my_piece = kEven ? lane % kChunks : 0;
+  const char *const my_k = p.k + my_piece * 16, *const my_v = p.v + my_piece * 16;
+  const uint32_t my_to = stages + my_row * S::kPitchK + my_piece * 16;
+  const uint32_t my_to_v = stages + kKeys * S::kPitchK + my_row * S::kPitchV + my_piece * 16;
+  auto load = [&](int stage, const Next &key) {
+    const int row = key.pos < 0 ? -1 : page_row(key.page, p.pages, key.pos, p.shift, p.kv_heads, key.head);
     const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
-    if (lane == 0) masks[stage * kWarps + warp] = mask;
-    constexpr int kChunks = S::kRowBytes / 16;
-    constexpr int kCopies = kKeys * kChunks / 32;
-    static_assert(kKeys * kChunks % 32 == 0, "whole warps");
+    const uint32_t at_stage = stage * S::kStage;
+    if (lane == 0) *reinterpret_cast<uint32_t *>(ring + at_stage + S::kStage - 16) = mask;
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const int at = i * 32 + lane, r = at / kChunks, c = at % kChunks;
+    for (unsigned i = 0; i < kCopies; ++i) {
+      const unsigned at = i * 32 + lane;
+      const unsigned r = kEven ? i * kEach + my_row : at / kChunks, c = kEven ? 0 : at % kChunks;
       const int from = __shfl_sync(0xffffffffu, row, r);
-      const long long off = from < 0 ? 0 : static_cast<long long>(from) * S::kRowBytes + c * 16;
       const uint32_t bytes = from < 0 ? 0 : 16;
-      copy16(smem_addr(k_s + r * S::kPitchK + c * 16), p.k + off, bytes);
-      copy16(smem_addr(v_s + r * S::kPitchV + c * 16), p.v + off, bytes);
+      const unsigned long long off = static_cast<unsigned long long>(static_cast<uint32_t>(max(from, 0))) * S::kRowBytes;
+      const uint32_t to_k = kEven ? i * kEach * S::kPitchK : r * S::kPitchK + c * 16;
+      const uint32_t to_v = kEven ? i * kEach * S::kPitchV : r * S::kPitchV + c * 16;
+      copy16(my_to + at_stage + to_k, my_k + off + c * 16, bytes);
+      copy16(my_to_v + at_stage + to_v, my_v + off + c * 16, bytes);
     }
     if constexpr (MODE == MODE_E4M3) {
-      float *s = reinterpret_cast<float *>(v_s + kKeys * S::kPitchV);
+      const uint32_t to = stages + at_stage + kKeys * (S::kPitchK + S::kPitchV) + 4 * lane;
       if constexpr (kKeys == 32) {
-        copy4(smem_addr(s + lane), p.k_scale + max(row, 0), row < 0 ? 0 : 4);
-        copy4(smem_addr(s + kKeys + lane), p.v_scale + max(row, 0), row < 0 ? 0 : 4);
+        copy4(to, p.k_scale + max(row, 0), row < 0 ? 0 : 4);
+        copy4(to + 4 * kKeys, p.v_scale + max(row, 0), row < 0 ? 0 : 4);
       } else {
         const int from = __shfl_sync(0xffffffffu, row, lane % 16);
-        copy4(smem_addr(s + lane), (lane < 16 ? p.k_scale : p.v_scale) + max(from, 0), from < 0 ? 0 : 4);
+        copy4(to, (lane < 16 ? p.k_scale : p.v_scale) + max(from, 0), from < 0 ? 0 : 4);
       }
     }
   };
-  int next_row = look_up(ahead);
+  Next next = look_up(ahead);
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) {
     if (ahead.left > 0) {
-      load(i, next_row);
-      advance(ahead, p, S::kTileKeys);
-      next_row = look_up(ahead);
+      load(i, next);
+      advance(ahead, p, kKeys);
+      next = look_up(ahead);
     }
     copies_commit();
   }
   int stage = 0, load_stage = S::kStages - 1;
 
   // ---- pairs ----
+  const float cap_to = 2.f * kLog2e / p.softcap, cap_back = p.softcap * kLog2e;
   const int k_lane = (lane % 16) * S::kPitchK + (lane / 16) * 16;                       // ldmatrix: 16 keys x 16 elements
   const int v_lane = ((lane / 16) * 8 + lane % 8) * S::kPitchV + (lane / 8 % 2) * 16;   // transposed
   while (cur.left > 0) {
@@ -365,17 +386,19 @@ __global__ void __launch_bounds__(kPagedThreads, Shape<D, NT, MODE>::kBlocks) pa
       copies_wait<S::kStages - 2>();
       __syncwarp();
       if (ahead.left > 0) {
-        load(load_stage, next_row);
-        advance(ahead, p, S::kTileKeys);
-        next_row = look_up(ahead);
+        load(load_stage, next);
+        advance(ahead, p, kKeys);
+        next = look_up(ahead);
       }
       copies_commit();
       load_stage = load_stage + 1 == S::kStages ? 0 : load_stage + 1;
 
-      const char *k_s = stages + stage * kWarps * S::kStage, *v_s = k_s + kKeys * S::kPitchK;
+      const char *k_s = ring + stage * S::kStage, *v_s = k_s + kKeys * S::kPitchK;
+      const uint32_t k_a = stages + stage * S::kStage + k_lane;
+      const uint32_t v_a = stages + stage * S::kStage + kKeys * S::kPitchK + v_lane;
       const float *f_s = reinterpret_cast<const float *>(v_s + kKeys * S::kPitchV);
-      const uint32_t mask = masks[stage * kWarps + warp];
-      if (mask != 0) {  // a warp may have no key in a pair's last tile
+      const uint32_t mask = *reinterpret_cast<const uint32_t *>(k_s + S::kStage - 16);
+      {
         // S^T
         float s[MT][NT][4] = {};
         if constexpr (MODE != MODE_E4M3) {
@@ -384,7 +407,7 @@ __global__ void __launch_bounds__(kPagedThreads, Shape<D, NT, MODE>::kBlocks) pa
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
               uint32_t a[4];
-              ldmatrix4(a, smem_addr(k_s) + i * 16 * S::kPitchK + k_lane + kk * 32);
+              ldmatrix4(a, k_a + i * 16 * S::kPitchK + kk * 32);
 #pragma unroll
               for (int j = 0; j < NT; ++j) mma<kBf16>(s[i][j], a, qf[j][kk][0], qf[j][kk][1]);
             }
@@ -397,8 +420,11 @@ __global__ void __launch_bounds__(kPagedThreads, Shape<D, NT, MODE>::kBlocks) pa
               const char *at = k_s + (16 * i + g) * S::kPitchK + 32 * ss + 8 * t;
               const uint2 lo = *reinterpret_cast<const uint2 *>(at);
               const uint2 hi = *reinterpret_cast<const uint2 *>(at + 8 * S::kPitchK);
-              const uint32_t a0[4] = {e4m3_lo(lo.x), e4m3_lo(hi.x), e4m3_hi(lo.x), e4m3_hi(hi.x)};
-              const uint32_t a1[4] = {e4m3_lo(lo.y), e4m3_lo(hi.y), e4m3_hi(lo.y), e4m3_hi(hi.y)};
+              uint32_t a0[4], a1[4];
+              e4m3_pairs(lo.x, a0[0], a0[2]);
+              e4m3_pairs(hi.x, a0[1], a0[3]);
+              e4m3_pairs(lo.y, a1[0], a1[2]);
+              e4m3_pairs(hi.y, a1[1], a1[3]);
 #pragma unroll
               for (int j = 0; j < NT; ++j) {
                 mma<false>(s[i][j], a0, qf[j][2 * ss][0], qf[j][2 * ss][1]);
@@ -428,7 +454,7 @@ __global__ void __launch_bounds__(kPagedThreads, Shape<D, NT, MODE>::kBlocks) pa
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 float x = s[i][j][2 * r + c] * q_scale[j][c] * f;
-                if (p.softcap > 0.f) x = p.softcap * kLog2e * tanhf(x / p.softcap);
+                if (p.softcap > 0.f) x = cap2(x, cap_to, cap_back);
                 x = seen ? x : -INFINITY;
                 s[i][j][2 * r + c] = x;
                 top[j][c] = fmaxf(top[j][c], x);
@@ -482,8 +508,9 @@ __global__ void __launch_bounds__(kPagedThreads, Shape<D, NT, MODE>::kBlocks) pa
           }
         }
         if constexpr (MODE == MODE_E4M3) v_unit = 1.f / cv;
-        // P^T
-        uint32_t pf[MT][NT][2];
+        // P^T, as a value rounded to the operand's type and the rounded rest: of one part alone the rounding of
+        // bf16 (2^-8) or fp16 (2^-11) would be as large as that of the result.
+        uint32_t pf[MT][NT][2], pr[MT][NT][2];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
 #pragma unroll
@@ -498,7 +525,11 @@ __global__ void __launch_bounds__(kPagedThreads, Shape<D, NT, MODE>::kBlocks) pa
                 l[j][c] += x[c];
                 if constexpr (MODE == MODE_E4M3) x[c] *= v_factor[i][r] * v_unit;
               }
-              pf[i][j][r] = transpose8x8(pack2<kBf16>(x[0], x[1]));
+              const uint32_t top2 = pack2<kBf16>(x[0], x[1]);
+              pf[i][j][r] = transpose8x8(top2);
+              float y[2];
+              unpack2<kBf16>(top2, y[0], y[1]);
+              pr[i][j][r] = transpose8x8(pack2<kBf16>(x[0] - y[0], x[1] - y[1]));
             }
           }
         }
@@ -509,9 +540,12 @@ __global__ void __launch_bounds__(kPagedThreads, Shape<D, NT, MODE>::kBlocks) pa
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
               uint32_t a[4];
-              ldmatrix4_trans(a, smem_addr(v_s) + i * 16 * S::kPitchV + v_lane + d * 32);
+              ldmatrix4_trans(a, v_a + i * 16 * S::kPitchV + d * 32);
 #pragma unroll
-              for (int j = 0; j < NT; ++j) mma<kBf16>(o[d][j], a, pf[i][j][0], pf[i][j][1]);
+              for (int j = 0; j < NT; ++j) {
+                mma<kBf16>(o[d][j], a, pf[i][j][0], pf[i][j][1]);
+                mma<kBf16>(o[d][j], a, pr[i][j][0], pr[i][j][1]);
+              }
             }
           }
         } else {
@@ -541,12 +575,17 @@ __global__ void __launch_bounds__(kPagedThreads, Shape<D, NT, MODE>::kBlocks) pa
             for (int x = 0; x < kWords; ++x) {
               const uint32_t u0 = __byte_perm(w[0][x], w[1][x], 0x5140), u1 = __byte_perm(w[0][x], w[1][x], 0x7362);
               const uint32_t u2 = __byte_perm(w[2][x], w[3][x], 0x5140), u3 = __byte_perm(w[2][x], w[3][x], 0x7362);
-              const uint32_t a0[4] = {e4m3_lo(u0), e4m3_hi(u0), e4m3_lo(u2), e4m3_hi(u2)};
-              const uint32_t a1[4] = {e4m3_lo(u1), e4m3_hi(u1), e4m3_lo(u3), e4m3_hi(u3)};
+              uint32_t a0[4], a1[4];
+              e4m3_pairs(u0, a0[0], a0[1]);
+              e4m3_pairs(u2, a0[2], a0[3]);
+              e4m3_pairs(u1, a1[0], a1[1]);
+              e4m3_pairs(u3, a1[2], a1[3]);
 #pragma unroll
               for (int j = 0; j < NT; ++j) {
                 mma<false>(o[2 * x][j], a0, pf[i][j][0], pf[i][j][1]);
                 mma<false>(o[2 * x + 1][j], a1, pf[i][j][0], pf[i][j][1]);
+                mma<false>(o[2 * x][j], a0, pr[i][j][0], pr[i][j][1]);
+                mma<false>(o[2 * x + 1][j], a1, pr[i][j][0], pr[i][j][1]);
               }
             }
           }
@@ -556,183 +595,211 @@ __global__ void __launch_bounds__(kPagedThreads, Shape<D, NT, MODE>::kBlocks) pa
       __syncwarp();  // all lanes are done with this stage before the next round refills it
       const int tile = cur.tile + 1;
       ends = tile == cur.n;
-      advance(cur, p, S::kTileKeys);
+      advance(cur, p, kKeys);
       if (ends || cur.left <= 0) break;
     }
 
-    // ---- the pair's (or piece's) result of this block: the warps' results joined ----
+    // ---- the result of the pair, or of this warp's part of it ----
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], d);
-        if (g == 0) {
-          stats[warp * S::kHeads + 8 * j + 2 * t + c] = m[j][c];
-          stats[(kWarps + warp) * S::kHeads + 8 * j + 2 * t + c] = l[j][c];
-        }
       }
     }
-    __syncthreads();
-    float factor[NT][2];
+    if (!(begins && ends)) {
+      // Fragments as they lie in the lanes; the join knows which element is where.
+      float *part = p.partial + (static_cast<long long>(blockIdx.x) * 2 + (begins ? 1 : 0)) * S::kPart;
+#pragma unroll
+      for (int d = 0; d < DK; ++d) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float f = MODE == MODE_E4M3 ? cv : 1.f;
+          reinterpret_cast<float4 *>(part)[(d * NT + j) * 32 + lane] =
+              make_float4(o[d][j][0] * f, o[d][j][1] * f, o[d][j][2] * f, o[d][j][3] * f);
+        }
+      }
+      if (g == 0) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          *reinterpret_cast<float2 *>(part + S::kFrags * 128 + 8 * j + 2 * t) = make_float2(m[j][0], m[j][1]);
+          *reinterpret_cast<float2 *>(part + S::kFrags * 128 + S::kHeads + 8 * j + 2 * t) = make_float2(l[j][0], l[j][1]);
+        }
+      }
+      continue;
+    }
+    const long long row0 = static_cast<long long>(b) * p.heads + h0;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
+      float inv[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int col = 8 * j + 2 * t + c;
-        float top = stats[col], sum = 0.f;
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, stats[w * S::kHeads + col]);
-        const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          sum = fmaf(exp2_fast(stats[w * S::kHeads + col] - base), stats[(kWarps + w) * S::kHeads + col], sum);
-        }
-        factor[j][c] = exp2_fast(m[j][c] - base) * (MODE == MODE_E4M3 ? cv : 1.f);
-        if (warp == 0 && g == 0) {
-          // For the writers below, in the place of warp-wise values that nobody else reads.
-          stats[2 * kWarps * S::kHeads + col] = top;
-          stats[(2 * kWarps + 1) * S::kHeads + col] = sum;
-        }
+        const bool none = m[j][c] == -INFINITY && l[j][c] == 0.f;
+        inv[c] = none ? 0.f : (MODE == MODE_E4M3 ? cv : 1.f) / l[j][c];
+        if (g == 0 && p.lse != nullptr && col < n_heads) p.lse[row0 + col] = none ? -INFINITY : m[j][c] * kLn2 + logf(l[j][c]);
       }
-    }
-    const bool whole = begins && ends;
-    float *part = p.partial + (static_cast<long long>(blockIdx.x) * 2 + (begins ? 1 : 0)) * S::kHeads * (D + 2);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      // Rows [half * D / 2, + D / 2) of O^T in the order of the fragments, as [warp][head][D / 2].
-#pragma unroll
-      for (int dd = 0; dd < DK / 2; ++dd) {
-        const int d = half * (DK / 2) + dd;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
+      for (int d = 0; d < DK; ++d) {
+        if (p.out_f32) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            // 16-bit: rows 16 dd + g and + 8. e4m3: the lane's elements 2 dd and 2 dd + 1.
             const int col = 8 * j + 2 * t + c % 2;
-            const int row = 16 * dd + 8 * (c / 2) + g;
-            merge[(warp * S::kHeads + col) * (D / 2) + row] = o[d][j][c] * factor[j][c % 2];
+            if (col < n_heads) {
+              static_cast<float *>(p.out)[(row0 + col) * D + element<D, MODE>(d, 8 * (c / 2) + g)] = o[d][j][c] * inv[c % 2];
+            }
+          }
+        } else if constexpr (MODE == MODE_E4M3) {
+          // A lane's rows g and g + 8 are neighbouring elements.
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int col = 8 * j + 2 * t + c;
+            const float x = o[d][j][c] * inv[c], y = o[d][j][2 + c] * inv[c];
+            if (col < n_heads) {
+              *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + (row0 + col) * D + element<D, MODE>(d, g)) =
+                  p.q_bf16 ? pack2<true>(x, y) : pack2<false>(x, y);
+            }
+          }
+        } else {
+          // Transposed, a lane has two neighbouring elements of head g.
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t w = transpose8x8(pack2<kBf16>(o[d][j][2 * r] * inv[0], o[d][j][2 * r + 1] * inv[1]));
+            if (8 * j + g < n_heads) {
+              *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + (row0 + 8 * j + g) * D + 16 * d + 8 * r + 2 * t) = w;
+            }
           }
         }
       }
-      __syncthreads();
-      for (int i = tid; i < n_heads * (D / 2); i += kPagedThreads) {
-        const int col = i / (D / 2), at = i % (D / 2);
-        float x = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) x += merge[(w * S::kHeads + col) * (D / 2) + at];
-        int e;  // which element of the head this row of O^T is
-        if constexpr (MODE != MODE_E4M3) {
-          e = half * (D / 2) + at;
-        } else {
-          const int of_lane = 2 * (half * (DK / 2) + at / 16) + at % 16 / 8, group = at % 8;
-          e = D <= 128 ? group * (D / 8) + of_lane : of_lane / 16 * 128 + group * 16 + of_lane % 16;
-        }
-        if (whole) {
-          const float sum = stats[(2 * kWarps + 1) * S::kHeads + col];
-          x = stats[2 * kWarps * S::kHeads + col] == -INFINITY && sum == 0.f ? 0.f : x / sum;
-          const long long to = (static_cast<long long>(b) * p.heads + h0 + col) * D + e;
-          if (p.out_f32) static_cast<float *>(p.out)[to] = x;
-          else if (p.q_bf16) store1(static_cast<__nv_bfloat16 *>(p.out) + to, x);
-          else store1(static_cast<__half *>(p.out) + to, x);
-        } else {
-          part[col * (D + 2) + e] = x;
-        }
-      }
-      __syncthreads();
     }
-    if (tid < n_heads) {
-      const float top = stats[2 * kWarps * S::kHeads + tid], sum = stats[(2 * kWarps + 1) * S::kHeads + tid];
-      if (!whole) {
-        part[tid * (D + 2) + D] = top;
-        part[tid * (D + 2) + D + 1] = sum;
-      } else if (p.lse != nullptr) {
-        p.lse[static_cast<long long>(b) * p.heads + h0 + tid] =
-            top == -INFINITY && sum == 0.f ? -INFINITY : top * kLn2 + logf(sum);
-      }
-    }
-    __syncthreads();
   }
   copies_wait<0>();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// Adds the partial results of the pairs that several blocks share, in the order of the blocks. A block has one head of one
-// pair; its groups of D / 2 threads take the pieces in turn, two elements a thread.
-template <int D, int HEADS>
-__global__ void __launch_bounds__(256) paged_join_kernel(const Params p, int tile_keys) {
-  constexpr int kLanes = D / 2, kGroups = 256 / kLanes;
-  __shared__ float2 sums[kGroups][kLanes];
-  __shared__ float tops[kGroups], totals[kGroups];
+constexpr int join_threads(int groups) { return groups > 8 ? 32 * groups : 256; }
+
+// Adds the partial results of the pairs that several warps share, in the order of the shares. A thread has the four values
+// that a lane had of one fragment; a block GROUPS sets of such threads, which take the parts in turn.
+template <int D, int NT, int MODE, int GROUPS>
+__global__ void __launch_bounds__(join_threads(GROUPS)) paged_join_kernel(const Params p) {
+  using S = Shape<D, NT, MODE>;
+  constexpr int kLanes = join_threads(GROUPS) / GROUPS, kAhead = 4;
+  __shared__ float4 s_o[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? kLanes : 1], s_ml[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? kLanes : 1];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int units = p.kv_heads * p.chunks;
-  const int col = blockIdx.x % HEADS, unit = blockIdx.x / HEADS % units, b = blockIdx.x / (HEADS * units);
-  const int kv = unit / p.chunks, head = kv * p.group + unit % p.chunks * HEADS + col;
-  if (head >= (kv + 1) * p.group) return;
-  const int n = tiles_of(visible(p.lengths[b], p.capacity, p.window), tile_keys);
+  const int units = p.kv_heads * p.chunks, unit = blockIdx.x % units, b = blockIdx.x / units;
+  const int n = tiles_of(visible(p.lengths[b], p.capacity, p.window), S::kKeys);
   if (n == 0) return;
-  const long long per = p.bases[p.batch + 1], begin = p.bases[b] + static_cast<long long>(unit) * n;
-  const Owners own = owners(begin, n, per);
+  const Owners own = owners(p.bases[b] + static_cast<long long>(unit) * n, n, p.bases[p.batch]);
   if (own.first == own.last) return;
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-  float2 acc = make_float2(0.f, 0.f);
-  float top = -INFINITY, total = 0.f;
-  if (group < kGroups) {
-    for (long long c = own.first + group; c <= own.last; c += kGroups) {
-      const float *part = p.partial + ((c * 2 + place(own, c)) * HEADS + col) * (D + 2);
-      const float2 x = *reinterpret_cast<const float2 *>(part + 2 * lane);
-      const float m = part[D], s = part[D + 1];
-      const float now = fmaxf(top, m), base = now == -INFINITY ? 0.f : now;
-      const float keep = exp2_fast(top - base), add = exp2_fast(m - base);
-      acc.x = fmaf(x.x, add, acc.x * keep);
-      acc.y = fmaf(x.y, add, acc.y * keep);
-      total = fmaf(s, add, total * keep);
-      top = now;
+  const int group = threadIdx.x / kLanes, at = blockIdx.y * kLanes + threadIdx.x % kLanes;
+  const int frag = at / 32, lane = at % 32, d = frag / NT, j = frag % NT, g = lane / 4, t = lane % 4;
+  const bool has = frag < S::kFrags;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float2 top = make_float2(-INFINITY, -INFINITY), sum = make_float2(0.f, 0.f);
+  auto add = [&](const float4 &x, const float2 &m, const float2 &l) {
+    const float2 now = make_float2(fmaxf(top.x, m.x), fmaxf(top.y, m.y));
+    const float bx = now.x == -INFINITY ? 0.f : now.x, by = now.y == -INFINITY ? 0.f : now.y;
+    const float kx = exp2_fast(top.x - bx), ky = exp2_fast(top.y - by), ax = exp2_fast(m.x - bx), ay = exp2_fast(m.y - by);
+    acc.x = fmaf(x.x, ax, acc.x * kx);
+    acc.y = fmaf(x.y, ay, acc.y * ky);
+    acc.z = fmaf(x.z, ax, acc.z * kx);
+    acc.w = fmaf(x.w, ay, acc.w * ky);
+    sum.x = fmaf(l.x, ax, sum.x * kx);
+    sum.y = fmaf(l.y, ay, sum.y * ky);
+    top = now;
+  };
+  if (has) {
+    for (long long c0 = own.first + group; c0 <= own.last; c0 += kAhead * GROUPS) {
+      float4 x[kAhead];
+      float2 m[kAhead], l[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const long long c = c0 + i * GROUPS;
+        if (c > own.last) break;
+        const float *part = p.partial + (c * 2 + place(own, c)) * S::kPart;
+        x[i] = reinterpret_cast<const float4 *>(part)[at];
+        m[i] = *reinterpret_cast<const float2 *>(part + S::kFrags * 128 + 8 * j + 2 * t);
+        l[i] = *reinterpret_cast<const float2 *>(part + S::kFrags * 128 + S::kHeads + 8 * j + 2 * t);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (c0 + i * GROUPS > own.last) break;
+        add(x[i], m[i], l[i]);
+      }
     }
-    sums[group][lane] = acc;
-    if (lane == 0) tops[group] = top, totals[group] = total;
   }
-  __syncthreads();
-  if (threadIdx.x >= kLanes) return;
-  float all = tops[0];
+  if constexpr (GROUPS > 1) {
+    const int at_s = threadIdx.x % kLanes;
+    s_o[group][at_s] = acc;
+    s_ml[group][at_s] = make_float4(top.x, top.y, sum.x, sum.y);
+    __syncthreads();
+    if (group != 0) return;
+#pragma unroll 8
+    for (int i = 1; i < GROUPS; ++i) {
+      const float4 ml = s_ml[i][at_s];
+      add(s_o[i][at_s], make_float2(ml.x, ml.y), make_float2(ml.z, ml.w));
+    }
+  }
+  if (!has) return;
+  const int kv = unit / p.chunks, h0 = kv * p.group + unit % p.chunks * S::kHeads, n_heads = min(S::kHeads, (kv + 1) * p.group - h0);
+  const long long row0 = static_cast<long long>(b) * p.heads + h0;
+  const float v[4] = {acc.x, acc.y, acc.z, acc.w}, tops[2] = {top.x, top.y}, sums[2] = {sum.x, sum.y};
 #pragma unroll
-  for (int i = 1; i < kGroups; ++i) all = fmaxf(all, tops[i]);
-  const float base = all == -INFINITY ? 0.f : all;
-  acc = make_float2(0.f, 0.f);
-  total = 0.f;
-#pragma unroll
-  for (int i = 0; i < kGroups; ++i) {
-    const float f = exp2_fast(tops[i] - base);
-    acc.x = fmaf(sums[i][lane].x, f, acc.x);
-    acc.y = fmaf(sums[i][lane].y, f, acc.y);
-    total = fmaf(totals[i], f, total);
-  }
-  const bool none = all == -INFINITY && total == 0.f;
-  const float inv = none ? 0.f : 1.f / total;
-  const long long to = (static_cast<long long>(b) * p.heads + head) * D + 2 * lane;
-  if (p.out_f32) {
-    *reinterpret_cast<float2 *>(static_cast<float *>(p.out) + to) = make_float2(acc.x * inv, acc.y * inv);
-  } else {
-    const uint32_t w = p.q_bf16 ? pack2<true>(acc.x * inv, acc.y * inv) : pack2<false>(acc.x * inv, acc.y * inv);
-    *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + to) = w;
-  }
-  if (lane == 0 && p.lse != nullptr) {
-    p.lse[static_cast<long long>(b) * p.heads + head] = none ? -INFINITY : all * kLn2 + logf(total);
+  for (int c = 0; c < 2; ++c) {
+    const int col = 8 * j + 2 * t + c;
+    if (col >= n_heads) continue;
+    const bool none = tops[c] == -INFINITY && sums[c] == 0.f;
+    const float inv = none ? 0.f : 1.f / sums[c];
+    store_out(p, (row0 + col) * D + element<D, MODE>(d, g), v[c] * inv);
+    store_out(p, (row0 + col) * D + element<D, MODE>(d, g + 8), v[2 + c] * inv);
+    if (d == 0 && g == 0 && p.lse != nullptr) p.lse[row0 + col] = none ? -INFINITY : tops[c] * kLn2 + logf(sums[c]);
   }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
-constexpr int kMostBlocksPerSm = 2;
-// Tiles that a block takes at least: below that its fixed costs weigh more than the loads that another SM would take over.
-constexpr int kLeastTiles = 2;
+// Keys that a share has at least: below that its fixed costs weigh more than the loads that another warp would take over.
+constexpr int kLeastKeys = 32;
 
 int heads_per_unit(int group, int dim) { return group > 8 && dim <= 128 ? 16 : 8; }
+
+// Calls f with the Shape of a call.
+template <typename F>
+auto with_shape(int dim, int group, int cache_type, F f) {
+  auto heads = [&](auto d, auto mode) {
+    constexpr int D = decltype(d)::value, M = decltype(mode)::value;
+    if constexpr (D <= 128) {
+      if (heads_per_unit(group, D) == 16) return f(Int<D>{}, Int<2>{}, Int<M>{});
+    }
+    return f(Int<D>{}, Int<1>{}, Int<M>{});
+  };
+  auto modes = [&](auto d) {
+    return cache_type == ATTN_BF16 ? heads(d, Int<MODE_BF16>{}) : cache_type == ATTN_F16 ? heads(d, Int<MODE_F16>{})
+                                                                                       : heads(d, Int<MODE_E4M3>{});
+  };
+  return dim == 64 ? modes(Int<64>{}) : dim == 96 ? modes(Int<96>{}) : dim == 128 ? modes(Int<128>{}) : modes(Int<256>{});
+}
+
+template <int D, int NT, int MODE, int GROUPS>
+int launch_join(const Params &p, cudaStream_t s) {
+  // The join's blocks may be set up while the warps above are running; they wait for them before they read.
+  constexpr int kLanes = join_threads(GROUPS) / GROUPS;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.kv_heads * p.chunks, (Shape<D, NT, MODE>::kFrags * 32 + kLanes - 1) / kLanes);
+  cfg.blockDim = dim3(join_threads(GROUPS));
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, NT, MODE, GROUPS>, p);
+}
 
 template <int D, int NT, int MODE>
 int launch(Params p, cudaStream_t s) {
   using S = Shape<D, NT, MODE>;
-  p.blocks = device_sm_count() * S::kBlocks;
   auto kernel = paged_kernel<D, NT, MODE>;
   // The attribute belongs to the device's context: set once for each device.
   static std::atomic<uint64_t> ready{0};
@@ -745,50 +812,28 @@ int launch(Params p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  kernel<<<p.blocks, kPagedThreads, S::kSmem, s>>>(p);
+  p.blocks = device_sm_count() * S::kBlocks;
+  p.least = kLeastKeys / S::kKeys;
+  kernel<<<p.blocks, 32, S::kSmem, s>>>(p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  if (p.capacity <= S::kTileKeys) return 0;  // no pair has two tiles: nothing to join
-  // The join's blocks may start while the last blocks above are running; they wait for them before they read.
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.kv_heads * p.chunks * S::kHeads);
-  cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, S::kHeads>, p, static_cast<int>(S::kTileKeys));
+  // The lengths are on the device: what counts is the most that they can be.
+  const int longest = p.window > 0 ? std::min(p.window, p.capacity) : p.capacity;
+  if (longest <= S::kKeys) return 0;  // no pair has two tiles: nothing to join
+  // Few pairs, many parts of each: sets of threads share the parts. Many pairs: few parts of each.
+  const int pairs = p.batch * p.kv_heads * p.chunks, shares = p.blocks;
+  if (pairs > shares / 8) return launch_join<D, NT, MODE, 1>(p, s);
+  return pairs > shares / 48 ? launch_join<D, NT, MODE, 8>(p, s) : launch_join<D, NT, MODE, 32>(p, s);
 }
 
-template <int D, int MODE>
-int launch_heads(const Params &p, cudaStream_t s) {
-  if constexpr (D <= 128) {
-    if (heads_per_unit(p.group, D) == 16) return launch<D, 2, MODE>(p, s);
-  }
-  return launch<D, 1, MODE>(p, s);
-}
-
-template <int D>
-int launch_mode(const Params &p, int cache_type, cudaStream_t s) {
-  switch (cache_type) {
-    case ATTN_BF16: return launch_heads<D, MODE_BF16>(p, s);
-    case ATTN_F16: return launch_heads<D, MODE_F16>(p, s);
-    case ATTN_E4M3: return launch_heads<D, MODE_E4M3>(p, s);
-    default: return cudaErrorInvalidValue;
-  }
-}
+// The first tiles, in whole 16 bytes.
+size_t base_bytes(int batch) { return (static_cast<size_t>(batch) + 1 + 1) / 2 * 16; }
 
 bool refuse_sizes(const KvCacheArgs &c, int batch, int heads) {
   return (c.dim != 64 && c.dim != 96 && c.dim != 128 && c.dim != 256) || batch < 0 || heads < 1 || c.kv_heads < 1 ||
          heads % c.kv_heads || c.pages < 0 || c.page_shift < 0 || c.page_shift > 20 ||
          (static_cast<long long>(c.pages) * c.kv_heads << c.page_shift) > 0x7fffffffll ||
-         static_cast<long long>(batch) * c.kv_heads * ((heads / c.kv_heads + 7) / 8) * 16 > 0x7fffffffll;
-}
-
-size_t partial_floats(const KvCacheArgs &c, int heads, int blocks) {
-  return static_cast<size_t>(blocks) * 2 * heads_per_unit(heads / c.kv_heads, c.dim) * (c.dim + 2);
+         static_cast<long long>(batch) * c.kv_heads * ((heads / c.kv_heads + 7) / 8) > 0x7fffffffll;
 }
 
 }  // namespace
@@ -798,7 +843,10 @@ using namespace attn;
 
 size_t paged_attention_workspace(const KvCacheArgs &c, int batch, int heads) {
   if (refuse_sizes(c, batch, heads)) return 0;
-  return (static_cast<size_t>(batch) + 2) * 8 + partial_floats(c, heads, device_sm_count() * kMostBlocksPerSm) * 4;
+  return with_shape(c.dim, heads / c.kv_heads, c.type, [&](auto d, auto nt, auto mode) -> size_t {
+    using S = Shape<decltype(d)::value, decltype(nt)::value, decltype(mode)::value>;
+    return base_bytes(batch) + static_cast<size_t>(device_sm_count()) * S::kBlocks * 2 * S::kPart * 4;
+  });
 }
 
 int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *workspace, size_t workspace_bytes,
@@ -830,6 +878,10 @@ int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *wor
   p.pages = c.pages;
   p.shift = c.page_shift;
   p.capacity = a.max_pages << c.page_shift;
+  // A warp counts its tiles (of 16 keys at least) in 32 bits.
+  if (static_cast<long long>(a.batch) * c.kv_heads * p.chunks > 0x7fffffffll * device_sm_count() / (p.capacity / 16 + 1)) {
+    return cudaErrorInvalidValue;
+  }
   p.window = a.window;
   p.scale = a.scale;
   p.softcap = a.softcap;
@@ -838,19 +890,10 @@ int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *wor
   p.q_bf16 = a.q_type == ATTN_BF16;
   p.out_f32 = a.out_type == ATTN_F32;
   p.bases = static_cast<long long *>(workspace);
-  p.partial = reinterpret_cast<float *>(p.bases + a.batch + 2);
-  p.least = kLeastTiles;
-  // A block counts its tiles in 32 bits (tiles have at least 64 keys).
-  if (static_cast<long long>(a.batch) * c.kv_heads * p.chunks > 0x7fffffffll * device_sm_count() / (p.capacity / 64 + 1)) {
-    return cudaErrorInvalidValue;
-  }
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  switch (c.dim) {
-    case 64: return launch_mode<64>(p, c.type, s);
-    case 96: return launch_mode<96>(p, c.type, s);
-    case 128: return launch_mode<128>(p, c.type, s);
-    default: return launch_mode<256>(p, c.type, s);
-  }
+  p.partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + base_bytes(a.batch));
+  return with_shape(c.dim, p.group, c.type, [&](auto d, auto nt, auto mode) -> int {
+    return launch<decltype(d)::value, decltype(nt)::value, decltype(mode)::value>(p, static_cast<cudaStream_t>(stream));
+  });
 }
 
 }  // namespace kernels

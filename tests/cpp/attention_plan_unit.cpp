@@ -1,5 +1,5 @@
 // The arithmetic of paged attention's split (attention_plan.hpp) on the CPU: every tile of every pair is taken by exactly
-// one block, in order; partial results of one pair lie in places of their own; rows of pages that do not exist are refused.
+// one share, in order; partial results of one pair lie in places of their own; rows of pages that do not exist are refused.
 #include <cstdio>
 #include <cstdlib>
 #include <map>
@@ -51,23 +51,23 @@ void check_rows() {
   CHECK(slot_row((1ll << 32) - 1, 1ll << 32, 4, 2, 1) == (((1ll << 28) - 1) * 2 + 1) * 16 + 15);
 }
 
-void check_split(const std::vector<int> &lengths, int capacity, int window, int units, int blocks, int least, int tile) {
+void check_split(const std::vector<int> &lengths, int capacity, int window, int units, int shares, int least, int tile) {
   std::vector<long long> bases;
   long long total = 0;
   for (int n : lengths) {
     bases.push_back(total);
     total += static_cast<long long>(tiles_of(visible(n, capacity, window), tile)) * units;
   }
-  const long long per = per_block(total, blocks, least);
-  CHECK(per >= least && per * blocks >= total);
+  const long long per = per_share(total, shares, least);
+  CHECK(per >= least && per * shares >= total);
   std::set<std::pair<long long, int>> places;
   for (size_t b = 0; b < lengths.size(); ++b) {
     const int n = tiles_of(visible(lengths[b], capacity, window), tile);
     for (int u = 0; u < units && n > 0; ++u) {
       const long long begin = bases[b] + static_cast<long long>(u) * n;
       const Owners own = owners(begin, n, per);
-      CHECK(own.first >= 0 && own.first <= own.last && own.last < blocks);
-      // The tiles that the owners' ranges hold of this pair are all of them.
+      CHECK(own.first >= 0 && own.first <= own.last && own.last < shares);
+      // The tiles that the owners' shares hold of this pair are all of them.
       long long seen = 0;
       for (long long c = own.first; c <= own.last; ++c) {
         const long long lo = c * per > begin ? c * per : begin;
@@ -75,7 +75,7 @@ void check_split(const std::vector<int> &lengths, int capacity, int window, int 
         CHECK(hi > lo);
         seen += hi - lo;
         if (own.first == own.last) continue;
-        // What the block itself goes by: it begins the pair (place 1) or finds it begun (place 0).
+        // What the warp itself goes by: it begins the pair (place 1) or finds it begun (place 0).
         CHECK(place(own, c) == (lo == begin ? 1 : 0));
         CHECK(places.insert({c, place(own, c)}).second);
       }
@@ -95,9 +95,10 @@ int main() {
     const int most = 1 << (rng() % 14);
     for (int &n : lengths) n = rng() % 5 == 0 ? 0 : static_cast<int>(rng() % (most + 2)) - 1;
     const int window = rng() % 3 == 0 ? 1 + rng() % most : 0;
-    check_split(lengths, most, window, 1 + rng() % 9, 1 + rng() % 300, 1 + rng() % 4, rng() % 2 ? 64 : 128);
+    check_split(lengths, most, window, 1 + rng() % 9, 1 + rng() % 300, 1 + rng() % 6, rng() % 2 ? 16 : 32);
   }
-  check_split({1000000, 0, 1}, 1 << 20, 0, 1, 296, 2, 64);
+  check_split({1000000, 0, 1}, 1 << 20, 0, 1, 1184, 4, 16);
+  check_split({0, 0}, 64, 0, 3, 1184, 4, 16);
   std::puts("ok");
   return 0;
 }
