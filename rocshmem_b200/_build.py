@@ -1,9 +1,11 @@
 """In-tree build of the native code for sm_100a.
 
-Three artefacts, all inside the package directory so that they travel with a source snapshot:
+Four artefacts, all inside the package directory so that they travel with a source snapshot:
 
 * ``lib/librocshmem_b200.so`` - host runtime (C++) plus every CUDA kernel of the library;
 * ``_C.<abi>.so``             - pybind11 bindings, linked against the library;
+* ``_A.<abi>.so``             - bindings of the attention operators, which take torch tensors (the only part that is
+                                compiled against torch's headers);
 * ``_testk.<abi>.so``         - kernels of the functional test-suite that exercise the device API
                                 from user code, linked against the same library (built on demand).
 
@@ -38,7 +40,8 @@ LIB_CU = [
     "kernels/gemm_kernels.cu", "kernels/fused_kernels.cu", "kernels/no_alloc.cu", "kernels/moe_kernels.cu", "kernels/gemm_fp8.cu",
     "kernels/attention_kernels.cu", "kernels/paged_attention.cu",
 ]
-BIND_CPP = ["bindings.cpp", "kernels/bindings_ep.cpp", "kernels/bindings_gemm.cpp", "kernels/bindings_attention.cpp"]
+BIND_CPP = ["bindings.cpp", "kernels/bindings_ep.cpp", "kernels/bindings_gemm.cpp"]
+TORCH_CPP = ["kernels/bindings_attention.cpp"]
 
 
 def _cuda_home() -> str:
@@ -54,6 +57,11 @@ def _cuda_home() -> str:
 def _pybind_include() -> str:
     import pybind11
     return pybind11.get_include()
+
+
+def _torch_dir() -> Path:
+    from importlib.util import find_spec
+    return Path(find_spec("torch").origin).resolve().parent
 
 
 def _rel(p: Path) -> str:
@@ -87,7 +95,7 @@ def _ninja_text(with_tests: bool) -> str:
         "  command = $nvcc -shared -o $out $in -lpthread -ldl -lrt",
         "rule linkext",
         f"  command = $nvcc -shared -o $out $in -L{_rel(LIBDIR)} -lrocshmem_b200 "
-        "-Xlinker -rpath -Xlinker '$$ORIGIN/lib' -lpthread -ldl -lrt",
+        "-Xlinker -rpath -Xlinker '$$ORIGIN/lib' -lpthread -ldl -lrt $libs",
     ]
     lib_objs = []
     for src in RUNTIME_CPP:
@@ -114,7 +122,17 @@ def _ninja_text(with_tests: bool) -> str:
         bind_objs.append(obj)
     ext = _rel(PKG / f"_C{EXT}")
     lines.append(f"build {ext}: linkext {' '.join(bind_objs)} | {lib}")
-    targets = [ext]
+    torch_dir = _torch_dir()
+    torch_objs = []
+    for src in TORCH_CPP:
+        obj = _rel(OBJ / (src.replace("/", "_") + ".o"))
+        lines.append(f"build {obj}: cxx {_rel(CSRC / src)}")
+        lines.append(f"  extra = $pyflags -isystem {torch_dir}/include -isystem {torch_dir}/include/torch/csrc/api/include")
+        torch_objs.append(obj)
+    ext_a = _rel(PKG / f"_A{EXT}")
+    lines.append(f"build {ext_a}: linkext {' '.join(torch_objs)} | {lib}")
+    lines.append(f"  libs = -L{torch_dir}/lib -lc10 -lc10_cuda -ltorch_cpu -ltorch_python -Xlinker -rpath -Xlinker {torch_dir}/lib")
+    targets = [ext, ext_a]
     tests_src = PKG.parent / "tests" / "csrc" / "test_kernels.cu"
     if with_tests and tests_src.exists():
         obj = _rel(OBJ / "tests_test_kernels.cu.o")
@@ -153,7 +171,7 @@ def build(with_tests: bool = True, verbose: bool = False, jobs: int | None = Non
 
 
 def is_built(with_tests: bool = False) -> bool:
-    ok = (LIBDIR / "librocshmem_b200.so").exists() and (PKG / f"_C{EXT}").exists()
+    ok = all(f.exists() for f in (LIBDIR / "librocshmem_b200.so", PKG / f"_C{EXT}", PKG / f"_A{EXT}"))
     if with_tests:
         ok = ok and (PKG / f"_testk{EXT}").exists()
     return ok

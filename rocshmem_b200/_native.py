@@ -9,6 +9,7 @@ import os
 from . import _build
 
 _C = None
+_A = None
 _testk = None
 
 
@@ -20,6 +21,16 @@ def load():
             _build.build(with_tests=False)
         _C = importlib.import_module("rocshmem_b200._C")
     return _C
+
+
+def load_attention():
+    """Return the extension with the attention operators (its functions take torch tensors)."""
+    global _A
+    if _A is None:
+        load()
+        importlib.import_module("torch")     # whose libraries the extension resolves its symbols from
+        _A = importlib.import_module("rocshmem_b200._A")
+    return _A
 
 
 def load_test_kernels():

@@ -7,12 +7,8 @@
 #include <cstring>
 
 #include "kernels/kernels.hpp"
-// Bindings of the MoE, GEMM and attention kernels live beside those kernels' launchers.
-namespace rocshmem { namespace kernels {
-void bind_ep(pybind11::module_ &m);
-void bind_gemm(pybind11::module_ &m);
-void bind_attention(pybind11::module_ &m);
-} }
+// Bindings of the MoE and GEMM kernels live beside those kernels' launchers.
+namespace rocshmem { namespace kernels { void bind_ep(pybind11::module_ &m); void bind_gemm(pybind11::module_ &m); } }
 #include "rocshmem/coalesce.h"
 #include "rocshmem/rocshmem_debug.hpp"
 #include "rocshmem/rocshmem_host.h"
@@ -283,7 +279,6 @@ PYBIND11_MODULE(_C, m) {
   m.def("coll_blocks_for", [](size_t bytes) { return kernels::coll_blocks_for(bytes); });
   kernels::bind_ep(m);
   kernels::bind_gemm(m);
-  kernels::bind_attention(m);
 
   // ---- proxy -----------------------------------------------------------------------------------------------
   m.def("proxy_running", [] {
