@@ -75,7 +75,39 @@ __device__ __forceinline__ void unpack8(const Raw8<e4m3> &r, float (&x)[8]) {
   }
 }
 
+// Four consecutive elements in 32 bits.
+template <typename T>
+struct Raw4 {
+  uint2 a;
+};
+template <>
+struct Raw4<float> {
+  float4 a;
+};
+template <typename T>
+__device__ __forceinline__ Raw4<T> load4(const T *p) {
+  return *reinterpret_cast<const Raw4<T> *>(p);
+}
+__device__ __forceinline__ void unpack4(const Raw4<float> &r, float *x) { x[0] = r.a.x, x[1] = r.a.y, x[2] = r.a.z, x[3] = r.a.w; }
+__device__ __forceinline__ void unpack4(const Raw4<__nv_bfloat16> &r, float *x) {
+  x[0] = __uint_as_float(r.a.x << 16), x[1] = __uint_as_float(r.a.x & 0xffff0000u);
+  x[2] = __uint_as_float(r.a.y << 16), x[3] = __uint_as_float(r.a.y & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack4(const Raw4<__half> &r, float *x) {
+  const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&r.a.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&r.a.y));
+  x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
+}
+
 // One rounding to the nearest value of the type, ties to even.
+__device__ __forceinline__ void store4(float *p, const float *x) { *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]); }
+__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float *x) {
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
+  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+}
+__device__ __forceinline__ void store4(__half *p, const float *x) {
+  const __half2 lo = __floats2half2_rn(x[0], x[1]), hi = __floats2half2_rn(x[2], x[3]);
+  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+}
 __device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
   float4 *v = reinterpret_cast<float4 *>(p);
   v[0] = make_float4(x[0], x[1], x[2], x[3]);

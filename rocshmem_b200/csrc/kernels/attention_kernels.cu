@@ -2,7 +2,7 @@
 // backward), writes into and reads from a paged cache, the join of partial attention results.
 //
 // All of them are bound by memory. A row (one head of one token) lies in 8, 16 or 32 neighbouring lanes, eight elements a
-// lane: 16-byte accesses for 16-bit types, sums over a row by shuffles, nothing in shared memory but the weights' gradients.
+// lane; sums over a row by shuffles, nothing in shared memory but the weights' gradients.
 // No counterpart exists in the reference.
 #include "attention_common.cuh"
 
@@ -20,47 +20,6 @@ __device__ __forceinline__ long long load_index(const void *p, int wide, int i) 
 
 // ---- norm and rotation -------------------------------------------------------------------------------------------
 
-// What a lane needs of its token's position: cosines and sines for its eight elements.
-struct Angles {
-  float c[8], s[8];
-};
-
-// `lane` is the lane's place in its row, elements [8 lane, 8 lane + 8). Pairs are (i, i + rotary / 2), or (2i, 2i + 1).
-__device__ __forceinline__ void load_angles(Angles &a, const float *row, int rotary, int lane, bool interleaved) {
-  const int half = rotary / 2;
-  if (interleaved) {
-    const float4 c = *reinterpret_cast<const float4 *>(row + 4 * lane);
-    const float4 s = *reinterpret_cast<const float4 *>(row + half + 4 * lane);
-    const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      a.c[i] = cv[i / 2];
-      a.s[i] = i % 2 ? sv[i / 2] : -sv[i / 2];
-    }
-  } else {
-    const int at = 8 * lane < half ? 8 * lane : 8 * lane - half;
-    const float sign = 8 * lane < half ? -1.f : 1.f;
-    unpack8(load8(row + at), a.c);
-    unpack8(load8(row + half + at), a.s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a.s[i] *= sign;
-  }
-}
-
-// The other element of each of the lane's pairs. All lanes of the warp call it.
-template <int LANES>
-__device__ __forceinline__ void partners(const float (&y)[8], float (&other)[8], int rotary, int lane, bool interleaved) {
-  if (interleaved) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) other[i] = y[i ^ 1];
-  } else {
-    const int half = rotary / 16;  // in lanes
-    const int from = lane < half ? lane + half : lane < 2 * half ? lane - half : lane;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, y[i], from, LANES);
-  }
-}
-
 template <typename T, typename W>
 struct NormRope {
   const T *q, *k;
@@ -69,195 +28,234 @@ struct NormRope {
   const void *positions;
   const float *table;
   int tokens, q_heads, k_heads, dim, rotary, table_rows;
-  float eps;
-  int interleaved, wide_positions;
+  float eps, inv_dim;
+  int wide_positions;
 };
 
-// Rows are taken ROWS at a time: an item is ROWS heads of one token, whose loads are all issued before the first is used
-// and which share the token's angles.
-template <typename T, typename W, int LANES, int ROWS>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRope<T, W> a, T *q_out, T *k_out) {
+// The eight elements of a lane: two pieces of four, so that both elements of each of its pairs are among them and the rotation needs
+// no exchange. Pairs (i, i + rotary / 2): the first lanes have a piece of either half, those behind eight neighbours that
+// are not rotated. Pairs (2i, 2i + 1): eight neighbours.
+template <bool INTERLEAVED>
+struct Place {
+  int e0, e1;
+  bool in_row, rotated;
+  __device__ __forceinline__ Place(int lane, int dim, int rotary) {
+    in_row = 8 * lane < dim;
+    rotated = 8 * lane < rotary;
+    const bool halves = !INTERLEAVED && rotated;
+    e0 = halves ? 4 * lane : 8 * lane;
+    e1 = halves ? rotary / 2 + 4 * lane : 8 * lane + 4;
+  }
+};
+
+template <typename T>
+struct RawRow {
+  Raw4<T> a, b;
+};
+template <typename T>
+__device__ __forceinline__ void unpack(const RawRow<T> &r, float (&x)[8]) {
+  unpack4(r.a, x);
+  unpack4(r.b, x + 4);
+}
+
+// Rotates the lane's four pairs by the angles with cosines c and sines s; BACK: the other way.
+template <bool INTERLEAVED, bool BACK>
+__device__ __forceinline__ void rotate(float (&x)[8], const float (&c)[4], const float (&s)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float &a = x[INTERLEAVED ? 2 * i : i], &b = x[INTERLEAVED ? 2 * i + 1 : 4 + i];
+    const float sn = BACK ? -s[i] : s[i], y = fmaf(-b, sn, a * c[i]);
+    b = fmaf(a, sn, b * c[i]);
+    a = y;
+  }
+}
+
+// ROWS heads of one token that a group of lanes takes at a time, all of queries or all of keys: their loads are issued
+// before the first is used, and they share weights and angles. Items are numbered queries first.
+template <typename T, typename W>
+struct Item {
+  const T *rows;      // of the first head
+  const W *weight;
+  long long head;     // stride
+  long long out;      // first head's row in the contiguous tensors
+  int heads;          // that are left from the first one on
+  bool is_q;
+  unsigned t;
+};
+template <int ROWS, typename T, typename W>
+__device__ __forceinline__ Item<T, W> item_of(const NormRope<T, W> &a, unsigned item) {
+  const unsigned q_chunks = (a.q_heads + ROWS - 1) / ROWS, k_chunks = (a.k_heads + ROWS - 1) / ROWS;
+  Item<T, W> x;
+  x.is_q = item < a.tokens * q_chunks;
+  if (!x.is_q) item -= a.tokens * q_chunks;
+  const unsigned chunks = x.is_q ? q_chunks : k_chunks;
+  x.t = item / chunks;
+  const int h0 = (item - x.t * chunks) * ROWS, heads = x.is_q ? a.q_heads : a.k_heads;
+  x.head = x.is_q ? a.q_head : a.k_head;
+  x.rows = (x.is_q ? a.q : a.k) + x.t * (x.is_q ? a.q_token : a.k_token) + h0 * x.head;
+  x.weight = x.is_q ? a.q_weight : a.k_weight;
+  x.out = static_cast<long long>(x.t) * heads + h0;
+  x.heads = heads - h0;
+  return x;
+}
+
+template <typename T, typename W, int LANES, int ROWS, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRope<T, W> a, unsigned items, T *q_out, T *k_out) {
   const int lane = threadIdx.x % LANES;
-  const int heads = a.q_heads + a.k_heads;
-  const unsigned chunks = (heads + ROWS - 1) / ROWS, items = a.tokens * chunks;
+  const Place<INTERLEAVED> at(lane, a.dim, a.rotary);
   // All lanes of a warp take part in every shuffle: groups past the last item work on it again and store nothing.
   const unsigned mine = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-  const unsigned item = min(mine, items - 1), t = item / chunks;
-  const int h0 = (item - t * chunks) * ROWS;
-  const bool in_row = 8 * lane < a.dim;
-  const long long pos = load_index(a.positions, a.wide_positions, t);
+  const Item<T, W> it = item_of<ROWS>(a, min(mine, items - 1));
+  const long long pos = load_index(a.positions, a.wide_positions, it.t);
   const bool live = pos >= 0, known = pos < a.table_rows;
-
-  Raw8<T> raw[ROWS];
+  RawRow<T> raw[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    const int h = h0 + r;
-    raw[r] = Raw8<T>{};
-    if (live && in_row && h < heads) {
-      raw[r] = load8(h < a.q_heads ? a.q + t * a.q_token + h * a.q_head : a.k + t * a.k_token + (h - a.q_heads) * a.k_head, lane);
+    raw[r] = RawRow<T>{};
+    if (at.in_row && r < it.heads) {
+      const T *row = it.rows + r * it.head;
+      raw[r] = RawRow<T>{load4(row + at.e0), load4(row + at.e1)};
     }
   }
-  Angles ang;
-  const bool rotated = 8 * lane < a.rotary;
-  if (rotated && live && known) {
-    load_angles(ang, a.table + pos * a.rotary, a.rotary, lane, a.interleaved);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ang.c[i] = 1.f, ang.s[i] = 0.f;
+  float w[8] = {}, c[4], s[4];
+  if (at.in_row) {
+    unpack4(load4(it.weight + at.e0), w);
+    unpack4(load4(it.weight + at.e1), w + 4);
   }
-  float wq[8] = {}, wk[8] = {};
-  if (in_row) {
-    unpack8(load8(a.q_weight, lane), wq);
-    unpack8(load8(a.k_weight, lane), wk);
+  const bool turn = at.rotated && live && known;
+  if (turn) {
+    unpack4(load4(a.table + pos * a.rotary + 4 * lane), c);
+    unpack4(load4(a.table + pos * a.rotary + a.rotary / 2 + 4 * lane), s);
   }
+  T *const out = (it.is_q ? q_out : k_out) + it.out * a.dim;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    const int h = h0 + r;
-    float x[8], other[8], sum = 0.f;
-    unpack8(raw[r], x);
+    float x[8], sum = 0.f;
+    unpack(raw[r], x);
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-    sum = group_sum<LANES>(sum);
-    float scale = rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
+    float scale = rsqrtf(fmaf(group_sum<LANES>(sum), a.inv_dim, a.eps));
     if (!known) scale = __int_as_float(0x7fc00000);  // a position without angles: NaN, not a wrong rotation
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= scale * (h < a.q_heads ? wq[i] : wk[i]);
-    partners<LANES>(x, other, a.rotary, lane, a.interleaved);
-    if (rotated) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = fmaf(other[i], ang.s[i], x[i] * ang.c[i]);
-    }
+    for (int i = 0; i < 8; ++i) x[i] *= scale * w[i];
+    if (turn) rotate<INTERLEAVED, false>(x, c, s);
     if (!live) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = 0.f;
     }
-    if (mine < items && in_row && h < heads) {
-      T *to = h < a.q_heads ? q_out + (static_cast<long long>(t) * a.q_heads + h) * a.dim
-                            : k_out + (static_cast<long long>(t) * a.k_heads + (h - a.q_heads)) * a.dim;
-      store8(to + 8 * lane, x);
+    if (mine < items && at.in_row && r < it.heads) {
+      store4(out + r * a.dim + at.e0, x);
+      store4(out + r * a.dim + at.e1, x + 4);
     }
   }
 }
 
 // With g the gradient of the output rotated back, n = x r and a = w g: dx = r (a - n mean(a n)), dw = sum of g n. The norm
-// is computed again (x is read anyway). Each group of lanes keeps the sums of its columns of both weights in registers
-// over all its rows; blocks add theirs up in a fixed order, and norm_rope_weights_kernel adds the blocks' sums, so that
-// the gradients are the same in every run.
-template <typename T, typename W, int LANES, int ROWS>
-__global__ void __launch_bounds__(kThreads) norm_rope_backward_kernel(NormRope<T, W> a, const T *gq, const T *gk, T *dq,
-                                                                      T *dk, float *partial) {
-  extern __shared__ float sums[];  // [groups][2 * dim]
+// is computed again (x is read anyway). Blocks below q_blocks have the queries, the others the keys, in proportion. Each
+// group of lanes keeps the sums of its columns of the weight in registers over all its rows; a block adds those up in a fixed
+// order, and norm_rope_weights_kernel adds the blocks' sums, so that the gradients are the same in every run.
+template <typename T, typename W, int LANES, int ROWS, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads, 3) norm_rope_backward_kernel(NormRope<T, W> a, unsigned q_items, unsigned items,
+                                                                         int q_blocks, const T *gq, const T *gk, T *dq,
+                                                                         T *dk, float *partial) {
+  extern __shared__ float sums[];  // [groups][dim]
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   constexpr int kGroups = kThreads / LANES;
-  const int heads = a.q_heads + a.k_heads;
-  const unsigned chunks = (heads + ROWS - 1) / ROWS, items = a.tokens * chunks;
-  const bool in_row = 8 * lane < a.dim, rotated = 8 * lane < a.rotary;
-  float wq[8] = {}, wk[8] = {}, dwq[8] = {}, dwk[8] = {};
-  if (in_row) {
-    unpack8(load8(a.q_weight, lane), wq);
-    unpack8(load8(a.k_weight, lane), wk);
+  const Place<INTERLEAVED> at(lane, a.dim, a.rotary);
+  const bool is_q = static_cast<int>(blockIdx.x) < q_blocks;
+  const unsigned first = is_q ? 0 : q_items, end = is_q ? q_items : items;
+  const unsigned block = is_q ? blockIdx.x : blockIdx.x - q_blocks, step = (is_q ? q_blocks : gridDim.x - q_blocks) * kGroups;
+  const W *weight = is_q ? a.q_weight : a.k_weight;
+  const T *const grad = is_q ? gq : gk;
+  T *const out = is_q ? dq : dk;
+  float w[8] = {}, dw[8] = {};
+  if (at.in_row) {
+    unpack4(load4(weight + at.e0), w);
+    unpack4(load4(weight + at.e1), w + 4);
   }
-  const unsigned step = gridDim.x * kGroups;
   // The same number of rounds for all groups of a block, for the shuffles.
-  for (unsigned base = blockIdx.x * kGroups; base < items; base += step) {
-    const bool has = base + group < items;
-    const unsigned item = has ? base + group : items - 1, t = item / chunks;
-    const int h0 = (item - t * chunks) * ROWS;
-    const long long pos = load_index(a.positions, a.wide_positions, t);
+  for (unsigned base = first + block * kGroups; base < end; base += step) {
+    const bool has = base + group < end;
+    const Item<T, W> it = item_of<ROWS>(a, has ? base + group : end - 1);
+    const long long pos = load_index(a.positions, a.wide_positions, it.t);
     const bool live = pos >= 0, known = pos < a.table_rows;
-    Raw8<T> raw[ROWS], graw[ROWS];
+    RawRow<T> raw[ROWS], graw[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      const int h = h0 + r;
-      raw[r] = Raw8<T>{};
-      graw[r] = Raw8<T>{};
-      if (has && live && in_row && h < heads) {
-        const bool is_q = h < a.q_heads;
-        raw[r] = load8(is_q ? a.q + t * a.q_token + h * a.q_head : a.k + t * a.k_token + (h - a.q_heads) * a.k_head, lane);
-        graw[r] = load8(is_q ? gq + (static_cast<long long>(t) * a.q_heads + h) * a.dim
-                             : gk + (static_cast<long long>(t) * a.k_heads + (h - a.q_heads)) * a.dim, lane);
+      raw[r] = RawRow<T>{};
+      graw[r] = RawRow<T>{};
+      if (at.in_row && r < it.heads) {
+        const T *row = it.rows + r * it.head, *g = grad + (it.out + r) * a.dim;
+        raw[r] = RawRow<T>{load4(row + at.e0), load4(row + at.e1)};
+        graw[r] = RawRow<T>{load4(g + at.e0), load4(g + at.e1)};
       }
     }
-    Angles ang;
-    if (rotated && live && known) {
-      load_angles(ang, a.table + pos * a.rotary, a.rotary, lane, a.interleaved);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ang.c[i] = 1.f, ang.s[i] = 0.f;
+    float c[4], s[4];
+    const bool turn = at.rotated && live && known;
+    if (turn) {
+      unpack4(load4(a.table + pos * a.rotary + 4 * lane), c);
+      unpack4(load4(a.table + pos * a.rotary + a.rotary / 2 + 4 * lane), s);
     }
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      const int h = h0 + r;
-      const bool is_q = h < a.q_heads;
-      float x[8], g[8], other[8], sum = 0.f, dot = 0.f;
-      unpack8(raw[r], x);
-      unpack8(graw[r], g);
-      partners<LANES>(g, other, a.rotary, lane, a.interleaved);
-      if (rotated) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = fmaf(other[i], -ang.s[i], g[i] * ang.c[i]);  // the inverse rotation
-      }
+      float x[8], g[8], sum = 0.f, dot = 0.f;
+      unpack(raw[r], x);
+      unpack(graw[r], g);
+      if (turn) rotate<INTERLEAVED, true>(g, c, s);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         sum = fmaf(x[i], x[i], sum);
-        dot = fmaf(x[i], g[i] * (is_q ? wq[i] : wk[i]), dot);
+        dot = fmaf(x[i], g[i] * w[i], dot);
       }
       sum = group_sum<LANES>(sum);
       dot = group_sum<LANES>(dot);
-      float scale = rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
+      float scale = rsqrtf(fmaf(sum, a.inv_dim, a.eps));
       if (!known) scale = __int_as_float(0x7fc00000);
-      const float mean = dot * scale / static_cast<float>(a.dim);
-      if (live) {  // a padded token leaves nothing in the weights' gradients, whatever its gradient holds
-        float d[8];
+      const float mean = dot * scale * a.inv_dim;
+      const bool counts = has && live && r < it.heads;  // a padded token leaves nothing in the weights' gradients, whatever its gradient holds
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float n = x[i] * scale;
-          if (is_q) dwq[i] = fmaf(g[i], n, dwq[i]);
-          else dwk[i] = fmaf(g[i], n, dwk[i]);
-          d[i] = scale * (g[i] * (is_q ? wq[i] : wk[i]) - n * mean);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = d[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+      for (int i = 0; i < 8; ++i) {
+        const float n = x[i] * scale;
+        if (counts) dw[i] = fmaf(g[i], n, dw[i]);
+        x[i] = live ? scale * fmaf(-n, mean, g[i] * w[i]) : 0.f;
       }
-      if (has && in_row && h < heads) {
-        T *to = is_q ? dq + (static_cast<long long>(t) * a.q_heads + h) * a.dim
-                     : dk + (static_cast<long long>(t) * a.k_heads + (h - a.q_heads)) * a.dim;
-        store8(to + 8 * lane, x);
+      if (has && at.in_row && r < it.heads) {
+        T *to = out + (it.out + r) * a.dim;
+        store4(to + at.e0, x);
+        store4(to + at.e1, x + 4);
       }
     }
   }
-  if (in_row) {
-    store8(sums + group * 2 * a.dim + 8 * lane, dwq);
-    store8(sums + group * 2 * a.dim + a.dim + 8 * lane, dwk);
+  if (at.in_row) {
+    store4(sums + group * a.dim + at.e0, dw);
+    store4(sums + group * a.dim + at.e1, dw + 4);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * a.dim; i += kThreads) {
+  for (int i = threadIdx.x; i < a.dim; i += kThreads) {
     float v = 0.f;
-    for (int g = 0; g < kGroups; ++g) v += sums[g * 2 * a.dim + i];
-    partial[static_cast<long long>(blockIdx.x) * 2 * a.dim + i] = v;
+    for (int g = 0; g < kGroups; ++g) v += sums[g * a.dim + i];
+    partial[static_cast<long long>(blockIdx.x) * a.dim + i] = v;
   }
 }
 
-// Adds the blocks' sums: a block has 32 columns, its warps take the rows in turn.
+// Adds the blocks' sums: a block has 32 columns of one weight, its warps take the rows in turn.
 template <typename W>
-__global__ void __launch_bounds__(1024) norm_rope_weights_kernel(const float *partial, int rows, int dim, W *dq_weight,
-                                                                 W *dk_weight) {
+__global__ void __launch_bounds__(1024) norm_rope_weights_kernel(const float *partial, int q_rows, int rows, int dim,
+                                                                 W *dq_weight, W *dk_weight) {
   __shared__ float s[32][33];
   const int col = blockIdx.x * 32 + threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int first = blockIdx.y ? q_rows : 0, end = blockIdx.y ? rows : q_rows;
   float v = 0.f;
-  if (col < 2 * dim) {
-    for (int r = warp; r < rows; r += 32) v += partial[static_cast<long long>(r) * 2 * dim + col];
+  if (col < dim) {
+#pragma unroll 4
+    for (int r = first + warp; r < end; r += 32) v += partial[static_cast<long long>(r) * dim + col];
   }
   s[warp][threadIdx.x % 32] = v;
   __syncthreads();
   // Warp w adds the 32 sums of column w.
-  float x = s[threadIdx.x % 32][warp];
-  x = group_sum<32>(x);
+  const float x = group_sum<32>(s[threadIdx.x % 32][warp]);
   const int c = blockIdx.x * 32 + warp;
-  if (threadIdx.x % 32 == 0 && c < 2 * dim) store1(c < dim ? dq_weight + c : dk_weight + (c - dim), x);
+  if (threadIdx.x % 32 == 0 && c < dim) store1((blockIdx.y ? dk_weight : dq_weight) + c, x);
 }
 
 // ---- the paged cache ---------------------------------------------------------------------------------------------
@@ -473,13 +471,19 @@ unsigned blocks_for(long long items, int lanes) {
   return n * per > 0x7fffffffll ? 0u : static_cast<unsigned>(n);
 }
 
-int backward_blocks() { return device_sm_count() * 2; }
+// Groups of lanes that the GPU's SMs hold at once.
+long long groups_at_once(int lanes) { return static_cast<long long>(device_sm_count()) * (2048 / lanes); }
+
+// Items of `rows` heads.
+long long items_of(int tokens, int heads, int rows) { return static_cast<long long>(tokens) * ((heads + rows - 1) / rows); }
+
+int backward_blocks() { return device_sm_count() * 3; }
 
 template <typename T, typename W>
 NormRope<T, W> norm_rope_args(const NormRopeArgs &a) {
   return NormRope<T, W>{static_cast<const T *>(a.q), static_cast<const T *>(a.k), a.q_token, a.q_head, a.k_token, a.k_head,
                         static_cast<const W *>(a.q_weight), static_cast<const W *>(a.k_weight), a.positions, a.table,
-                        a.tokens, a.q_heads, a.k_heads, a.dim, a.rotary, a.table_rows, a.eps, a.interleaved,
+                        a.tokens, a.q_heads, a.k_heads, a.dim, a.rotary, a.table_rows, a.eps, 1.f / static_cast<float>(a.dim),
                         a.wide_positions};
 }
 
@@ -494,8 +498,8 @@ int with_row_and_weight(const NormRopeArgs &a, F f) {
 }
 
 bool refuse(const NormRopeArgs &a) {
-  return bad_rows(a.dim) || a.rotary < 16 || a.rotary > a.dim || a.rotary % 16 || a.tokens < 0 || a.q_heads < 0 ||
-         a.k_heads < 0 || a.q_heads + a.k_heads < 1 || a.table_rows < 1;
+  return bad_rows(a.dim) || a.rotary < 16 || a.rotary > a.dim || a.rotary % 16 || a.tokens < 0 || a.q_heads < 1 ||
+         a.k_heads < 1 || a.table_rows < 1;
 }
 
 template <typename F>
@@ -531,24 +535,25 @@ int qk_norm_rope(const NormRopeArgs &a, void *q_out, void *k_out, void *stream) 
     using W = typename decltype(w)::type;
     return with_lanes(a.dim, [&](auto l) -> int {
       constexpr int kLanes = decltype(l)::value;
-      const auto args = norm_rope_args<T, W>(a);
-      const cudaStream_t s = static_cast<cudaStream_t>(stream);
-      const int heads = a.q_heads + a.k_heads;
-      auto launch = [&](auto rows) -> int {
+      auto launch = [&](auto rows, auto pairs) -> int {
         constexpr int kRows = decltype(rows)::value;
-        const unsigned blocks = blocks_for(static_cast<long long>(a.tokens) * ((heads + kRows - 1) / kRows), kLanes);
+        const long long items = items_of(a.tokens, a.q_heads, kRows) + items_of(a.tokens, a.k_heads, kRows);
+        const unsigned blocks = blocks_for(items, kLanes);
         if (!blocks) return cudaErrorInvalidValue;
-        norm_rope_kernel<T, W, kLanes, kRows><<<blocks, kThreads, 0, s>>>(args, static_cast<T *>(q_out), static_cast<T *>(k_out));
+        norm_rope_kernel<T, W, kLanes, kRows, decltype(pairs)::value != 0>
+            <<<blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(norm_rope_args<T, W>(a), static_cast<unsigned>(items),
+                                                                         static_cast<T *>(q_out), static_cast<T *>(k_out));
         return cudaGetLastError();
       };
       // One row a group while that leaves SMs without work, four rows in flight beyond.
-      const long long groups = static_cast<long long>(device_sm_count()) * (2048 / kLanes);
-      return static_cast<long long>(a.tokens) * heads <= groups ? launch(Int<1>{}) : launch(Int<4>{});
+      const bool few = static_cast<long long>(a.tokens) * (a.q_heads + a.k_heads) <= groups_at_once(kLanes);
+      if (a.interleaved) return few ? launch(Int<1>{}, Int<1>{}) : launch(Int<4>{}, Int<1>{});
+      return few ? launch(Int<1>{}, Int<0>{}) : launch(Int<4>{}, Int<0>{});
     });
   });
 }
 
-size_t qk_norm_rope_workspace(int dim) { return static_cast<size_t>(backward_blocks()) * 2 * static_cast<size_t>(dim); }
+size_t qk_norm_rope_workspace(int dim) { return static_cast<size_t>(backward_blocks()) * static_cast<size_t>(dim); }
 
 int qk_norm_rope_backward(const NormRopeArgs &a, const void *gq, const void *gk, void *dq, void *dk, void *dq_weight,
                           void *dk_weight, float *workspace, void *stream) {
@@ -560,20 +565,23 @@ int qk_norm_rope_backward(const NormRopeArgs &a, const void *gq, const void *gk,
       constexpr int kLanes = decltype(l)::value;
       constexpr int kRows = 2;
       const cudaStream_t s = static_cast<cudaStream_t>(stream);
-      const int heads = a.q_heads + a.k_heads;
-      const long long items = static_cast<long long>(a.tokens) * ((heads + kRows - 1) / kRows);
+      const long long q_items = items_of(a.tokens, a.q_heads, kRows), items = q_items + items_of(a.tokens, a.k_heads, kRows);
       const long long per = kThreads / kLanes;
-      const int blocks = static_cast<int>(std::min<long long>(backward_blocks(), (items + per - 1) / per));
-      if (items > 0x7fffffffll - static_cast<long long>(blocks) * per) return cudaErrorInvalidValue;
-      if (blocks > 0) {
-        norm_rope_backward_kernel<T, W, kLanes, kRows><<<blocks, kThreads, kThreads / kLanes * 2 * a.dim * sizeof(float), s>>>(
-            norm_rope_args<T, W>(a), static_cast<const T *>(gq), static_cast<const T *>(gk), static_cast<T *>(dq),
-            static_cast<T *>(dk), workspace);
-        const cudaError_t e = cudaGetLastError();
-        if (e != cudaSuccess) return e;
-      }
-      norm_rope_weights_kernel<W><<<(2 * a.dim + 31) / 32, 1024, 0, s>>>(workspace, blocks, a.dim, static_cast<W *>(dq_weight),
-                                                                     static_cast<W *>(dk_weight));
+      if (items > 0x7fffffffll - backward_blocks() * per) return cudaErrorInvalidValue;
+      // Blocks in proportion to the items of queries and keys, at least one for either.
+      const int blocks = static_cast<int>(std::max<long long>(2, std::min<long long>(backward_blocks(), (items + per - 1) / per)));
+      const int q_blocks = static_cast<int>(std::min<long long>(std::max<long long>(q_items * blocks / std::max(items, 1ll), 1), blocks - 1));
+      auto launch = [&](auto pairs) -> int {
+        norm_rope_backward_kernel<T, W, kLanes, kRows, decltype(pairs)::value != 0>
+            <<<blocks, kThreads, kThreads / kLanes * a.dim * sizeof(float), s>>>(
+                norm_rope_args<T, W>(a), static_cast<unsigned>(q_items), static_cast<unsigned>(items), q_blocks,
+                static_cast<const T *>(gq), static_cast<const T *>(gk), static_cast<T *>(dq), static_cast<T *>(dk), workspace);
+        return cudaGetLastError();
+      };
+      const int e = a.interleaved ? launch(Int<1>{}) : launch(Int<0>{});
+      if (e != cudaSuccess) return e;
+      norm_rope_weights_kernel<W><<<dim3((a.dim + 31) / 32, 2), 1024, 0, s>>>(
+          workspace, q_blocks, blocks, a.dim, static_cast<W *>(dq_weight), static_cast<W *>(dk_weight));
       return cudaGetLastError();
     });
   });
@@ -601,7 +609,7 @@ int kv_cache_write(const KvCacheArgs &c, const void *k, const void *v, long long
               wide_slots, tokens);
           return cudaGetLastError();
         };
-        return rows <= static_cast<long long>(device_sm_count()) * (2048 / kLanes) ? launch(Int<1>{}) : launch(Int<4>{});
+        return rows <= groups_at_once(kLanes) ? launch(Int<1>{}) : launch(Int<4>{});
       });
     });
   });
@@ -627,7 +635,7 @@ int kv_cache_read(const KvCacheArgs &c, void *k_out, void *v_out, const void *sl
                                                                          static_cast<T *>(v_out), slots, wide_slots, tokens);
           return cudaGetLastError();
         };
-        return rows <= static_cast<long long>(device_sm_count()) * (2048 / kLanes) ? launch(Int<1>{}) : launch(Int<4>{});
+        return rows <= groups_at_once(kLanes) ? launch(Int<1>{}) : launch(Int<4>{});
       });
     });
   });
