@@ -88,26 +88,26 @@ template <typename T>
 __device__ __forceinline__ Raw4<T> load4(const T *p) {
   return *reinterpret_cast<const Raw4<T> *>(p);
 }
-__device__ __forceinline__ void unpack4(const Raw4<float> &r, float *x) { x[0] = r.a.x, x[1] = r.a.y, x[2] = r.a.z, x[3] = r.a.w; }
-__device__ __forceinline__ void unpack4(const Raw4<__nv_bfloat16> &r, float *x) {
-  x[0] = __uint_as_float(r.a.x << 16), x[1] = __uint_as_float(r.a.x & 0xffff0000u);
-  x[2] = __uint_as_float(r.a.y << 16), x[3] = __uint_as_float(r.a.y & 0xffff0000u);
+__device__ __forceinline__ void unpack4(const Raw4<float> &r, float2 *x) { x[0] = make_float2(r.a.x, r.a.y), x[1] = make_float2(r.a.z, r.a.w); }
+__device__ __forceinline__ void unpack4(const Raw4<__nv_bfloat16> &r, float2 *x) {
+  x[0] = make_float2(__uint_as_float(r.a.x << 16), __uint_as_float(r.a.x & 0xffff0000u));
+  x[1] = make_float2(__uint_as_float(r.a.y << 16), __uint_as_float(r.a.y & 0xffff0000u));
 }
-__device__ __forceinline__ void unpack4(const Raw4<__half> &r, float *x) {
-  const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&r.a.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&r.a.y));
-  x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
+__device__ __forceinline__ void unpack4(const Raw4<__half> &r, float2 *x) {
+  x[0] = __half22float2(*reinterpret_cast<const __half2 *>(&r.a.x));
+  x[1] = __half22float2(*reinterpret_cast<const __half2 *>(&r.a.y));
+}
+__device__ __forceinline__ void store4(float *p, const float2 *x) { *reinterpret_cast<float4 *>(p) = make_float4(x[0].x, x[0].y, x[1].x, x[1].y); }
+__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float2 *x) {
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0].x, x[0].y), hi = __floats2bfloat162_rn(x[1].x, x[1].y);
+  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+}
+__device__ __forceinline__ void store4(__half *p, const float2 *x) {
+  const __half2 lo = __floats2half2_rn(x[0].x, x[0].y), hi = __floats2half2_rn(x[1].x, x[1].y);
+  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
 }
 
 // One rounding to the nearest value of the type, ties to even.
-__device__ __forceinline__ void store4(float *p, const float *x) { *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]); }
-__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float *x) {
-  const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
-  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-}
-__device__ __forceinline__ void store4(__half *p, const float *x) {
-  const __half2 lo = __floats2half2_rn(x[0], x[1]), hi = __floats2half2_rn(x[2], x[3]);
-  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-}
 __device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
   float4 *v = reinterpret_cast<float4 *>(p);
   v[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -140,6 +140,20 @@ __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ void store1(float *p, float x) { *p = x; }
 __device__ __forceinline__ void store1(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 __device__ __forceinline__ void store1(__half *p, float x) { *p = __float2half_rn(x); }
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ unsigned long long bits2(float2 a) { return *reinterpret_cast<unsigned long long *>(&a); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return *reinterpret_cast<float2 *>(&r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+  return *reinterpret_cast<float2 *>(&r);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // Sum over the `LANES` neighbouring lanes (a power of two) that hold one row.
 template <int LANES>

@@ -53,99 +53,101 @@ struct RawRow {
   Raw4<T> a, b;
 };
 template <typename T>
-__device__ __forceinline__ void unpack(const RawRow<T> &r, float (&x)[8]) {
+__device__ __forceinline__ void unpack(const RawRow<T> &r, float2 (&x)[4]) {
   unpack4(r.a, x);
-  unpack4(r.b, x + 4);
+  unpack4(r.b, x + 2);
 }
 
-// Rotates the lane's four pairs by the angles with cosines c and sines s; BACK: the other way.
-template <bool INTERLEAVED, bool BACK>
-__device__ __forceinline__ void rotate(float (&x)[8], const float (&c)[4], const float (&s)[4]) {
+// Cosines and sines of the lane's four pairs, as the packed products of rotate() take them.
+template <bool INTERLEAVED>
+struct Turn {
+  float2 c[INTERLEAVED ? 4 : 2], s[INTERLEAVED ? 4 : 2];
+  __device__ __forceinline__ void load(const float *row, int rotary, int lane) {
+    const float4 cv = *reinterpret_cast<const float4 *>(row + 4 * lane), sv = *reinterpret_cast<const float4 *>(row + rotary / 2 + 4 * lane);
+    if constexpr (INTERLEAVED) {
+      c[0] = both(cv.x), c[1] = both(cv.y), c[2] = both(cv.z), c[3] = both(cv.w);
+      s[0] = make_float2(-sv.x, sv.x), s[1] = make_float2(-sv.y, sv.y), s[2] = make_float2(-sv.z, sv.z), s[3] = make_float2(-sv.w, sv.w);
+    } else {
+      c[0] = make_float2(cv.x, cv.y), c[1] = make_float2(cv.z, cv.w);
+      s[0] = make_float2(sv.x, sv.y), s[1] = make_float2(sv.z, sv.w);
+    }
+  }
+};
+
+// Rotates the lane's four pairs; BACK: the other way.
+template <bool BACK, bool INTERLEAVED>
+__device__ __forceinline__ void rotate(float2 (&x)[4], const Turn<INTERLEAVED> &a) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float &a = x[INTERLEAVED ? 2 * i : i], &b = x[INTERLEAVED ? 2 * i + 1 : 4 + i];
-    const float sn = BACK ? -s[i] : s[i], y = fmaf(-b, sn, a * c[i]);
-    b = fmaf(a, sn, b * c[i]);
-    a = y;
+  for (int i = 0; i < (INTERLEAVED ? 4 : 2); ++i) {
+    if constexpr (INTERLEAVED) {  // (u, v) -> (u, v) c + (v, u) (-s, s)
+      const float2 s = BACK ? make_float2(a.s[i].y, a.s[i].x) : a.s[i];
+      x[i] = fma2(make_float2(x[i].y, x[i].x), s, mul2(x[i], a.c[i]));
+    } else {
+      const float2 n = make_float2(-a.s[i].x, -a.s[i].y), s = BACK ? n : a.s[i], ns = BACK ? a.s[i] : n, u = x[i], v = x[2 + i];
+      x[i] = fma2(v, ns, mul2(u, a.c[i]));
+      x[2 + i] = fma2(u, s, mul2(v, a.c[i]));
+    }
   }
 }
 
 // ROWS heads of one token that a group of lanes takes at a time, all of queries or all of keys: their loads are issued
-// before the first is used, and they share weights and angles. Items are numbered queries first.
+// before the first is used, and they share weights and angles.
 template <typename T, typename W>
-struct Item {
-  const T *rows;      // of the first head
+struct Side {
+  const T *x;
   const W *weight;
-  long long head;     // stride
-  long long out;      // first head's row in the contiguous tensors
-  int heads;          // that are left from the first one on
-  bool is_q;
-  unsigned t;
+  long long token, head;
+  int heads;
+  __device__ __forceinline__ Side(const NormRope<T, W> &a, bool is_q)
+      : x(is_q ? a.q : a.k), weight(is_q ? a.q_weight : a.k_weight), token(is_q ? a.q_token : a.k_token),
+        head(is_q ? a.q_head : a.k_head), heads(is_q ? a.q_heads : a.k_heads) {}
 };
-template <int ROWS, typename T, typename W>
-__device__ __forceinline__ Item<T, W> item_of(const NormRope<T, W> &a, unsigned item) {
-  const unsigned q_chunks = (a.q_heads + ROWS - 1) / ROWS, k_chunks = (a.k_heads + ROWS - 1) / ROWS;
-  Item<T, W> x;
-  x.is_q = item < a.tokens * q_chunks;
-  if (!x.is_q) item -= a.tokens * q_chunks;
-  const unsigned chunks = x.is_q ? q_chunks : k_chunks;
-  x.t = item / chunks;
-  const int h0 = (item - x.t * chunks) * ROWS, heads = x.is_q ? a.q_heads : a.k_heads;
-  x.head = x.is_q ? a.q_head : a.k_head;
-  x.rows = (x.is_q ? a.q : a.k) + x.t * (x.is_q ? a.q_token : a.k_token) + h0 * x.head;
-  x.weight = x.is_q ? a.q_weight : a.k_weight;
-  x.out = static_cast<long long>(x.t) * heads + h0;
-  x.heads = heads - h0;
-  return x;
-}
 
 template <typename T, typename W, int LANES, int ROWS, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRope<T, W> a, unsigned items, T *q_out, T *k_out) {
+__global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRope<T, W> a, unsigned q_items, unsigned items, T *q_out,
+                                                             T *k_out) {
   const int lane = threadIdx.x % LANES;
   const Place<INTERLEAVED> at(lane, a.dim, a.rotary);
-  // All lanes of a warp take part in every shuffle: groups past the last item work on it again and store nothing.
+  // All lanes of a warp take part in every shuffle: groups past the last item have no rows.
   const unsigned mine = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-  const Item<T, W> it = item_of<ROWS>(a, min(mine, items - 1));
-  const long long pos = load_index(a.positions, a.wide_positions, it.t);
-  const bool live = pos >= 0, known = pos < a.table_rows;
+  const bool is_q = mine < q_items;
+  const Side<T, W> side(a, is_q);
+  const unsigned item = is_q ? mine : min(mine, items - 1) - q_items, chunks = (side.heads + ROWS - 1) / ROWS, t = item / chunks;
+  const int h0 = (item - t * chunks) * ROWS, left = mine < items && at.in_row ? side.heads - h0 : 0;
+  const long long pos = load_index(a.positions, a.wide_positions, t);
+  const T *const rows = side.x + t * side.token + h0 * side.head;
   RawRow<T> raw[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     raw[r] = RawRow<T>{};
-    if (at.in_row && r < it.heads) {
-      const T *row = it.rows + r * it.head;
-      raw[r] = RawRow<T>{load4(row + at.e0), load4(row + at.e1)};
-    }
+    if (r < left) raw[r] = RawRow<T>{load4(rows + r * side.head + at.e0), load4(rows + r * side.head + at.e1)};
   }
-  float w[8] = {}, c[4], s[4];
+  float2 w[4] = {};
   if (at.in_row) {
-    unpack4(load4(it.weight + at.e0), w);
-    unpack4(load4(it.weight + at.e1), w + 4);
+    unpack4(load4(side.weight + at.e0), w);
+    unpack4(load4(side.weight + at.e1), w + 2);
   }
-  const bool turn = at.rotated && live && known;
-  if (turn) {
-    unpack4(load4(a.table + pos * a.rotary + 4 * lane), c);
-    unpack4(load4(a.table + pos * a.rotary + a.rotary / 2 + 4 * lane), s);
-  }
-  T *const out = (it.is_q ? q_out : k_out) + it.out * a.dim;
+  const bool live = pos >= 0, known = pos < a.table_rows, turn = at.rotated && live && known;
+  Turn<INTERLEAVED> angles;
+  if (turn) angles.load(a.table + pos * a.rotary, a.rotary, lane);
+  // A position without angles: NaN, not a wrong rotation.
+  const float eps = known ? a.eps : __int_as_float(0x7fc00000);
+  T *const out = (is_q ? q_out : k_out) + (static_cast<long long>(t) * side.heads + h0) * a.dim;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    float x[8], sum = 0.f;
+    float2 x[4];
     unpack(raw[r], x);
+    float2 square = mul2(x[0], x[0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-    float scale = rsqrtf(fmaf(group_sum<LANES>(sum), a.inv_dim, a.eps));
-    if (!known) scale = __int_as_float(0x7fc00000);  // a position without angles: NaN, not a wrong rotation
+    for (int i = 1; i < 4; ++i) square = fma2(x[i], x[i], square);
+    const float scale = rsqrtf(fmaf(group_sum<LANES>(square.x + square.y), a.inv_dim, eps));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= scale * w[i];
-    if (turn) rotate<INTERLEAVED, false>(x, c, s);
-    if (!live) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    }
-    if (mine < items && at.in_row && r < it.heads) {
+    for (int i = 0; i < 4; ++i) x[i] = mul2(x[i], mul2(both(scale), w[i]));
+    if (turn) rotate<false>(x, angles);
+    if (!live) x[0] = x[1] = x[2] = x[3] = make_float2(0.f, 0.f);
+    if (r < left) {
       store4(out + r * a.dim + at.e0, x);
-      store4(out + r * a.dim + at.e1, x + 4);
+      store4(out + r * a.dim + at.e1, x + 2);
     }
   }
 }
@@ -163,72 +165,84 @@ __global__ void __launch_bounds__(kThreads, 3) norm_rope_backward_kernel(NormRop
   constexpr int kGroups = kThreads / LANES;
   const Place<INTERLEAVED> at(lane, a.dim, a.rotary);
   const bool is_q = static_cast<int>(blockIdx.x) < q_blocks;
-  const unsigned first = is_q ? 0 : q_items, end = is_q ? q_items : items;
-  const unsigned block = is_q ? blockIdx.x : blockIdx.x - q_blocks, step = (is_q ? q_blocks : gridDim.x - q_blocks) * kGroups;
-  const W *weight = is_q ? a.q_weight : a.k_weight;
+  const Side<T, W> side(a, is_q);
+  const unsigned n_items = is_q ? q_items : items - q_items, block = is_q ? blockIdx.x : blockIdx.x - q_blocks;
+  const unsigned step = (is_q ? q_blocks : gridDim.x - q_blocks) * kGroups, chunks = (side.heads + ROWS - 1) / ROWS;
   const T *const grad = is_q ? gq : gk;
   T *const out = is_q ? dq : dk;
-  float w[8] = {}, dw[8] = {};
+  float2 w[4] = {}, dw[4] = {};
   if (at.in_row) {
-    unpack4(load4(weight + at.e0), w);
-    unpack4(load4(weight + at.e1), w + 4);
+    unpack4(load4(side.weight + at.e0), w);
+    unpack4(load4(side.weight + at.e1), w + 2);
   }
-  // The same number of rounds for all groups of a block, for the shuffles.
-  for (unsigned base = first + block * kGroups; base < end; base += step) {
-    const bool has = base + group < end;
-    const Item<T, W> it = item_of<ROWS>(a, has ? base + group : end - 1);
-    const long long pos = load_index(a.positions, a.wide_positions, it.t);
-    const bool live = pos >= 0, known = pos < a.table_rows;
+  // The same number of rounds for all groups of a block, for the shuffles; a group behind the last item has no rows. Token
+  // and chunk move by the step's quotient and remainder.
+  const unsigned start = block * kGroups + group, step_t = step / chunks, step_c = step - step_t * chunks;
+  unsigned t = start / chunks, chunk = start - t * chunks;
+  for (unsigned base = block * kGroups; base < n_items; base += step) {
+    const bool has = base + group < n_items;
+    const int h0 = chunk * ROWS, left = has && at.in_row ? side.heads - h0 : 0;
+    const long long pos = load_index(a.positions, a.wide_positions, has ? t : 0);
+    const T *const rows = side.x + t * side.token + h0 * side.head;
+    const long long plain = (static_cast<long long>(t) * side.heads + h0) * a.dim;
     RawRow<T> raw[ROWS], graw[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       raw[r] = RawRow<T>{};
       graw[r] = RawRow<T>{};
-      if (at.in_row && r < it.heads) {
-        const T *row = it.rows + r * it.head, *g = grad + (it.out + r) * a.dim;
+      if (r < left) {
+        const T *row = rows + r * side.head, *g = grad + plain + r * a.dim;
         raw[r] = RawRow<T>{load4(row + at.e0), load4(row + at.e1)};
         graw[r] = RawRow<T>{load4(g + at.e0), load4(g + at.e1)};
       }
     }
-    float c[4], s[4];
-    const bool turn = at.rotated && live && known;
-    if (turn) {
-      unpack4(load4(a.table + pos * a.rotary + 4 * lane), c);
-      unpack4(load4(a.table + pos * a.rotary + a.rotary / 2 + 4 * lane), s);
-    }
+    const bool live = pos >= 0, known = pos < a.table_rows, turn = at.rotated && live && known;
+    Turn<INTERLEAVED> angles;
+    if (turn) angles.load(a.table + pos * a.rotary, a.rotary, lane);
+    const float eps = known ? a.eps : __int_as_float(0x7fc00000);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      float x[8], g[8], sum = 0.f, dot = 0.f;
+      float2 x[4], g[4];
       unpack(raw[r], x);
       unpack(graw[r], g);
-      if (turn) rotate<INTERLEAVED, true>(g, c, s);
+      if (!live) {  // a padded token leaves nothing in the weights' gradients, whatever its rows hold
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sum = fmaf(x[i], x[i], sum);
-        dot = fmaf(x[i], g[i] * w[i], dot);
+        for (int i = 0; i < 4; ++i) x[i] = g[i] = make_float2(0.f, 0.f);
       }
-      sum = group_sum<LANES>(sum);
-      dot = group_sum<LANES>(dot);
-      float scale = rsqrtf(fmaf(sum, a.inv_dim, a.eps));
-      if (!known) scale = __int_as_float(0x7fc00000);
-      const float mean = dot * scale * a.inv_dim;
-      const bool counts = has && live && r < it.heads;  // a padded token leaves nothing in the weights' gradients, whatever its gradient holds
+      if (turn) rotate<true>(g, angles);
+      float2 wg[4], square = mul2(x[0], x[0]), dots;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float n = x[i] * scale;
-        if (counts) dw[i] = fmaf(g[i], n, dw[i]);
-        x[i] = live ? scale * fmaf(-n, mean, g[i] * w[i]) : 0.f;
+      for (int i = 0; i < 4; ++i) {
+        wg[i] = mul2(g[i], w[i]);
+        dots = i == 0 ? mul2(x[i], wg[i]) : fma2(x[i], wg[i], dots);
+        if (i > 0) square = fma2(x[i], x[i], square);
       }
-      if (has && at.in_row && r < it.heads) {
-        T *to = out + (it.out + r) * a.dim;
+      const float sum = group_sum<LANES>(square.x + square.y), dot = group_sum<LANES>(dots.x + dots.y);
+      // Rows that are not there add zeros: with their sum of zero and eps = 0 the scale would be infinite.
+      const float scale = rsqrtf(r < side.heads - h0 && has && live ? fmaf(sum, a.inv_dim, eps) : 1.f);
+      const float2 s2 = both(scale), mean = both(-dot * scale * a.inv_dim);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 n = mul2(x[i], s2);
+        dw[i] = fma2(g[i], n, dw[i]);
+        x[i] = mul2(s2, fma2(n, mean, wg[i]));
+      }
+      if (r < left) {
+        T *to = out + plain + r * a.dim;
         store4(to + at.e0, x);
-        store4(to + at.e1, x + 4);
+        store4(to + at.e1, x + 2);
       }
+    }
+    t += step_t;
+    chunk += step_c;
+    if (chunk >= chunks) {
+      chunk -= chunks;
+      ++t;
     }
   }
   if (at.in_row) {
     store4(sums + group * a.dim + at.e0, dw);
-    store4(sums + group * a.dim + at.e1, dw + 4);
+    store4(sums + group * a.dim + at.e1, dw + 2);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < a.dim; i += kThreads) {
@@ -537,12 +551,13 @@ int qk_norm_rope(const NormRopeArgs &a, void *q_out, void *k_out, void *stream) 
       constexpr int kLanes = decltype(l)::value;
       auto launch = [&](auto rows, auto pairs) -> int {
         constexpr int kRows = decltype(rows)::value;
-        const long long items = items_of(a.tokens, a.q_heads, kRows) + items_of(a.tokens, a.k_heads, kRows);
+        const long long q_items = items_of(a.tokens, a.q_heads, kRows), items = q_items + items_of(a.tokens, a.k_heads, kRows);
         const unsigned blocks = blocks_for(items, kLanes);
         if (!blocks) return cudaErrorInvalidValue;
         norm_rope_kernel<T, W, kLanes, kRows, decltype(pairs)::value != 0>
-            <<<blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(norm_rope_args<T, W>(a), static_cast<unsigned>(items),
-                                                                         static_cast<T *>(q_out), static_cast<T *>(k_out));
+            <<<blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(norm_rope_args<T, W>(a), static_cast<unsigned>(q_items),
+                                                                         static_cast<unsigned>(items), static_cast<T *>(q_out),
+                                                                         static_cast<T *>(k_out));
         return cudaGetLastError();
       };
       // One row a group while that leaves SMs without work, four rows in flight beyond.
