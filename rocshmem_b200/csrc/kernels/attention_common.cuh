@@ -162,17 +162,54 @@ __device__ __forceinline__ float group_sum(float v) {
   for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+
+// The largest magnitude among the row's elements, of which the lane holds eight: that of the bits, so that a NaN or infinity
+// is it. 16-bit types compare two elements in one instruction.
 template <int LANES>
-__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+__device__ __forceinline__ float group_top(const Raw8<float> &r) {
+  const float v[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+  uint32_t top = 0;
 #pragma unroll
-  for (int o = LANES / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  return __uint_as_float(top);
+}
+template <int LANES>
+__device__ __forceinline__ uint32_t group_top16(const uint4 &r) {
+  uint32_t top = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+  return max(top & 0xffffu, top >> 16);
+}
+template <int LANES>
+__device__ __forceinline__ float group_top(const Raw8<__nv_bfloat16> &r) { return __uint_as_float(group_top16<LANES>(r.a) << 16); }
+template <int LANES>
+__device__ __forceinline__ float group_top(const Raw8<__half> &r) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(group_top16<LANES>(r.a))));
 }
 
 template <int V>
 struct Int {
   static constexpr int value = V;
 };
+
+// Launches a kernel that may be set up while the one before it on the stream is running; it has to wait for that one's end
+// (griddepcontrol.wait) before it reads.
+template <typename... KArgs>
+cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, unsigned threads, cudaStream_t s,
+                         typename same_as_kernel<KArgs>::type... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 // Lanes that hold a row of `dim` elements, eight each: 8, 16 or 32 (those past the row's end hold zeros).
 inline int row_lanes(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }

@@ -104,7 +104,7 @@ struct Side {
 };
 
 template <typename T, typename W, int LANES, int ROWS, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRope<T, W> a, unsigned q_items, unsigned items, T *q_out,
+__global__ void __launch_bounds__(kThreads, 5) norm_rope_kernel(NormRope<T, W> a, unsigned q_items, unsigned items, T *q_out,
                                                              T *k_out) {
   const int lane = threadIdx.x % LANES;
   const Place<INTERLEAVED> at(lane, a.dim, a.rotary);
@@ -161,6 +161,8 @@ __global__ void __launch_bounds__(kThreads, 3) norm_rope_backward_kernel(NormRop
                                                                          int q_blocks, const T *gq, const T *gk, T *dq,
                                                                          T *dk, float *partial) {
   extern __shared__ float sums[];  // [groups][dim]
+  // The sum over the blocks may be set up from here on; it waits for the end of this grid before it reads.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   constexpr int kGroups = kThreads / LANES;
   const Place<INTERLEAVED> at(lane, a.dim, a.rotary);
@@ -257,6 +259,7 @@ template <typename W>
 __global__ void __launch_bounds__(1024) norm_rope_weights_kernel(const float *partial, int q_rows, int rows, int dim,
                                                                  W *dq_weight, W *dk_weight) {
   __shared__ float s[32][33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int col = blockIdx.x * 32 + threadIdx.x % 32, warp = threadIdx.x / 32;
   const int first = blockIdx.y ? q_rows : 0, end = blockIdx.y ? rows : q_rows;
   float v = 0.f;
@@ -278,7 +281,7 @@ template <typename C>
 struct Cache {
   C *k, *v;
   float *k_scale, *v_scale;
-  long long slots;
+  int slots;
   int kv_heads, shift, dim;
 };
 
@@ -310,7 +313,7 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(Cache<C> c, const T 
   const T *from = (w.is_v ? v + w.head * v_head : k + w.head * k_head) + w.token * (w.is_v ? v_token : k_token);
   const long long step = w.is_v ? v_token : k_token;
   Raw8<T> raw[ROWS];
-  long long to[ROWS];
+  int to[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     to[r] = -1;
@@ -320,36 +323,31 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(Cache<C> c, const T 
       to[r] = slot_row(load_index(slots, wide_slots, static_cast<int>(w.token) + r), c.slots, c.shift, c.kv_heads, w.head);
     }
   }
-  C *base = w.is_v ? c.v : c.k;
+  C *const base = (w.is_v ? c.v : c.k) + 8 * lane;
+  float *const scales = w.is_v ? c.v_scale : c.k_scale;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     float x[8];
     unpack8(raw[r], x);
     if constexpr (kQuantize) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-      top = group_max<LANES>(top);
-      float m = __uint_as_float(max(top, __float_as_uint(0x1p-110f)));
-      if (top >= 0x7f800000u) m = __int_as_float(0x7fc00000);
+      const float top = group_top<LANES>(raw[r]);
+      const float m = top < INFINITY ? fmaxf(top, 0x1p-110f) : __int_as_float(0x7fc00000);  // the comparison fails for NaN too
       const float inv = 448.0f / m;
       if (to[r] >= 0) {
         if (in_row) {
-          uint2 o;
-          uint32_t *codes = reinterpret_cast<uint32_t *>(&o);
+          uint32_t codes[4];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float2 a = make_float2(x[4 * i] * inv, x[4 * i + 1] * inv);
-            const float2 b = make_float2(x[4 * i + 2] * inv, x[4 * i + 3] * inv);
-            codes[i] = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
-                   static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3)) << 16;
+          for (int i = 0; i < 4; ++i) {
+            const float2 y = mul2(make_float2(x[2 * i], x[2 * i + 1]), both(inv));
+            codes[i] = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
           }
-          *reinterpret_cast<uint2 *>(base + to[r] * c.dim + 8 * lane) = o;
+          *reinterpret_cast<uint2 *>(base + static_cast<long long>(to[r]) * c.dim) =
+              make_uint2(__byte_perm(codes[0], codes[1], 0x5410), __byte_perm(codes[2], codes[3], 0x5410));
         }
-        if (lane == 0) (w.is_v ? c.v_scale : c.k_scale)[to[r]] = m * (1.0f / 448.0f);
+        if (lane == 0) scales[to[r]] = m * (1.0f / 448.0f);
       }
     } else {
-      if (to[r] >= 0 && in_row) store8(base + to[r] * c.dim + 8 * lane, x);
+      if (to[r] >= 0 && in_row) store8(base + static_cast<long long>(to[r]) * c.dim, x);
     }
   }
 }
@@ -366,7 +364,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(Cache<C> c, T *k_out,
   if (!in_row) return;
   Raw8<C> raw[ROWS];
   float factor[ROWS];
-  long long from[ROWS];
+  int from[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     from[r] = w.token + r < tokens ? slot_row(load_index(slots, wide_slots, static_cast<int>(w.token) + r), c.slots, c.shift,
@@ -377,7 +375,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(Cache<C> c, T *k_out,
     raw[r] = Raw8<C>{};
     factor[r] = 0.f;
     if (from[r] >= 0) {
-      raw[r] = load8(base + from[r] * c.dim, lane);
+      raw[r] = load8(base + static_cast<long long>(from[r]) * c.dim, lane);
       if constexpr (sizeof(C) == 1) factor[r] = (w.is_v ? c.v_scale : c.k_scale)[from[r]];
     }
   }
@@ -521,7 +519,7 @@ int with_cache(const KvCacheArgs &c, F f) {
   auto args = [&](auto tag) {
     using C = typename decltype(tag)::type;
     return Cache<C>{static_cast<C *>(c.k), static_cast<C *>(c.v), c.k_scale, c.v_scale,
-                    static_cast<long long>(c.pages) << c.page_shift, c.kv_heads, c.page_shift, c.dim};
+                    c.pages << c.page_shift, c.kv_heads, c.page_shift, c.dim};
   };
   switch (c.type) {
     case ATTN_BF16: return f(args(Tag<__nv_bfloat16>{}), Tag<__nv_bfloat16>{});
@@ -533,6 +531,7 @@ int with_cache(const KvCacheArgs &c, F f) {
 
 bool refuse(const KvCacheArgs &c) {
   return bad_rows(c.dim) || c.pages < 0 || c.kv_heads < 1 || c.page_shift < 0 || c.page_shift > 20 ||
+         (static_cast<long long>(c.pages) * c.kv_heads << c.page_shift) > 0x7fffffffll ||
          (c.type == ATTN_E4M3 && (!c.k_scale || !c.v_scale));
 }
 
@@ -595,9 +594,8 @@ int qk_norm_rope_backward(const NormRopeArgs &a, const void *gq, const void *gk,
       };
       const int e = a.interleaved ? launch(Int<1>{}) : launch(Int<0>{});
       if (e != cudaSuccess) return e;
-      norm_rope_weights_kernel<W><<<dim3((a.dim + 31) / 32, 2), 1024, 0, s>>>(
-          workspace, q_blocks, blocks, a.dim, static_cast<W *>(dq_weight), static_cast<W *>(dk_weight));
-      return cudaGetLastError();
+      return launch_after(norm_rope_weights_kernel<W>, dim3((a.dim + 31) / 32, 2), 1024, s, workspace, q_blocks, blocks, a.dim,
+                          static_cast<W *>(dq_weight), static_cast<W *>(dk_weight));
     });
   });
 }

@@ -55,10 +55,11 @@ ATTN_HD int page_row(int page, int num_pages, int pos, int shift, int kv_heads, 
   return ((page * kv_heads + head) << shift) + (pos & ((1 << shift) - 1));
 }
 
-// The same for a flat slot (page * page_size + offset), or -1 for a slot outside the cache.
-ATTN_HD long long slot_row(long long slot, long long num_slots, int shift, int kv_heads, int head) {
+// The same for a flat slot (page * page_size + offset), or -1 for a slot outside the cache, which has at most 2^31 - 1 rows.
+ATTN_HD int slot_row(long long slot, int num_slots, int shift, int kv_heads, int head) {
   if (slot < 0 || slot >= num_slots) return -1;
-  return (((slot >> shift) * kv_heads + head) << shift) + (slot & ((1ll << shift) - 1));
+  const int s = static_cast<int>(slot);
+  return (((s >> shift) * kv_heads + head) << shift) + (s & ((1 << shift) - 1));
 }
 
 }  // namespace attn

@@ -236,6 +236,7 @@ KvCacheArgs cache_args(const Cache &c) {
   if (heads < 1 || heads > (1 << 20) || pages > INT32_MAX || dim % 8 || dim < 8 || dim > 256) {
     bad_value("KvCache: at least one head, head_dim a multiple of 8 up to 256");
   }
+  if (pages * heads * size > INT32_MAX) bad_value("KvCache: at most 2^31 - 1 rows (pages * kv_heads * page_size), got ", pages * heads * size);
   const bool scaled = k.scalar_type() == at::kFloat8_e4m3fn;
   for (const OptTensor *s : {&c.k_scale, &c.v_scale}) {
     if (scaled && (!s->has_value() || (*s)->scalar_type() != at::kFloat || (*s)->sizes() != k.sizes().slice(0, 3))) {
@@ -315,9 +316,7 @@ Paged check_paged(const Tensor &q, const Cache &c, const Tensor &block_table, co
     bad_value("scale must be positive, softcap and window not negative");
   }
   const int64_t most = block_table.size(1) * c.k.size(2);
-  if (most > INT32_MAX - 256 || c.k.size(0) * c.k.size(1) * c.k.size(2) > INT32_MAX) {
-    bad_value("paged_attention: a sequence's pages hold at most 2^31 - 257 tokens, the cache at most 2^31 - 1 rows");
-  }
+  if (most > INT32_MAX - 256) bad_value("paged_attention: a sequence's pages hold at most 2^31 - 257 tokens, got ", most);
   PagedAttentionArgs &a = p.args;
   a.q = data(q);
   a.q_token = s.token;

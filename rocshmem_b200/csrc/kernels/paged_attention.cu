@@ -783,18 +783,9 @@ auto with_shape(int dim, int group, int cache_type, F f) {
 
 template <int D, int NT, int MODE, int GROUPS>
 int launch_join(const Params &p, cudaStream_t s) {
-  // The join's blocks may be set up while the warps above are running; they wait for them before they read.
   constexpr int kLanes = join_threads(GROUPS) / GROUPS;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.kv_heads * p.chunks, (Shape<D, NT, MODE>::kFrags * 32 + kLanes - 1) / kLanes);
-  cfg.blockDim = dim3(join_threads(GROUPS));
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, NT, MODE, GROUPS>, p);
+  const dim3 grid(static_cast<unsigned>(p.batch) * p.kv_heads * p.chunks, (Shape<D, NT, MODE>::kFrags * 32 + kLanes - 1) / kLanes);
+  return launch_after(paged_join_kernel<D, NT, MODE, GROUPS>, grid, join_threads(GROUPS), s, p);
 }
 
 template <int D, int NT, int MODE>

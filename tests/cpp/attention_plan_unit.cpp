@@ -47,8 +47,11 @@ void check_rows() {
   CHECK(slot_row(64, 64, 4, 2, 1) == -1);
   CHECK(slot_row(1ll << 40, 64, 4, 2, 1) == -1);
   CHECK(slot_row(63, 64, 4, 2, 1) == ((3 * 2 + 1) << 4) + 15);
-  // Row numbers past 32 bits, with 2^28 pages of 16 slots and two heads.
-  CHECK(slot_row((1ll << 32) - 1, 1ll << 32, 4, 2, 1) == (((1ll << 28) - 1) * 2 + 1) * 16 + 15);
+  CHECK(slot_row((1ll << 32) + 5, 64, 4, 2, 1) == -1);  // not what its low 32 bits say
+  // The last row of the largest cache, 2^31 - 32 rows in pages of 16 slots and two heads.
+  const int slots = 0x7fffffe0 / 2;
+  CHECK(slot_row(slots - 1, slots, 4, 2, 1) == 0x7fffffe0 - 1);
+  CHECK(slot_row(slots, slots, 4, 2, 1) == -1);
 }
 
 void check_split(const std::vector<int> &lengths, int capacity, int window, int units, int shares, int least, int tile) {
