@@ -44,9 +44,12 @@ struct Owners {
 };
 ATTN_HD Owners owners(long long begin, int n, long long per) { return Owners{begin / per, (begin + n - 1) / per}; }
 
-// Which of share c's two places holds its partial result of a pair that lies in shares `o`: 0 for a pair that an earlier
-// share began, 1 for one that a later share ends.
-ATTN_HD int place(Owners o, long long c) { return c > o.first ? 0 : 1; }
+// Which of share c's two places holds its partial result of a pair that begins in share `first`: 0 for a pair that an
+// earlier share began, 1 for one that a later share ends.
+ATTN_HD int place(long long first, long long c) { return c > first ? 0 : 1; }
+
+// The last share that a pair of n tiles lies in which begins in share `share` with `left` of the share's tiles left.
+ATTN_HD int last_share(int share, int n, int left, int per) { return n > left ? share + (n - left + per - 1) / per : share; }
 
 // Row (of `dim` elements) of position `pos` in a cache [pages, kv_heads, page_size, dim], or -1 where the position is
 // not visible or its page is no page of the cache. page_size = 1 << shift.

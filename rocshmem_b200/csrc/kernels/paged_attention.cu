@@ -126,13 +126,16 @@ struct Shape {
   static constexpr int kHeads = 8 * NT;
   static constexpr int kFrags = D / 16 * NT;               // of O^T, four values a lane
   static constexpr int kPart = kFrags * 128 + 2 * kHeads;  // floats of a partial result: O^T, maxima (base 2), sums
-  // As many blocks as registers allow, with as many stages as then fit: bytes on their way, and warps to issue between them.
-  static constexpr int kBlocks = D == 256 ? (MODE == MODE_E4M3 ? 8 : 6) : D == 128 || (NT == 2 && D == 96) ? 8
-                                 : NT == 1 && D == 64 && MODE == MODE_E4M3 ? 16 : 12;
-  static constexpr int kFit = (227 * 1024 / kBlocks - 1024) / kStage;
-  static constexpr int kStages = kFit > 6 ? 6 : kFit;
+  // Two stages: one tile on its way while the other is used. e4m3 is bound by instructions and takes as many warps as its
+  // registers allow. 16-bit caches are bound by memory and want 64 - 70 KB on their way for each SM, no more: SMs of
+  // large GPCs get less of the bandwidth than others, and the further the queues reach, the later they end (128 elements,
+  // 64 sequences, blocks x stages an SM: 8 x 2 119 us, 12 x 2 123, 5 x 4 123, 8 x 3 127).
+  static constexpr int kStages = 2;
+  static constexpr int kWarpsByRegisters = NT == 2 ? (D == 64 ? 12 : 8) : D == 64 ? 16 : D == 96 ? 12 : 8;
+  static constexpr int kWarpsByBytes = 70 * 1024 / kStage;
+  static constexpr int kBlocks = MODE == MODE_E4M3 || kWarpsByBytes > kWarpsByRegisters ? kWarpsByRegisters : kWarpsByBytes;
   static constexpr int kSmem = kStages * kStage;
-  static_assert(kStages >= 2 && kPitchK % 16 == 0 && kPitchV % 16 == 0 && kStage % 16 == 0, "alignment");
+  static_assert(kBlocks * (kSmem + 1024) <= 228 * 1024 && kPitchK % 16 == 0 && kPitchV % 16 == 0 && kStage % 16 == 0, "alignment");
 };
 
 struct Params {
@@ -149,7 +152,7 @@ struct Params {
   float *lse;
   int q_bf16, out_f32;
   float *partial;     // [shares][2][kPart]
-  long long *bases;   // [batch + 1]: a sequence's first tile; then the tiles of a share
+  int2 *spans;        // [batch][units]: the first and the last share that a pair lies in
   int blocks, least;
 };
 
@@ -196,6 +199,55 @@ __device__ __forceinline__ void store_out(const Params &p, long long at, float x
   else store1(static_cast<__half *>(p.out) + at, x);
 }
 
+// For the two heads of a lane's columns in group j: the factor that makes sums of p v results, and, by one lane each, the lse.
+template <int NT>
+__device__ __forceinline__ void finish(const Params &p, long long row0, int n_heads, int j, int lane, const float (&m)[2],
+                                       const float (&l)[2], float (&inv)[2]) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int col = 8 * j + 2 * (lane % 4) + c;
+    const bool none = m[c] == -INFINITY && l[c] == 0.f;
+    inv[c] = none ? 0.f : 1.f / l[c];
+    if (lane < 4 && p.lse != nullptr && col < n_heads) p.lse[row0 + col] = none ? -INFINITY : m[c] * kLn2 + logf(l[c]);
+  }
+}
+
+// Fragment (d, j) of O^T times the heads' factors, to the result. All lanes of the warp call it.
+template <int D, int MODE>
+__device__ __forceinline__ void store_fragment(const Params &p, long long row0, int n_heads, int j, int d, int lane,
+                                               const float (&o)[4], const float (&inv)[2]) {
+  const int g = lane / 4, t = lane % 4;
+  if (p.out_f32) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int col = 8 * j + 2 * t + c % 2;
+      if (col < n_heads) {
+        static_cast<float *>(p.out)[(row0 + col) * D + element<D, MODE>(d, 8 * (c / 2) + g)] = o[c] * inv[c % 2];
+      }
+    }
+  } else if constexpr (MODE == MODE_E4M3) {
+    // A lane's rows g and g + 8 are neighbouring elements.
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int col = 8 * j + 2 * t + c;
+      const float x = o[c] * inv[c], y = o[2 + c] * inv[c];
+      if (col < n_heads) {
+        *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + (row0 + col) * D + element<D, MODE>(d, g)) =
+            p.q_bf16 ? pack2<true>(x, y) : pack2<false>(x, y);
+      }
+    }
+  } else {
+    // Transposed, a lane has two neighbouring elements of head g.
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const uint32_t w = transpose8x8(pack2<MODE == MODE_BF16>(o[2 * r] * inv[0], o[2 * r + 1] * inv[1]));
+      if (8 * j + g < n_heads) {
+        *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + (row0 + 8 * j + g) * D + 16 * d + 8 * r + 2 * t) = w;
+      }
+    }
+  }
+}
+
 template <int D, int NT, int MODE>
 __global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(const Params p) {
   using S = Shape<D, NT, MODE>;
@@ -220,29 +272,23 @@ __global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(
   const long long total = __shfl_sync(0xffffffffu, upto, 31), per = per_share(total, p.blocks, p.least);
   // The join may be set up from here on; it waits for the end of this grid before it reads.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // The lane whose sequences hold the share's first tile finds the sequence. Block 0 writes down all first tiles for the
-  // join; a sequence that sees nothing gets its result here.
+  // The lane whose sequences hold the share's first tile finds the sequence.
   const long long t0 = per * blockIdx.x, t1 = min(total, t0 + per);
   const bool holds = t0 < t1 && t0 >= upto - mine && t0 < upto;
-  int first_b = 0;
-  long long into = 0;
-  if (holds || blockIdx.x == 0) {
-    long long at = upto - mine;
-    for (int b = b_lo; b < b_hi; ++b) {
-      const long long n = tiles_at(b);
-      if (t0 >= at && t0 < at + n) {
-        first_b = b;
-        into = t0 - at;
-      }
-      if (blockIdx.x == 0) p.bases[b] = at;
-      at += n;
+  int first_b = b_lo;
+  long long into = t0 - (upto - mine);
+  if (holds) {
+    for (long long n = tiles_at(first_b); into >= n; n = tiles_at(first_b)) {
+      into -= n;
+      ++first_b;
     }
-    if (blockIdx.x == 0 && lane == 0) p.bases[p.batch] = per;
   }
+  // A sequence that sees nothing gets its result here.
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
     const Span s = visible(p.lengths[b], p.capacity, p.window);
     if (s.end > s.first) continue;
     for (int i = lane; i < p.heads * D; i += 32) store_out(p, static_cast<long long>(b) * p.heads * D + i, 0.f);
+    for (int i = lane; i < units; i += 32) p.spans[static_cast<long long>(b) * units + i] = make_int2(0, 0);
     if (p.lse != nullptr) {
       for (int i = lane; i < p.heads; i += 32) p.lse[static_cast<long long>(b) * p.heads + i] = -INFINITY;
     }
@@ -381,6 +427,10 @@ __global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(
     for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -INFINITY;
 
     const bool begins = cur.tile == 0;
+    if (begins && lane == 0) {
+      const int share = blockIdx.x;
+      p.spans[static_cast<long long>(b) * units + cur.unit] = make_int2(share, last_share(share, cur.n, cur.left, static_cast<int>(per)));
+    }
     bool ends = false;
     while (true) {
       copies_wait<S::kStages - 2>();
@@ -633,65 +683,25 @@ __global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       float inv[2];
+      finish<NT>(p, row0, n_heads, j, lane, m[j], l[j], inv);
+      if constexpr (MODE == MODE_E4M3) inv[0] *= cv, inv[1] *= cv;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int col = 8 * j + 2 * t + c;
-        const bool none = m[j][c] == -INFINITY && l[j][c] == 0.f;
-        inv[c] = none ? 0.f : (MODE == MODE_E4M3 ? cv : 1.f) / l[j][c];
-        if (g == 0 && p.lse != nullptr && col < n_heads) p.lse[row0 + col] = none ? -INFINITY : m[j][c] * kLn2 + logf(l[j][c]);
-      }
-#pragma unroll
-      for (int d = 0; d < DK; ++d) {
-        if (p.out_f32) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int col = 8 * j + 2 * t + c % 2;
-            if (col < n_heads) {
-              static_cast<float *>(p.out)[(row0 + col) * D + element<D, MODE>(d, 8 * (c / 2) + g)] = o[d][j][c] * inv[c % 2];
-            }
-          }
-        } else if constexpr (MODE == MODE_E4M3) {
-          // A lane's rows g and g + 8 are neighbouring elements.
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int col = 8 * j + 2 * t + c;
-            const float x = o[d][j][c] * inv[c], y = o[d][j][2 + c] * inv[c];
-            if (col < n_heads) {
-              *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + (row0 + col) * D + element<D, MODE>(d, g)) =
-                  p.q_bf16 ? pack2<true>(x, y) : pack2<false>(x, y);
-            }
-          }
-        } else {
-          // Transposed, a lane has two neighbouring elements of head g.
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint32_t w = transpose8x8(pack2<kBf16>(o[d][j][2 * r] * inv[0], o[d][j][2 * r + 1] * inv[1]));
-            if (8 * j + g < n_heads) {
-              *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + (row0 + 8 * j + g) * D + 16 * d + 8 * r + 2 * t) = w;
-            }
-          }
-        }
-      }
+      for (int d = 0; d < DK; ++d) store_fragment<D, MODE>(p, row0, n_heads, j, d, lane, o[d][j], inv);
     }
   }
   copies_wait<0>();
 }
 
-constexpr int join_threads(int groups) { return groups > 8 ? 32 * groups : 256; }
-
 // Adds the partial results of the pairs that several warps share, in the order of the shares. A thread has the four values
 // that a lane had of one fragment; a block GROUPS sets of such threads, which take the parts in turn.
 template <int D, int NT, int MODE, int GROUPS>
-__global__ void __launch_bounds__(join_threads(GROUPS)) paged_join_kernel(const Params p) {
+__global__ void __launch_bounds__(256) paged_join_kernel(const Params p) {
   using S = Shape<D, NT, MODE>;
-  constexpr int kLanes = join_threads(GROUPS) / GROUPS, kAhead = 4;
+  constexpr int kLanes = 256 / GROUPS, kAhead = 4;
   __shared__ float4 s_o[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? kLanes : 1], s_ml[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? kLanes : 1];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int units = p.kv_heads * p.chunks, unit = blockIdx.x % units, b = blockIdx.x / units;
-  const int n = tiles_of(visible(p.lengths[b], p.capacity, p.window), S::kKeys);
-  if (n == 0) return;
-  const Owners own = owners(p.bases[b] + static_cast<long long>(unit) * n, n, p.bases[p.batch]);
-  if (own.first == own.last) return;
+  const int2 own = p.spans[blockIdx.x];
+  if (own.x == own.y) return;
   const int group = threadIdx.x / kLanes, at = blockIdx.y * kLanes + threadIdx.x % kLanes;
   const int frag = at / 32, lane = at % 32, d = frag / NT, j = frag % NT, g = lane / 4, t = lane % 4;
   const bool has = frag < S::kFrags;
@@ -710,21 +720,21 @@ __global__ void __launch_bounds__(join_threads(GROUPS)) paged_join_kernel(const 
     top = now;
   };
   if (has) {
-    for (long long c0 = own.first + group; c0 <= own.last; c0 += kAhead * GROUPS) {
+    for (int c0 = own.x + group; c0 <= own.y; c0 += kAhead * GROUPS) {
       float4 x[kAhead];
       float2 m[kAhead], l[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const long long c = c0 + i * GROUPS;
-        if (c > own.last) break;
-        const float *part = p.partial + (c * 2 + place(own, c)) * S::kPart;
+        const int c = c0 + i * GROUPS;
+        if (c > own.y) break;
+        const float *part = p.partial + (static_cast<long long>(c) * 2 + place(own.x, c)) * S::kPart;
         x[i] = reinterpret_cast<const float4 *>(part)[at];
         m[i] = *reinterpret_cast<const float2 *>(part + S::kFrags * 128 + 8 * j + 2 * t);
         l[i] = *reinterpret_cast<const float2 *>(part + S::kFrags * 128 + S::kHeads + 8 * j + 2 * t);
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        if (c0 + i * GROUPS > own.last) break;
+        if (c0 + i * GROUPS > own.y) break;
         add(x[i], m[i], l[i]);
       }
     }
@@ -735,26 +745,20 @@ __global__ void __launch_bounds__(join_threads(GROUPS)) paged_join_kernel(const 
     s_ml[group][at_s] = make_float4(top.x, top.y, sum.x, sum.y);
     __syncthreads();
     if (group != 0) return;
-#pragma unroll 8
+#pragma unroll
     for (int i = 1; i < GROUPS; ++i) {
       const float4 ml = s_ml[i][at_s];
       add(s_o[i][at_s], make_float2(ml.x, ml.y), make_float2(ml.z, ml.w));
     }
   }
   if (!has) return;
+  const int units = p.kv_heads * p.chunks, unit = blockIdx.x % units, b = blockIdx.x / units;
   const int kv = unit / p.chunks, h0 = kv * p.group + unit % p.chunks * S::kHeads, n_heads = min(S::kHeads, (kv + 1) * p.group - h0);
-  const long long row0 = static_cast<long long>(b) * p.heads + h0;
   const float v[4] = {acc.x, acc.y, acc.z, acc.w}, tops[2] = {top.x, top.y}, sums[2] = {sum.x, sum.y};
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int col = 8 * j + 2 * t + c;
-    if (col >= n_heads) continue;
-    const bool none = tops[c] == -INFINITY && sums[c] == 0.f;
-    const float inv = none ? 0.f : 1.f / sums[c];
-    store_out(p, (row0 + col) * D + element<D, MODE>(d, g), v[c] * inv);
-    store_out(p, (row0 + col) * D + element<D, MODE>(d, g + 8), v[2 + c] * inv);
-    if (d == 0 && g == 0 && p.lse != nullptr) p.lse[row0 + col] = none ? -INFINITY : tops[c] * kLn2 + logf(sums[c]);
-  }
+  float inv[2];
+  // One warp for each group of heads writes the lse.
+  finish<NT>(p, static_cast<long long>(b) * p.heads + h0, d == 0 ? n_heads : 0, j, lane, tops, sums, inv);
+  store_fragment<D, MODE>(p, static_cast<long long>(b) * p.heads + h0, n_heads, j, d, lane, v, inv);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------
@@ -783,9 +787,9 @@ auto with_shape(int dim, int group, int cache_type, F f) {
 
 template <int D, int NT, int MODE, int GROUPS>
 int launch_join(const Params &p, cudaStream_t s) {
-  constexpr int kLanes = join_threads(GROUPS) / GROUPS;
+  constexpr int kLanes = 256 / GROUPS;
   const dim3 grid(static_cast<unsigned>(p.batch) * p.kv_heads * p.chunks, (Shape<D, NT, MODE>::kFrags * 32 + kLanes - 1) / kLanes);
-  return launch_after(paged_join_kernel<D, NT, MODE, GROUPS>, grid, join_threads(GROUPS), s, p);
+  return launch_after(paged_join_kernel<D, NT, MODE, GROUPS>, grid, 256, s, p);
 }
 
 template <int D, int NT, int MODE>
@@ -811,14 +815,17 @@ int launch(Params p, cudaStream_t s) {
   // The lengths are on the device: what counts is the most that they can be.
   const int longest = p.window > 0 ? std::min(p.window, p.capacity) : p.capacity;
   if (longest <= S::kKeys) return 0;  // no pair has two tiles: nothing to join
-  // Few pairs, many parts of each: sets of threads share the parts. Many pairs: few parts of each.
+  // Many parts of each of a few pairs are shared by eight sets of threads (8 pairs of 148 parts: 35 us the whole call, with one set
+  // 62); few parts of many pairs are not worth the exchange (128 pairs of 9 parts: 73 us with one set, 76 with eight).
   const int pairs = p.batch * p.kv_heads * p.chunks, shares = p.blocks;
-  if (pairs > shares / 8) return launch_join<D, NT, MODE, 1>(p, s);
-  return pairs > shares / 48 ? launch_join<D, NT, MODE, 8>(p, s) : launch_join<D, NT, MODE, 32>(p, s);
+  return pairs > shares / 24 ? launch_join<D, NT, MODE, 1>(p, s) : launch_join<D, NT, MODE, 8>(p, s);
 }
 
-// The first tiles, in whole 16 bytes.
-size_t base_bytes(int batch) { return (static_cast<size_t>(batch) + 1 + 1) / 2 * 16; }
+// The pairs' spans, in whole 16 bytes.
+size_t span_bytes(const KvCacheArgs &c, int batch, int heads) {
+  const int group = heads / c.kv_heads, each = heads_per_unit(group, c.dim);
+  return (static_cast<size_t>(batch) * c.kv_heads * ((group + each - 1) / each) + 1) / 2 * 16;
+}
 
 bool refuse_sizes(const KvCacheArgs &c, int batch, int heads) {
   return (c.dim != 64 && c.dim != 96 && c.dim != 128 && c.dim != 256) || batch < 0 || heads < 1 || c.kv_heads < 1 ||
@@ -836,7 +843,7 @@ size_t paged_attention_workspace(const KvCacheArgs &c, int batch, int heads) {
   if (refuse_sizes(c, batch, heads)) return 0;
   return with_shape(c.dim, heads / c.kv_heads, c.type, [&](auto d, auto nt, auto mode) -> size_t {
     using S = Shape<decltype(d)::value, decltype(nt)::value, decltype(mode)::value>;
-    return base_bytes(batch) + static_cast<size_t>(device_sm_count()) * S::kBlocks * 2 * S::kPart * 4;
+    return span_bytes(c, batch, heads) + static_cast<size_t>(device_sm_count()) * S::kBlocks * 2 * S::kPart * 4;
   });
 }
 
@@ -880,8 +887,8 @@ int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *wor
   p.lse = a.lse;
   p.q_bf16 = a.q_type == ATTN_BF16;
   p.out_f32 = a.out_type == ATTN_F32;
-  p.bases = static_cast<long long *>(workspace);
-  p.partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + base_bytes(a.batch));
+  p.spans = static_cast<int2 *>(workspace);
+  p.partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + span_bytes(c, a.batch, a.heads));
   return with_shape(c.dim, p.group, c.type, [&](auto d, auto nt, auto mode) -> int {
     return launch<decltype(d)::value, decltype(nt)::value, decltype(mode)::value>(p, static_cast<cudaStream_t>(stream));
   });

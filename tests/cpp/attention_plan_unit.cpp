@@ -70,6 +70,8 @@ void check_split(const std::vector<int> &lengths, int capacity, int window, int 
       const long long begin = bases[b] + static_cast<long long>(u) * n;
       const Owners own = owners(begin, n, per);
       CHECK(own.first >= 0 && own.first <= own.last && own.last < shares);
+      const long long left = ((own.first + 1) * per < total ? (own.first + 1) * per : total) - begin;
+      CHECK(last_share(static_cast<int>(own.first), n, static_cast<int>(left), static_cast<int>(per)) == own.last);
       // The tiles that the owners' shares hold of this pair are all of them.
       long long seen = 0;
       for (long long c = own.first; c <= own.last; ++c) {
@@ -79,8 +81,8 @@ void check_split(const std::vector<int> &lengths, int capacity, int window, int 
         seen += hi - lo;
         if (own.first == own.last) continue;
         // What the warp itself goes by: it begins the pair (place 1) or finds it begun (place 0).
-        CHECK(place(own, c) == (lo == begin ? 1 : 0));
-        CHECK(places.insert({c, place(own, c)}).second);
+        CHECK(place(own.first, c) == (lo == begin ? 1 : 0));
+        CHECK(places.insert({c, place(own.first, c)}).second);
       }
       CHECK(seen == n);
     }
