@@ -532,7 +532,7 @@ int with_cache(const KvCacheArgs &c, F f) {
 bool refuse(const KvCacheArgs &c) {
   return bad_rows(c.dim) || c.pages < 0 || c.kv_heads < 1 || c.page_shift < 0 || c.page_shift > 20 ||
          (static_cast<long long>(c.pages) * c.kv_heads << c.page_shift) > 0x7fffffffll ||
-         (c.type == ATTN_E4M3 && (!c.k_scale || !c.v_scale));
+         (c.type == ATTN_E4M3 && c.pages > 0 && (!c.k_scale || !c.v_scale));
 }
 
 }  // namespace

@@ -8,14 +8,18 @@
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <cmath>
 #include <optional>
 #include <sstream>
 #include <stdexcept>
 #include <string>
 #include <tuple>
 #include <utility>
+#include <vector>
 
 #include "attention_kernels.hpp"
 
@@ -218,6 +222,21 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> py_qk_norm_rope_backward(const Tensor
   return {dq, dk, dwq, dwk};
 }
 
+// A leaf whose gradients an eager graph, alive at the time, accumulates on another stream cannot take part in a captured
+// backward pass: the engine would make that stream wait for the captured one, which ends the process. Refused instead.
+void check_capture(const std::vector<Tensor> &tensors) {
+  for (const Tensor &t : tensors) {
+    if (!t.requires_grad() || !t.is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) continue;
+    const auto stream = node->stream();
+    if (stream.has_value() && *stream != c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap()) {
+      throw std::runtime_error("qk_norm_rope: a graph of the same leaves from outside the capture is alive; drop it (its outputs "
+                               "and losses) before a backward pass is captured");
+    }
+  }
+}
+
 // ---- the paged cache --------------------------------------------------------------------------------------------------
 
 struct Cache {
@@ -248,6 +267,9 @@ KvCacheArgs cache_args(const Cache &c) {
     if (t != nullptr && (!t->is_contiguous() || !aligned(*t) || t->device() != k.device())) {
       bad_value("KvCache: tensors must be contiguous, 16-byte aligned and on one device");
     }
+  }
+  for (const Tensor *t : {&c.k, &c.v}) {
+    if (t->requires_grad()) bad_value("KvCache: the cache is written in place and cannot require a gradient");
   }
   int shift = 0;
   while ((int64_t{1} << shift) < size) ++shift;
@@ -407,6 +429,7 @@ PYBIND11_MODULE(_A, m) {
   }));
   m.def("qk_norm_rope", &py_qk_norm_rope);
   m.def("qk_norm_rope_backward", &py_qk_norm_rope_backward);
+  m.def("check_capture", &check_capture);
   m.def("kv_cache_write", &py_kv_cache_write);
   m.def("kv_cache_read", &py_kv_cache_read);
   m.def("check_paged", [](const Tensor &q, const Cache &c, const Tensor &table, const Tensor &lengths,

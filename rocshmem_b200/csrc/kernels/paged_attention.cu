@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(
             if constexpr (MODE == MODE_E4M3) {
               f = f_s[row];
               v_factor[i][r] = f_s[kKeys + row];
-              v_top = fmaxf(v_top, v_factor[i][r]);
+              v_top = fmaxf(v_top, fabsf(v_factor[i][r]));
             }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -849,7 +849,7 @@ size_t paged_attention_workspace(const KvCacheArgs &c, int batch, int heads) {
 
 int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *workspace, size_t workspace_bytes,
                     void *stream) {
-  if (refuse_sizes(c, a.batch, a.heads) || (c.type == ATTN_E4M3 && (!c.k_scale || !c.v_scale)) ||
+  if (refuse_sizes(c, a.batch, a.heads) || (c.type == ATTN_E4M3 && c.pages > 0 && (!c.k_scale || !c.v_scale)) ||
       (a.q_type != ATTN_BF16 && a.q_type != ATTN_F16) || (c.type != ATTN_E4M3 && c.type != a.q_type) ||
       (a.out_type != a.q_type && a.out_type != ATTN_F32) || a.window < 0 || a.max_pages < 0 ||
       (static_cast<long long>(a.max_pages) << c.page_shift) > 0x7fffffffll - 256 ||
@@ -875,7 +875,7 @@ int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *wor
   p.chunks = (p.group + heads_per_unit(p.group, c.dim) - 1) / heads_per_unit(p.group, c.dim);
   p.pages = c.pages;
   p.shift = c.page_shift;
-  p.capacity = a.max_pages << c.page_shift;
+  p.capacity = c.pages > 0 ? a.max_pages << c.page_shift : 0;  // without pages there is not even an address to skip
   // A warp counts its tiles (of 16 keys at least) in 32 bits.
   if (static_cast<long long>(a.batch) * c.kv_heads * p.chunks > 0x7fffffffll * device_sm_count() / (p.capacity / 16 + 1)) {
     return cudaErrorInvalidValue;

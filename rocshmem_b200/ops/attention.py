@@ -101,18 +101,22 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     ``(2 i, 2 i + 1)``. ``positions [T]`` int32 or int64: a negative one marks padding, whose rows become zeros and have no
     gradient; one past the table makes its token's rows NaN.
 
-    Differentiable once with respect to ``q``, ``k`` and both weights; the weights' gradients are the same in every run."""
+    Differentiable once with respect to ``q``, ``k`` and both weights; the weights' gradients are the same in every run. A
+    backward pass can be captured into a CUDA graph with its forward pass; while an eager graph of the same leaves is alive, the
+    captured forward pass is refused."""
     if stream is not None:
         with _On(stream, q, k, q_weight, k_weight, positions, table):
             return qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved)
     if (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad) and torch.is_grad_enabled():
+        if q.is_cuda and torch.cuda.is_current_stream_capturing():
+            _native.load_attention().check_capture([q, k, q_weight, k_weight])
         return _NormRope.apply(q, k, q_weight, k_weight, positions, table, eps, interleaved)
     return _native.load_attention().qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved)
 
 
 # ---- the paged cache --------------------------------------------------------------------------------------------------
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class KvCache:
     """Keys and values of many sequences in pages: ``k``, ``v`` ``[pages, kv_heads, page_size, head_dim]`` in bf16, fp16
     or e4m3; for e4m3 with ``k_scale``, ``v_scale [pages, kv_heads, page_size]`` fp32, the factor of each row. The page
@@ -124,6 +128,9 @@ class KvCache:
 
     def __post_init__(self):
         object.__setattr__(self, "_cache", _native.load_attention().Cache(self.k, self.v, self.k_scale, self.v_scale))
+
+    def __reduce__(self):
+        return KvCache, (self.k, self.v, self.k_scale, self.v_scale)
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
@@ -224,7 +231,8 @@ def paged_attention(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor, 
     memory with an input. ``block_table [B, pages]`` and ``lengths [B]`` are int32 on the device.
 
     Lengths are taken between 0 and the table's end. Tokens in a page that is no page of the cache are not seen. A sequence that sees
-    nothing has zeros and an lse of -inf. Rows that are not seen may hold anything, NaN included."""
+    nothing has zeros and an lse of -inf. Rows that are not seen may hold anything, NaN included; an infinity or NaN in a row
+    that is seen makes the results of its heads NaN, except a score of -inf, which counts for nothing."""
     if stream is not None:
         with _On(stream, q, block_table, lengths, *cache._tensors(), out, lse):
             return paged_attention(q, cache, block_table, lengths, scale, softcap, window, out, lse, return_lse)

@@ -613,3 +613,105 @@ def test_prefill_then_decode_steps(cache, size):
                                   out=torch.empty(B, H, D, device="cuda"))
         joined, lse2 = at.attention_join(torch.stack([first[0], rest[0]]), torch.stack([first[1], rest[1]]), dtype=BF16)
         check_paged(at, c, q, table, lengths, joined, lse2)
+
+
+# ---- captures, far offsets, odd but allowed arguments ---------------------------------------------------------------
+
+def test_norm_rope_training_step_in_a_graph():
+    """Forward and backward captured together and replayed on new contents; refused while an eager graph of the same leaves
+    is alive."""
+    at, q, k, wq, wk, pos, table = norm_rope_case(200, 4, 2, 128, 128, BF16, F32, False, False, seed=8)
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, wq, wk)]
+    grads = [randn(gen(20 + i), *t.shape, dtype=BF16) for i, t in enumerate((q, k))]
+
+    def step():
+        out = at.qk_norm_rope(*leaves, pos, table)
+        return out, torch.autograd.grad(out, leaves, grads)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, back = step()
+    out = [x.detach() for x in out]
+    with torch.no_grad():
+        leaves[0].copy_(randn(gen(31), 200, 4, 128, dtype=BF16))
+        leaves[3].mul_(0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [x.clone() for x in (*out, *back)]
+    fresh = [t.detach().clone().requires_grad_() for t in leaves]
+    want = at.qk_norm_rope(*fresh, pos, table)
+    want = [x.detach() for x in want] + list(torch.autograd.grad(want, fresh, grads))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    new = [t.detach().clone().requires_grad_() for t in (q, k, wq, wk)]
+    alive = at.qk_norm_rope(*new, pos, table)
+    with pytest.raises(RuntimeError, match="alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            at.qk_norm_rope(*new, pos, table)
+    torch.cuda.synchronize()
+    assert torch.autograd.grad(alive, new, grads)[0].isfinite().all()
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+def test_rows_behind_four_gigabytes(cache):
+    """Rows whose offset in bytes does not fit 32 bits: written, read back and attended to."""
+    from rocshmem_b200.ops import attention as at
+    D, size, K = 256, 64, 4
+    pages = (9 << 30) // (2 if cache == BF16 else 1) // (K * size * D) // 2 + 3
+    c = at.KvCache.allocate(pages, size, K, D, cache)
+    assert c.k.numel() * c.k.element_size() > 1 << 32
+    g = gen(3)
+    n = 150
+    k, v = randn(g, n, K, D, dtype=BF16), randn(g, n, K, D, dtype=BF16)
+    table = torch.tensor([[pages - 1, 0, pages - 2]], dtype=torch.int32, device="cuda")
+    pos = torch.arange(n, device="cuda")
+    slots = at.token_slots(table, torch.zeros_like(pos), pos, size)
+    at.kv_cache_write(c, k, v, slots)
+    small = at.KvCache.allocate(3, size, K, D, cache)
+    near_table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
+    at.kv_cache_write(small, k, v, at.token_slots(near_table, torch.zeros_like(pos), pos, size))
+    for a, b in zip(at.kv_cache_read(c, slots), at.kv_cache_read(small, at.token_slots(near_table, torch.zeros_like(pos), pos, size))):
+        assert torch.equal(a, b) and (cache == E4M3 or torch.equal(a, k) or torch.equal(a, v))
+    q = randn(g, 1, 8, D, dtype=BF16)
+    ln = torch.tensor([n], dtype=torch.int32, device="cuda")
+    assert torch.equal(at.paged_attention(q, c, table, ln), at.paged_attention(q, small, near_table, ln))
+
+
+def test_caches_without_pages_and_factors_below_zero():
+    from rocshmem_b200.ops import attention as at
+    q = randn(gen(1), 2, 4, 64, dtype=BF16)
+    for dtype in (BF16, E4M3):
+        empty = at.KvCache.allocate(0, 16, 2, 64, dtype)
+        out, lse = at.paged_attention(q, empty, torch.zeros(2, 3, dtype=torch.int32, device="cuda"),
+                                      torch.full((2,), 40, dtype=torch.int32, device="cuda"), return_lse=True)
+        assert (out == 0).all() and (lse == -math.inf).all()
+    c, q, table, ln = paged_case([40, 129], 8, 2, 128, 16, BF16, E4M3, seed=3, poison=False)
+    c.k_scale[:, :, ::3] *= -1
+    c.v_scale[:, 1:] *= -40.0
+    out, lse = at.paged_attention(q, c, table, ln, return_lse=True)
+    mags = at.KvCache(c.k, c.v, c.k_scale, c.v_scale.abs())
+    want, want_lse = at.ref_paged_attention(q, c, table, ln)
+    a = (mags.v.view(torch.uint8) & 0x7f).view(E4M3)
+    sum_pv, _ = at.ref_paged_attention(q, at.KvCache(c.k, a, c.k_scale, mags.v_scale), table, ln)
+    near(out, want, HALF_STEP[BF16] * want.abs() + 2.0 ** -11 * sum_pv, "out")
+
+
+def test_expanded_queries_and_caches_that_are_copied():
+    import copy
+    import pickle
+    from rocshmem_b200.ops import attention as at
+    c, q, table, ln = paged_case([40, 129, 3], 8, 2, 64, 16, BF16, BF16, seed=3, poison=False)
+    one = q[:1].expand(3, -1, -1)
+    want = at.paged_attention(one.contiguous(), c, table, ln)
+    assert torch.equal(at.paged_attention(one, c, table, ln), want)
+    for other in (copy.copy(c), copy.deepcopy(c), pickle.loads(pickle.dumps(c))):
+        assert torch.equal(at.paged_attention(one, other, table, ln), want)
+    assert c != copy.copy(c) and c == c
+    with pytest.raises(ValueError, match="gradient"):
+        at.KvCache(torch.zeros(2, 2, 16, 64, dtype=BF16, device="cuda", requires_grad=True), torch.zeros(2, 2, 16, 64, dtype=BF16, device="cuda"))
