@@ -135,6 +135,7 @@ struct Shape {
   static constexpr int kWarpsByBytes = 70 * 1024 / kStage;
   static constexpr int kBlocks = MODE == MODE_E4M3 || kWarpsByBytes > kWarpsByRegisters ? kWarpsByRegisters : kWarpsByBytes;
   static constexpr int kSmem = kStages * kStage;
+  static constexpr int kTeam = 8 * kSmem <= 226 * 1024 ? 8 : 4;  // warps of a block of paged_short_kernel
   static_assert(kBlocks * (kSmem + 1024) <= 228 * 1024 && kPitchK % 16 == 0 && kPitchV % 16 == 0 && kStage % 16 == 0, "alignment");
 };
 
@@ -248,60 +249,14 @@ __device__ __forceinline__ void store_fragment(const Params &p, long long row0, 
   }
 }
 
-template <int D, int NT, int MODE>
-__global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(const Params p) {
+// Streams the tiles of a warp's share, from `cur` on. done(...) is called at the end of every pair, or of the share's part of
+// one, with the accumulators of O^T (e4m3: in units of cv), maxima and sums of the lane's columns, and whether the pair begins and ends here.
+template <int D, int NT, int MODE, typename F>
+__device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cur, int lane, F done) {
   using S = Shape<D, NT, MODE>;
   constexpr bool kBf16 = MODE == MODE_BF16;
   constexpr int kKeys = S::kKeys, MT = kKeys / 16, DK = D / 16;
-  extern __shared__ __align__(16) char ring[];
-  const int lane = threadIdx.x, g = lane / 4, t = lane % 4;
-  const int units = p.kv_heads * p.chunks;
-
-  // ---- the line of tiles ----
-  // Lanes take neighbouring sequences, `per_lane` each; a scan over the lanes gives each one its first tile.
-  const int per_lane = (p.batch + 31) / 32, b_lo = min(lane * per_lane, p.batch), b_hi = min(b_lo + per_lane, p.batch);
-  auto tiles_at = [&](int b) { return static_cast<long long>(tiles_of(visible(p.lengths[b], p.capacity, p.window), kKeys)) * units; };
-  long long mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += tiles_at(b);
-  long long upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  const long long total = __shfl_sync(0xffffffffu, upto, 31), per = per_share(total, p.blocks, p.least);
-  // The join may be set up from here on; it waits for the end of this grid before it reads.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // The lane whose sequences hold the share's first tile finds the sequence.
-  const long long t0 = per * blockIdx.x, t1 = min(total, t0 + per);
-  const bool holds = t0 < t1 && t0 >= upto - mine && t0 < upto;
-  int first_b = b_lo;
-  long long into = t0 - (upto - mine);
-  if (holds) {
-    for (long long n = tiles_at(first_b); into >= n; n = tiles_at(first_b)) {
-      into -= n;
-      ++first_b;
-    }
-  }
-  // A sequence that sees nothing gets its result here.
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    const Span s = visible(p.lengths[b], p.capacity, p.window);
-    if (s.end > s.first) continue;
-    for (int i = lane; i < p.heads * D; i += 32) store_out(p, static_cast<long long>(b) * p.heads * D + i, 0.f);
-    for (int i = lane; i < units; i += 32) p.spans[static_cast<long long>(b) * units + i] = make_int2(0, 0);
-    if (p.lse != nullptr) {
-      for (int i = lane; i < p.heads; i += 32) p.lse[static_cast<long long>(b) * p.heads + i] = -INFINITY;
-    }
-  }
-  if (t0 >= t1) return;
-  const int from = __ffs(__ballot_sync(0xffffffffu, holds)) - 1;
-  Cursor cur;
-  cur.b = __shfl_sync(0xffffffffu, first_b, from);
-  into = __shfl_sync(0xffffffffu, into, from);
-  enter(cur, p, kKeys);
-  cur.unit = static_cast<int>(into / cur.n);
-  cur.tile = static_cast<int>(into - static_cast<long long>(cur.unit) * cur.n);
-  cur.left = static_cast<int>(t1 - t0);
+  const int g = lane / 4, t = lane % 4;
   Cursor ahead = cur;
 
   // ---- loads: `ahead` runs kStages - 1 tiles before `cur`; a tile's page is looked up one step before its rows are ----
@@ -427,10 +382,7 @@ __global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(
     for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -INFINITY;
 
     const bool begins = cur.tile == 0;
-    if (begins && lane == 0) {
-      const int share = blockIdx.x;
-      p.spans[static_cast<long long>(b) * units + cur.unit] = make_int2(share, last_share(share, cur.n, cur.left, static_cast<int>(per)));
-    }
+    const Cursor pair = cur;
     bool ends = false;
     while (true) {
       copies_wait<S::kStages - 2>();
@@ -649,7 +601,6 @@ __global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(
       if (ends || cur.left <= 0) break;
     }
 
-    // ---- the result of the pair, or of this warp's part of it ----
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -658,28 +609,139 @@ __global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(
         for (int d = 4; d < 32; d <<= 1) l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], d);
       }
     }
-    if (!(begins && ends)) {
-      // Fragments as they lie in the lanes; the join knows which element is where.
-      float *part = p.partial + (static_cast<long long>(blockIdx.x) * 2 + (begins ? 1 : 0)) * S::kPart;
+    done(pair, begins, ends, h0, n_heads, o, m, l, cv);
+  }
+  copies_wait<0>();
+}
+
+// A partial result: fragments as they lie in the lanes, then maxima and sums of the columns.
+template <int D, int NT, int MODE>
+__device__ __forceinline__ void store_part(float *part, int lane, const float (&o)[D / 16][NT][4], const float (&m)[NT][2],
+                                           const float (&l)[NT][2], float cv) {
+  using S = Shape<D, NT, MODE>;
+  const float f = MODE == MODE_E4M3 ? cv : 1.f;
 #pragma unroll
-      for (int d = 0; d < DK; ++d) {
+  for (int d = 0; d < D / 16; ++d) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const float f = MODE == MODE_E4M3 ? cv : 1.f;
-          reinterpret_cast<float4 *>(part)[(d * NT + j) * 32 + lane] =
-              make_float4(o[d][j][0] * f, o[d][j][1] * f, o[d][j][2] * f, o[d][j][3] * f);
-        }
-      }
-      if (g == 0) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          *reinterpret_cast<float2 *>(part + S::kFrags * 128 + 8 * j + 2 * t) = make_float2(m[j][0], m[j][1]);
-          *reinterpret_cast<float2 *>(part + S::kFrags * 128 + S::kHeads + 8 * j + 2 * t) = make_float2(l[j][0], l[j][1]);
-        }
-      }
-      continue;
+    for (int j = 0; j < NT; ++j) {
+      reinterpret_cast<float4 *>(part)[(d * NT + j) * 32 + lane] =
+          make_float4(o[d][j][0] * f, o[d][j][1] * f, o[d][j][2] * f, o[d][j][3] * f);
     }
-    const long long row0 = static_cast<long long>(b) * p.heads + h0;
+  }
+  if (lane < 4) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      *reinterpret_cast<float2 *>(part + S::kFrags * 128 + 8 * j + 2 * lane) = make_float2(m[j][0], m[j][1]);
+      *reinterpret_cast<float2 *>(part + S::kFrags * 128 + S::kHeads + 8 * j + 2 * lane) = make_float2(l[j][0], l[j][1]);
+    }
+  }
+}
+
+// What a thread of a join has: the four values that a lane had of one fragment, and its two columns' maxima and sums.
+struct Joined {
+  float4 o;
+  float2 m, l;
+};
+__device__ __forceinline__ Joined nothing() {
+  return Joined{make_float4(0.f, 0.f, 0.f, 0.f), make_float2(-INFINITY, -INFINITY), make_float2(0.f, 0.f)};
+}
+__device__ __forceinline__ void add(Joined &a, const Joined &x) {
+  const float2 now = make_float2(fmaxf(a.m.x, x.m.x), fmaxf(a.m.y, x.m.y));
+  const float bx = now.x == -INFINITY ? 0.f : now.x, by = now.y == -INFINITY ? 0.f : now.y;
+  const float kx = exp2_fast(a.m.x - bx), ky = exp2_fast(a.m.y - by), ax = exp2_fast(x.m.x - bx), ay = exp2_fast(x.m.y - by);
+  a.o.x = fmaf(x.o.x, ax, a.o.x * kx);
+  a.o.y = fmaf(x.o.y, ay, a.o.y * ky);
+  a.o.z = fmaf(x.o.z, ax, a.o.z * kx);
+  a.o.w = fmaf(x.o.w, ay, a.o.w * ky);
+  a.l.x = fmaf(x.l.x, ax, a.l.x * kx);
+  a.l.y = fmaf(x.l.y, ay, a.l.y * ky);
+  a.m = now;
+}
+template <int D, int NT, int MODE>
+__device__ __forceinline__ Joined load_part(const float *part, int at) {
+  using S = Shape<D, NT, MODE>;
+  const int col = 8 * (at / 32 % NT) + 2 * (at % 4);
+  return Joined{reinterpret_cast<const float4 *>(part)[at], *reinterpret_cast<const float2 *>(part + S::kFrags * 128 + col),
+                *reinterpret_cast<const float2 *>(part + S::kFrags * 128 + S::kHeads + col)};
+}
+// The result of fragment at / 32. All lanes of the warp call it.
+template <int D, int NT, int MODE>
+__device__ __forceinline__ void store_joined(const Params &p, int b, int unit, int at, const Joined &a) {
+  using S = Shape<D, NT, MODE>;
+  const int lane = at % 32, d = at / 32 / NT, j = at / 32 % NT;
+  const int kv = unit / p.chunks, h0 = kv * p.group + unit % p.chunks * S::kHeads, n_heads = min(S::kHeads, (kv + 1) * p.group - h0);
+  const float v[4] = {a.o.x, a.o.y, a.o.z, a.o.w}, tops[2] = {a.m.x, a.m.y}, sums[2] = {a.l.x, a.l.y};
+  float inv[2];
+  // One warp for each group of heads writes the lse.
+  finish<NT>(p, static_cast<long long>(b) * p.heads + h0, d == 0 ? n_heads : 0, j, lane, tops, sums, inv);
+  store_fragment<D, MODE>(p, static_cast<long long>(b) * p.heads + h0, n_heads, j, d, lane, v, inv);
+}
+
+template <int D, int NT, int MODE>
+__global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(const Params p) {
+  using S = Shape<D, NT, MODE>;
+  constexpr int kKeys = S::kKeys, DK = D / 16;
+  extern __shared__ __align__(16) char ring[];
+  const int lane = threadIdx.x;
+  const int units = p.kv_heads * p.chunks;
+
+  // ---- the line of tiles ----
+  // Lanes take neighbouring sequences, `per_lane` each; a scan over the lanes gives each one its first tile.
+  const int per_lane = (p.batch + 31) / 32, b_lo = min(lane * per_lane, p.batch), b_hi = min(b_lo + per_lane, p.batch);
+  auto tiles_at = [&](int b) { return static_cast<long long>(tiles_of(visible(p.lengths[b], p.capacity, p.window), kKeys)) * units; };
+  long long mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) mine += tiles_at(b);
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  const long long total = __shfl_sync(0xffffffffu, upto, 31), per = per_share(total, p.blocks, p.least);
+  // The join may be set up from here on; it waits for the end of this grid before it reads.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // The lane whose sequences hold the share's first tile finds the sequence.
+  const long long t0 = per * blockIdx.x, t1 = min(total, t0 + per);
+  const bool holds = t0 < t1 && t0 >= upto - mine && t0 < upto;
+  int first_b = b_lo;
+  long long into = t0 - (upto - mine);
+  if (holds) {
+    for (long long n = tiles_at(first_b); into >= n; n = tiles_at(first_b)) {
+      into -= n;
+      ++first_b;
+    }
+  }
+  // A sequence that sees nothing gets its result here.
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    const Span s = visible(p.lengths[b], p.capacity, p.window);
+    if (s.end > s.first) continue;
+    for (int i = lane; i < p.heads * D; i += 32) store_out(p, static_cast<long long>(b) * p.heads * D + i, 0.f);
+    for (int i = lane; i < units; i += 32) p.spans[static_cast<long long>(b) * units + i] = make_int2(0, 0);
+    if (p.lse != nullptr) {
+      for (int i = lane; i < p.heads; i += 32) p.lse[static_cast<long long>(b) * p.heads + i] = -INFINITY;
+    }
+  }
+  if (t0 >= t1) return;
+  const int from = __ffs(__ballot_sync(0xffffffffu, holds)) - 1;
+  Cursor cur;
+  cur.b = __shfl_sync(0xffffffffu, first_b, from);
+  into = __shfl_sync(0xffffffffu, into, from);
+  enter(cur, p, kKeys);
+  cur.unit = static_cast<int>(into / cur.n);
+  cur.tile = static_cast<int>(into - static_cast<long long>(cur.unit) * cur.n);
+  cur.left = static_cast<int>(t1 - t0);
+  run_share<D, NT, MODE>(p, ring, cur, lane, [&](const Cursor &pair, bool begins, bool ends, int h0, int n_heads,
+                                                 float (&o)[DK][NT][4], float (&m)[NT][2], float (&l)[NT][2], float cv) {
+    if (begins && lane == 0) {
+      const int share = blockIdx.x;
+      p.spans[static_cast<long long>(pair.b) * units + pair.unit] =
+          make_int2(share, last_share(share, pair.n, pair.left, static_cast<int>(per)));
+    }
+    if (!(begins && ends)) {
+      store_part<D, NT, MODE>(p.partial + (static_cast<long long>(blockIdx.x) * 2 + (begins ? 1 : 0)) * S::kPart, lane, o, m, l, cv);
+      return;
+    }
+    const long long row0 = static_cast<long long>(pair.b) * p.heads + h0;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       float inv[2];
@@ -688,8 +750,45 @@ __global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(
 #pragma unroll
       for (int d = 0; d < DK; ++d) store_fragment<D, MODE>(p, row0, n_heads, j, d, lane, o[d][j], inv);
     }
+  });
+}
+
+// Short caches: a block has one pair, its warps take equal parts of the pair's tiles and join their results through the
+// ring's memory. One launch instead of two, for calls that are bound by latency.
+template <int D, int NT, int MODE>
+__global__ void __launch_bounds__(32 * Shape<D, NT, MODE>::kTeam) paged_short_kernel(const Params p) {
+  using S = Shape<D, NT, MODE>;
+  constexpr int DK = D / 16, kTeam = S::kTeam;
+  extern __shared__ __align__(16) char rings[];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, units = p.kv_heads * p.chunks;
+  char *const ring = rings + warp * S::kSmem;
+  Cursor cur{};
+  cur.b = blockIdx.x / units;
+  cur.unit = blockIdx.x % units;
+  enter(cur, p, S::kKeys);
+  cur.tile = cur.n * warp / kTeam;
+  cur.left = cur.n * (warp + 1) / kTeam - cur.tile;
+  float *const part = reinterpret_cast<float *>(ring);
+  static_assert(S::kPart * 4 <= S::kSmem, "a part fits the ring");
+  if (cur.left > 0) {
+    run_share<D, NT, MODE>(p, ring, cur, lane, [&](const Cursor &, bool, bool, int, int, float (&o)[DK][NT][4], float (&m)[NT][2],
+                                                   float (&l)[NT][2], float cv) {
+      copies_wait<0>();
+      __syncwarp();
+      store_part<D, NT, MODE>(part, lane, o, m, l, cv);
+    });
   }
-  copies_wait<0>();
+  __syncthreads();
+  for (int at = threadIdx.x; at < S::kFrags * 32; at += 32 * kTeam) {
+    Joined a = nothing();
+#pragma unroll
+    for (int w = 0; w < kTeam; ++w) {
+      if (cur.n * (w + 1) / kTeam > cur.n * w / kTeam) {
+        add(a, load_part<D, NT, MODE>(reinterpret_cast<const float *>(rings + w * S::kSmem), at));
+      }
+    }
+    store_joined<D, NT, MODE>(p, cur.b, cur.unit, at, a);
+  }
 }
 
 // Adds the partial results of the pairs that several warps share, in the order of the shares. A thread has the four values
@@ -698,71 +797,46 @@ template <int D, int NT, int MODE, int GROUPS>
 __global__ void __launch_bounds__(256) paged_join_kernel(const Params p) {
   using S = Shape<D, NT, MODE>;
   constexpr int kLanes = 256 / GROUPS, kAhead = 4;
-  __shared__ float4 s_o[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? kLanes : 1], s_ml[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? kLanes : 1];
+  __shared__ Joined shared[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? kLanes : 1];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 own = p.spans[blockIdx.x];
   if (own.x == own.y) return;
   const int group = threadIdx.x / kLanes, at = blockIdx.y * kLanes + threadIdx.x % kLanes;
-  const int frag = at / 32, lane = at % 32, d = frag / NT, j = frag % NT, g = lane / 4, t = lane % 4;
-  const bool has = frag < S::kFrags;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float2 top = make_float2(-INFINITY, -INFINITY), sum = make_float2(0.f, 0.f);
-  auto add = [&](const float4 &x, const float2 &m, const float2 &l) {
-    const float2 now = make_float2(fmaxf(top.x, m.x), fmaxf(top.y, m.y));
-    const float bx = now.x == -INFINITY ? 0.f : now.x, by = now.y == -INFINITY ? 0.f : now.y;
-    const float kx = exp2_fast(top.x - bx), ky = exp2_fast(top.y - by), ax = exp2_fast(m.x - bx), ay = exp2_fast(m.y - by);
-    acc.x = fmaf(x.x, ax, acc.x * kx);
-    acc.y = fmaf(x.y, ay, acc.y * ky);
-    acc.z = fmaf(x.z, ax, acc.z * kx);
-    acc.w = fmaf(x.w, ay, acc.w * ky);
-    sum.x = fmaf(l.x, ax, sum.x * kx);
-    sum.y = fmaf(l.y, ay, sum.y * ky);
-    top = now;
-  };
+  const bool has = at < S::kFrags * 32;
+  Joined a = nothing();
   if (has) {
     for (int c0 = own.x + group; c0 <= own.y; c0 += kAhead * GROUPS) {
-      float4 x[kAhead];
-      float2 m[kAhead], l[kAhead];
+      Joined x[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int c = c0 + i * GROUPS;
         if (c > own.y) break;
-        const float *part = p.partial + (static_cast<long long>(c) * 2 + place(own.x, c)) * S::kPart;
-        x[i] = reinterpret_cast<const float4 *>(part)[at];
-        m[i] = *reinterpret_cast<const float2 *>(part + S::kFrags * 128 + 8 * j + 2 * t);
-        l[i] = *reinterpret_cast<const float2 *>(part + S::kFrags * 128 + S::kHeads + 8 * j + 2 * t);
+        x[i] = load_part<D, NT, MODE>(p.partial + (static_cast<long long>(c) * 2 + place(own.x, c)) * S::kPart, at);
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         if (c0 + i * GROUPS > own.y) break;
-        add(x[i], m[i], l[i]);
+        add(a, x[i]);
       }
     }
   }
   if constexpr (GROUPS > 1) {
     const int at_s = threadIdx.x % kLanes;
-    s_o[group][at_s] = acc;
-    s_ml[group][at_s] = make_float4(top.x, top.y, sum.x, sum.y);
+    shared[group][at_s] = a;
     __syncthreads();
     if (group != 0) return;
 #pragma unroll
-    for (int i = 1; i < GROUPS; ++i) {
-      const float4 ml = s_ml[i][at_s];
-      add(s_o[i][at_s], make_float2(ml.x, ml.y), make_float2(ml.z, ml.w));
-    }
+    for (int i = 1; i < GROUPS; ++i) add(a, shared[i][at_s]);
   }
-  if (!has) return;
-  const int units = p.kv_heads * p.chunks, unit = blockIdx.x % units, b = blockIdx.x / units;
-  const int kv = unit / p.chunks, h0 = kv * p.group + unit % p.chunks * S::kHeads, n_heads = min(S::kHeads, (kv + 1) * p.group - h0);
-  const float v[4] = {acc.x, acc.y, acc.z, acc.w}, tops[2] = {top.x, top.y}, sums[2] = {sum.x, sum.y};
-  float inv[2];
-  // One warp for each group of heads writes the lse.
-  finish<NT>(p, static_cast<long long>(b) * p.heads + h0, d == 0 ? n_heads : 0, j, lane, tops, sums, inv);
-  store_fragment<D, MODE>(p, static_cast<long long>(b) * p.heads + h0, n_heads, j, d, lane, v, inv);
+  const int units = p.kv_heads * p.chunks;
+  if (has) store_joined<D, NT, MODE>(p, blockIdx.x / units, blockIdx.x % units, at, a);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
+// Keys a warp of paged_short_kernel, at most: with more, splitting over more SMs pays for a second launch. 128 elements, bf16,
+// 32 pairs, one launch against two: 128 keys 6.2 us against 9.9, 512 keys 10.3 and 10.3, 1024 keys 14.4 and 11.1.
+constexpr int kShortKeys = 64;
 // Keys that a share has at least: below that its fixed costs weigh more than the loads that another warp would take over.
 constexpr int kLeastKeys = 32;
 
@@ -795,7 +869,12 @@ int launch_join(const Params &p, cudaStream_t s) {
 template <int D, int NT, int MODE>
 int launch(Params p, cudaStream_t s) {
   using S = Shape<D, NT, MODE>;
-  auto kernel = paged_kernel<D, NT, MODE>;
+  // The lengths are on the device: what counts is the most that they can be.
+  const int longest = p.window > 0 ? std::min(p.window, p.capacity) : p.capacity;
+  const int pairs = p.batch * p.kv_heads * p.chunks;
+  // A block for each pair, no more than SMs. From half the SMs on there is less to split: twice the keys (128 pairs of 1024
+  // keys: 14.4 us against 18.0; of 2048: 24.7 and 26.8).
+  const bool is_short = pairs <= device_sm_count() && longest <= kShortKeys * S::kTeam * (2 * pairs > device_sm_count() ? 2 : 1);
   // The attribute belongs to the device's context: set once for each device.
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
@@ -803,21 +882,25 @@ int launch(Params p, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    e = cudaFuncSetAttribute(paged_kernel<D, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(paged_short_kernel<D, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTeam * S::kSmem);
     if (e != cudaSuccess) return e;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
   p.blocks = device_sm_count() * S::kBlocks;
   p.least = kLeastKeys / S::kKeys;
-  kernel<<<p.blocks, 32, S::kSmem, s>>>(p);
+  if (is_short) {
+    paged_short_kernel<D, NT, MODE><<<pairs, 32 * S::kTeam, S::kTeam * S::kSmem, s>>>(p);
+    return cudaGetLastError();
+  }
+  paged_kernel<D, NT, MODE><<<p.blocks, 32, S::kSmem, s>>>(p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  // The lengths are on the device: what counts is the most that they can be.
-  const int longest = p.window > 0 ? std::min(p.window, p.capacity) : p.capacity;
   if (longest <= S::kKeys) return 0;  // no pair has two tiles: nothing to join
   // Many parts of each of a few pairs are shared by eight sets of threads (8 pairs of 148 parts: 35 us the whole call, with one set
   // 62); few parts of many pairs are not worth the exchange (128 pairs of 9 parts: 73 us with one set, 76 with eight).
-  const int pairs = p.batch * p.kv_heads * p.chunks, shares = p.blocks;
+  const int shares = p.blocks;
   return pairs > shares / 24 ? launch_join<D, NT, MODE, 1>(p, s) : launch_join<D, NT, MODE, 8>(p, s);
 }
 

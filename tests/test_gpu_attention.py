@@ -715,3 +715,20 @@ def test_expanded_queries_and_caches_that_are_copied():
     assert c != copy.copy(c) and c == c
     with pytest.raises(ValueError, match="gradient"):
         at.KvCache(torch.zeros(2, 2, 16, 64, dtype=BF16, device="cuda", requires_grad=True), torch.zeros(2, 2, 16, 64, dtype=BF16, device="cuda"))
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("B,K,H,pages", [(1, 1, 1, 1), (2, 2, 12, 7), (37, 4, 16, 20), (37, 4, 16, 33), (149, 1, 8, 5), (5, 1, 40, 16)])
+def test_paged_attention_one_launch_and_two(cache, D, B, K, H, pages):
+    """Calls on both sides of the rule that chooses between a block for each pair and shares of all tiles."""
+    from rocshmem_b200.ops import attention as at
+    g = torch.Generator().manual_seed(B + pages)
+    lengths = [int(n) for n in torch.randint(0, 32 * pages + 1, (B,), generator=g)]
+    lengths[B // 2] = 32 * pages
+    c, q, table, ln = paged_case(lengths, H, K, D, 32, BF16, cache, seed=pages, extra_pages=0)
+    out, lse = at.paged_attention(q, c, table, ln, return_lse=True)
+    check_paged(at, c, q, table, ln, out, lse)
+    exact = torch.empty(q.shape, device="cuda")
+    at.paged_attention(q, c, table, ln, out=exact)
+    assert torch.equal(exact.to(BF16), out)
