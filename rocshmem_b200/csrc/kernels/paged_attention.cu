@@ -103,12 +103,19 @@ __device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t &lo, uint32_t &h
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
       : "=r"(lo), "=r"(hi) : "r"(w));
 }
-// c tanh(x / c) in base 2, with to = 2 log2(e) / c and back = c log2(e): tanh y = 1 - 2 / (exp(2y) + 1). Off by 2^-22 of c, which
-// is what counts in an exponent; tanhf, exact near zero too, cost a fifth of the kernel's time.
-__device__ __forceinline__ float cap2(float x, float to, float back) {
+__device__ __forceinline__ float reciprocal(float x) {
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(exp2_fast(x * to) + 1.f));
-  return fmaf(-2.f * back, r, back);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// c tanh(x / c) in base 2, with in = 1 / c and back = c log2(e). Up to one, where most scores are, tanh y is Lambert's continued
+// fraction y / (1 + y^2 / (3 + y^2 / (5 + y^2 / (7 + y^2 / 9)))) as a quotient (off by 6e-8 of it at most), beyond 1 - 2 / (exp(2y) +
+// 1), whose error there is one of the last bits too. tanhf cost a fifth of the kernel's time.
+__device__ __forceinline__ float cap2(float x, float in, float back) {
+  const float y = x * in, y2 = y * y;
+  const float near = y * fmaf(y2 + 105.f, y2, 945.f) * reciprocal(fmaf(fmaf(15.f, y2, 420.f), y2, 945.f));
+  const float far = fmaf(-2.f, reciprocal(exp2_fast(y * (2.f * kLog2e)) + 1.f), 1.f);
+  return back * (fabsf(y) <= 1.f ? near : far);
 }
 
 // Shared memory and tile sizes of one instantiation. Rows are padded so that the accesses of a fragment fall into
@@ -320,7 +327,7 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
   int stage = 0, load_stage = S::kStages - 1;
 
   // ---- pairs ----
-  const float cap_to = 2.f * kLog2e / p.softcap, cap_back = p.softcap * kLog2e;
+  const float cap_in = 1.f / p.softcap, cap_back = p.softcap * kLog2e;
   const int k_lane = (lane % 16) * S::kPitchK + (lane / 16) * 16;                       // ldmatrix: 16 keys x 16 elements
   const int v_lane = ((lane / 16) * 8 + lane % 8) * S::kPitchV + (lane / 8 % 2) * 16;   // transposed
   while (cur.left > 0) {
@@ -456,7 +463,7 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 float x = s[i][j][2 * r + c] * q_scale[j][c] * f;
-                if (p.softcap > 0.f) x = cap2(x, cap_to, cap_back);
+                if (p.softcap > 0.f) x = cap2(x, cap_in, cap_back);
                 x = seen ? x : -INFINITY;
                 s[i][j][2 * r + c] = x;
                 top[j][c] = fmaxf(top[j][c], x);
