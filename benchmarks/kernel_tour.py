@@ -3,7 +3,7 @@
 a quick timing table, and the target of profiler captures (one kernel family per capture, selected by name).
 
     python benchmarks/kernel_tour.py                          # all families, CUDA-event times
-    python benchmarks/kernel_tour.py --only collectives       # comma list of: collectives, ep, moe, tp
+    python benchmarks/kernel_tour.py --only collectives       # comma list of: collectives, ep, moe, tp, attention
     ncu --set full --clock-control none -k regex:allreduce_two_shot -c 2 -o <out> \
         python benchmarks/kernel_tour.py --only collectives --reps 1
 
@@ -15,6 +15,8 @@ Families:
                block-scaled forms (gathered e4m3 rows, quantising epilogue) (32 experts x ~1024 rows, hidden 7168, intermediate 2048)
   tp           all-gather -> GEMM and GEMM -> reduce-scatter on a team of one (the tensor-core side of the fused
                kernels; the NVLink side needs several GPUs and is timed by benchmarks/model_bench.py)
+  attention    norm and rotation of query and key heads (forward, and with the backward pass), writes into and reads from a
+               paged cache, attention of one new token over it (bf16, e4m3), the join of partial results
 """
 from __future__ import annotations
 
@@ -29,7 +31,7 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 import rocshmem_b200 as shm  # noqa: E402
 from rocshmem_b200.ops import collectives as coll  # noqa: E402
-from rocshmem_b200.ops import gemm, moe  # noqa: E402
+from rocshmem_b200.ops import attention, gemm, moe  # noqa: E402
 
 
 def timed(fn, reps, flush):
@@ -150,9 +152,44 @@ def tour_tp(reps, flush, rows):
         shm.finalize()
 
 
+def tour_attention(reps, flush, rows):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    T, H, K, D, size = 16384, 32, 8, 128, 64
+
+    def add(name, us, nbytes):
+        rows.append({"family": "attention", "kernel": name, "us": us, "gbs": nbytes / us / 1e3})
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").to(torch.bfloat16)
+
+    q, k, v = randn(T, H, D), randn(T, K, D), randn(T, K, D)
+    wq, wk = torch.ones(D, device="cuda"), torch.ones(D, device="cuda")
+    pos, table = torch.arange(T, device="cuda"), attention.rope_table(T, D, device="cuda")
+    n = T * (H + K) * D * 2
+    add("norm and rotation, forward", timed(lambda: attention.qk_norm_rope(q, k, wq, wk, pos, table), reps, flush), 2 * n)
+    leaves = [t.clone().requires_grad_() for t in (q, k, wq, wk)]
+    out = attention.qk_norm_rope(*leaves, pos, table)
+    gq, gk = randn(T, H, D), randn(T, K, D)
+    add("norm and rotation, backward", timed(lambda: torch.autograd.grad(out, leaves, (gq, gk), retain_graph=True), reps, flush), 3 * n)
+    slots = torch.randperm(T, generator=g, device="cuda")
+    for dtype, label, width in ((torch.bfloat16, "bf16", 2 * D), (torch.float8_e4m3fn, "e4m3", D + 4)):
+        pages = 64 * 128
+        cache = attention.KvCache.allocate(pages, size, K, D, dtype)
+        both = 2 * T * K * (2 * D + width)
+        add(f"cache write, {label}", timed(lambda: attention.kv_cache_write(cache, k, v, slots), reps, flush), both)
+        add(f"cache read, {label}", timed(lambda: attention.kv_cache_read(cache, slots), reps, flush), both)
+        pages_of = torch.randperm(pages, generator=g, device="cuda").view(64, 128).to(torch.int32)
+        lengths = torch.full((64,), 128 * size, dtype=torch.int32, device="cuda")
+        add(f"attention of one token, 64 x {128 * size} tokens, {label}",
+            timed(lambda: attention.paged_attention(q[:64], cache, pages_of, lengths), reps, flush), 2 * 64 * 128 * size * K * width)
+    outs, lses = torch.randn(8, 512, H, D, generator=g, device="cuda"), torch.randn(8, 512, H, generator=g, device="cuda")
+    add("join of 8 parts, 512 x 32 heads", timed(lambda: attention.attention_join(outs, lses, dtype=torch.bfloat16), reps, flush),
+        512 * H * (8 * (4 * D + 4) + 2 * D + 4))
+
+
 def main() -> int:
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
-    ap.add_argument("--only", default="collectives,ep,moe,tp")
+    ap.add_argument("--only", default="collectives,ep,moe,tp,attention")
     ap.add_argument("--reps", type=int, default=3)
     ap.add_argument("--out", default="")
     args = ap.parse_args()
@@ -168,6 +205,8 @@ def main() -> int:
         tour_moe(args.reps, flush, rows)
     if "tp" in only:
         tour_tp(args.reps, flush, rows)
+    if "attention" in only:
+        tour_attention(args.reps, flush, rows)
     for r in rows:
         print(json.dumps({k: (round(v, 1) if isinstance(v, float) else v) for k, v in r.items()}))
     if args.out:

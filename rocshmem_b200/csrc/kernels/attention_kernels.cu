@@ -104,7 +104,7 @@ struct Side {
 };
 
 template <typename T, typename W, int LANES, int ROWS, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads, 5) norm_rope_kernel(NormRope<T, W> a, unsigned q_items, unsigned items, T *q_out,
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5) norm_rope_kernel(NormRope<T, W> a, unsigned q_items, unsigned items, T *q_out,
                                                              T *k_out) {
   const int lane = threadIdx.x % LANES;
   const Place<INTERLEAVED> at(lane, a.dim, a.rotary);

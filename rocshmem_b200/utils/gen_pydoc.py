@@ -9,9 +9,10 @@ import sys
 from typing import List
 
 MODULES = ["rocshmem_b200.runtime", "rocshmem_b200.ops.collectives", "rocshmem_b200.ops.moe", "rocshmem_b200.ops.moe_host",
-           "rocshmem_b200.ops.gemm", "rocshmem_b200.ops.host_algorithms", "rocshmem_b200.models.moe_ffn",
+           "rocshmem_b200.ops.gemm", "rocshmem_b200.ops.attention", "rocshmem_b200.ops.host_algorithms", "rocshmem_b200.models.moe_ffn",
            "rocshmem_b200.models.tp_mlp", "rocshmem_b200.parallel.layout", "rocshmem_b200.parallel.pipeline",
-           "rocshmem_b200.parallel.membership", "rocshmem_b200.parallel.elastic", "rocshmem_b200.parallel.data_parallel", "rocshmem_b200.parallel.ulysses", "rocshmem_b200.parallel.ring", "rocshmem_b200.utils.checkpoint", "rocshmem_b200.utils.trace",
+           "rocshmem_b200.parallel.membership", "rocshmem_b200.parallel.elastic", "rocshmem_b200.parallel.data_parallel", "rocshmem_b200.parallel.ulysses", "rocshmem_b200.parallel.ring",
+           "rocshmem_b200.parallel.context", "rocshmem_b200.utils.checkpoint", "rocshmem_b200.utils.trace",
            "rocshmem_b200.utils.roofline", "rocshmem_b200.baselines.nccl_collectives", "rocshmem_b200.baselines.tp_mlp",
            "rocshmem_b200.baselines.moe", "rocshmem_b200.baselines.ep"]
 
