@@ -65,12 +65,18 @@ __device__ __forceinline__ void unpack8(const Raw8<__half> &r, float (&x)[8]) {
     x[2 * i] = f.x, x[2 * i + 1] = f.y;
   }
 }
+// Four e4m3 codes as two pairs of fp16 values (exact).
+__device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
+}
 __device__ __forceinline__ void unpack8(const Raw8<e4m3> &r, float (&x)[8]) {
-  const uint32_t w[2] = {r.a.x, r.a.y};
+  uint32_t w[4];
+  e4m3_pairs(r.a.x, w[0], w[1]);
+  e4m3_pairs(r.a.y, w[2], w[3]);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i / 2] >> (16 * (i % 2))), __NV_E4M3);
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
     x[2 * i] = f.x, x[2 * i + 1] = f.y;
   }
 }

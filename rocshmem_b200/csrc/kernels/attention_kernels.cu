@@ -104,16 +104,16 @@ struct Side {
 };
 
 template <typename T, typename W, int LANES, int ROWS, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5) norm_rope_kernel(NormRope<T, W> a, unsigned q_items, unsigned items, T *q_out,
-                                                             T *k_out) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5) norm_rope_kernel(NormRope<T, W> a, unsigned q_items, unsigned items,
+                                                                                       Divisor q_chunks, Divisor k_chunks, T *q_out, T *k_out) {
   const int lane = threadIdx.x % LANES;
   const Place<INTERLEAVED> at(lane, a.dim, a.rotary);
   // All lanes of a warp take part in every shuffle: groups past the last item have no rows.
   const unsigned mine = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   const bool is_q = mine < q_items;
   const Side<T, W> side(a, is_q);
-  const unsigned item = is_q ? mine : min(mine, items - 1) - q_items, chunks = (side.heads + ROWS - 1) / ROWS, t = item / chunks;
-  const int h0 = (item - t * chunks) * ROWS, left = mine < items && at.in_row ? side.heads - h0 : 0;
+  const unsigned item = is_q ? mine : min(mine, items - 1) - q_items, t = divide(item, is_q ? q_chunks : k_chunks);
+  const int h0 = (item - t * (is_q ? q_chunks.d : k_chunks.d)) * ROWS, left = mine < items && at.in_row ? side.heads - h0 : 0;
   const long long pos = load_index(a.positions, a.wide_positions, t);
   const T *const rows = side.x + t * side.token + h0 * side.head;
   RawRow<T> raw[ROWS];
@@ -283,6 +283,7 @@ struct Cache {
   float *k_scale, *v_scale;
   int slots;
   int kv_heads, shift, dim;
+  Divisor each;  // two times kv_heads
 };
 
 // The head and the first of its tokens that a group of lanes has.
@@ -291,9 +292,21 @@ struct Row {
   int head;
   bool is_v;
 };
-__device__ __forceinline__ Row row_of(unsigned group, int tokens_each, int kv_heads) {
-  const unsigned each = 2 * kv_heads, chunk = group / each, h = group - chunk * each;
-  return Row{static_cast<long long>(chunk) * tokens_each, static_cast<int>(h < kv_heads ? h : h - kv_heads), h >= kv_heads};
+__device__ __forceinline__ Row row_of(unsigned group, int tokens_each, const Divisor &each) {  // each: two times the heads
+  const unsigned chunk = divide(group, each), h = group - chunk * each.d, heads = each.d / 2;
+  return Row{static_cast<long long>(chunk) * tokens_each, static_cast<int>(h < heads ? h : h - heads), h >= heads};
+}
+
+// The cache rows of the group's tokens: lane r looks up token r and hands it to the others. All lanes of the warp call it.
+template <int LANES, int ROWS, typename C>
+__device__ __forceinline__ void look_up_rows(const C &c, const Row &w, const void *slots, int wide_slots, int tokens, int (&row)[ROWS]) {
+  const int lane = threadIdx.x % LANES;
+  int mine = -1;
+  if (lane < ROWS && w.token + lane < tokens) {
+    mine = slot_row(load_index(slots, wide_slots, static_cast<int>(w.token) + lane), c.slots, c.shift, c.kv_heads, w.head);
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) row[r] = __shfl_sync(0xffffffffu, mine, r, LANES);
 }
 
 // A group of lanes takes one head's row (of k or of v) of ROWS neighbouring tokens, their loads first. Neighbouring groups
@@ -303,26 +316,23 @@ __device__ __forceinline__ Row row_of(unsigned group, int tokens_each, int kv_he
 // below which 448 / m would overflow. The largest magnitude is that of the bits, so that a NaN or infinity becomes m, and
 // with it the factor: such a row reads back as NaN.
 template <typename T, typename C, int LANES, int ROWS>
-__global__ void __launch_bounds__(kThreads) kv_write_kernel(Cache<C> c, const T *k, const T *v, long long k_token,
+__global__ void __launch_bounds__(kThreads, 6) kv_write_kernel(Cache<C> c, const T *k, const T *v, long long k_token,
                                                             long long k_head, long long v_token, long long v_head,
                                                             const void *slots, int wide_slots, int tokens) {
   constexpr bool kQuantize = sizeof(C) == 1;
   const int lane = threadIdx.x % LANES;
   const bool in_row = 8 * lane < c.dim;
-  const Row w = row_of(blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES, ROWS, c.kv_heads);
+  const Row w = row_of(blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES, ROWS, c.each);
   const T *from = (w.is_v ? v + w.head * v_head : k + w.head * k_head) + w.token * (w.is_v ? v_token : k_token);
   const long long step = w.is_v ? v_token : k_token;
   Raw8<T> raw[ROWS];
   int to[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    to[r] = -1;
     raw[r] = Raw8<T>{};
-    if (w.token + r < tokens) {
-      if (in_row) raw[r] = load8(from + r * step, lane);
-      to[r] = slot_row(load_index(slots, wide_slots, static_cast<int>(w.token) + r), c.slots, c.shift, c.kv_heads, w.head);
-    }
+    if (in_row && w.token + r < tokens) raw[r] = load8(from + r * step, lane);
   }
+  look_up_rows<LANES>(c, w, slots, wide_slots, tokens, to);
   C *const base = (w.is_v ? c.v : c.k) + 8 * lane;
   float *const scales = w.is_v ? c.v_scale : c.k_scale;
 #pragma unroll
@@ -357,19 +367,15 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(Cache<C> c, T *k_out,
                                                            int wide_slots, int tokens) {
   const int lane = threadIdx.x % LANES;
   const bool in_row = 8 * lane < c.dim;
-  const Row w = row_of(blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES, ROWS, c.kv_heads);
+  const Row w = row_of(blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES, ROWS, c.each);
   const C *base = w.is_v ? c.v : c.k;
   T *out = (w.is_v ? v_out : k_out) + (w.token * c.kv_heads + w.head) * c.dim + 8 * lane;
   const long long step = static_cast<long long>(c.kv_heads) * c.dim;
-  if (!in_row) return;
   Raw8<C> raw[ROWS];
   float factor[ROWS];
   int from[ROWS];
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    from[r] = w.token + r < tokens ? slot_row(load_index(slots, wide_slots, static_cast<int>(w.token) + r), c.slots, c.shift,
-                                              c.kv_heads, w.head) : -1;
-  }
+  look_up_rows<LANES>(c, w, slots, wide_slots, tokens, from);
+  if (!in_row) return;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     raw[r] = Raw8<C>{};
@@ -386,7 +392,10 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(Cache<C> c, T *k_out,
     unpack8(raw[r], x);
     if constexpr (sizeof(C) == 1) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= factor[r];
+      for (int i = 0; i < 4; ++i) {
+        const float2 y = mul2(make_float2(x[2 * i], x[2 * i + 1]), both(factor[r]));
+        x[2 * i] = y.x, x[2 * i + 1] = y.y;
+      }
     }
     store8(out + r * step, x);
   }
@@ -519,7 +528,8 @@ int with_cache(const KvCacheArgs &c, F f) {
   auto args = [&](auto tag) {
     using C = typename decltype(tag)::type;
     return Cache<C>{static_cast<C *>(c.k), static_cast<C *>(c.v), c.k_scale, c.v_scale,
-                    c.pages << c.page_shift, c.kv_heads, c.page_shift, c.dim};
+                    c.pages << c.page_shift, c.kv_heads, c.page_shift, c.dim,
+                    divisor(2 * static_cast<uint32_t>(c.kv_heads))};
   };
   switch (c.type) {
     case ATTN_BF16: return f(args(Tag<__nv_bfloat16>{}), Tag<__nv_bfloat16>{});
@@ -555,8 +565,9 @@ int qk_norm_rope(const NormRopeArgs &a, void *q_out, void *k_out, void *stream) 
         if (!blocks) return cudaErrorInvalidValue;
         norm_rope_kernel<T, W, kLanes, kRows, decltype(pairs)::value != 0>
             <<<blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(norm_rope_args<T, W>(a), static_cast<unsigned>(q_items),
-                                                                         static_cast<unsigned>(items), static_cast<T *>(q_out),
-                                                                         static_cast<T *>(k_out));
+                                                                         static_cast<unsigned>(items), divisor((a.q_heads + kRows - 1) / kRows),
+                                                                         divisor((a.k_heads + kRows - 1) / kRows),
+                                                                         static_cast<T *>(q_out), static_cast<T *>(k_out));
         return cudaGetLastError();
       };
       // One row a group while that leaves SMs without work, four rows in flight beyond.

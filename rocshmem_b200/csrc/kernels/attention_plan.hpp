@@ -51,6 +51,21 @@ ATTN_HD int place(long long first, long long c) { return c > first ? 0 : 1; }
 // The last share that a pair of n tiles lies in which begins in share `share` with `left` of the share's tiles left.
 ATTN_HD int last_share(int share, int n, int left, int per) { return n > left ? share + (n - left + per - 1) / per : share; }
 
+// Division of numbers below 2^31 by one divisor, by a multiplication (Granlund and Montgomery): with l = ceil(log2 d) and m =
+// floor(2^32 (2^l - d) / d) + 1, n / d = (floor(m n / 2^32) + n) >> l. A division proper takes 20 instructions, as many as a
+// fifth of what a row of a cache write needs.
+struct Divisor {
+  uint32_t d, m, l;
+};
+inline Divisor divisor(uint32_t d) {
+  uint32_t l = 0;
+  while ((1ull << l) < d) ++l;
+  return Divisor{d, static_cast<uint32_t>(((1ull << 32) * ((1ull << l) - d)) / d + 1), l};
+}
+ATTN_HD uint32_t divide(uint32_t n, const Divisor &v) {
+  return (static_cast<uint32_t>((static_cast<unsigned long long>(v.m) * n) >> 32) + n) >> v.l;
+}
+
 // Row (of `dim` elements) of position `pos` in a cache [pages, kv_heads, page_size, dim], or -1 where the position is
 // not visible or its page is no page of the cache. page_size = 1 << shift.
 ATTN_HD int page_row(int page, int num_pages, int pos, int shift, int kv_heads, int head) {

@@ -98,11 +98,6 @@ __device__ __forceinline__ void unpack2(uint32_t w, float &lo, float &hi) {
     lo = f.x, hi = f.y;
   }
 }
-// Four e4m3 codes as two pairs of fp16 values (exact).
-__device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t &lo, uint32_t &hi) {
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-      : "=r"(lo), "=r"(hi) : "r"(w));
-}
 __device__ __forceinline__ float reciprocal(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

@@ -54,6 +54,20 @@ void check_rows() {
   CHECK(slot_row(slots, slots, 4, 2, 1) == -1);
 }
 
+void check_division() {
+  std::mt19937 rng(9);
+  for (uint32_t d = 1; d < 5000; ++d) {
+    const Divisor v = divisor(d);
+    for (uint32_t n : {0u, 1u, d - 1, d, d + 1, 2 * d - 1, 2 * d, 0x7fffffffu, 0x7fffffffu - d, 0x7fffffffu / d * d, 0x7fffffffu / d * d - 1,
+                       static_cast<uint32_t>(rng() >> 1), static_cast<uint32_t>(rng() >> 9), static_cast<uint32_t>(rng() >> 20)}) {
+      if (n <= 0x7fffffffu) CHECK(divide(n, v) == n / d);
+    }
+  }
+  for (uint32_t d : {1u << 20, (1u << 20) + 1, (1u << 21) - 1, 1u << 21, 0x7ffffffeu, 0x7fffffffu}) {
+    for (uint32_t n : {0u, d - 1, d, 0x7fffffffu}) CHECK(divide(n, divisor(d)) == n / d);
+  }
+}
+
 void check_split(const std::vector<int> &lengths, int capacity, int window, int units, int shares, int least, int tile) {
   std::vector<long long> bases;
   long long total = 0;
@@ -94,6 +108,7 @@ void check_split(const std::vector<int> &lengths, int capacity, int window, int 
 int main() {
   check_spans();
   check_rows();
+  check_division();
   std::mt19937 rng(5);
   for (int round = 0; round < 3000; ++round) {
     std::vector<int> lengths(1 + rng() % 40);
