@@ -20,7 +20,12 @@
 // barrier. A pair that lies in several shares leaves unnormalised partial results, which paged_join_kernel adds in the order of the
 // shares: results do not depend on which warp is done first.
 //
-// e4m3 caches: codes become fp16 exactly (cvt), a key's factor multiplies its score, a value's factor its probability.
+// e4m3 caches: codes become fp16 exactly (cvt), a key's factor multiplies its score, a value's factor its probability. They are
+// bound by instructions as much as by memory: 32 keys a step need 650 (two steps of 16 keys took 15 % longer).
+//
+// Measured on one B200, 128 elements a head: 64 sequences of 1024 - 4096 tokens, 32 / 8 heads, bf16, 116 us for 676 MB (5.8 TB/s; a
+// device copy: 6.4); two sequences of 130 - 520 thousand, 64 / 8 heads, e4m3, 307 us for 1.94 GB (6.3). Without the join, 111 and
+// 302. What is left in the first is the start, 4 us until data arrives, and the SMs that end last (see Shape).
 #include "attention_common.cuh"
 
 #include <atomic>
