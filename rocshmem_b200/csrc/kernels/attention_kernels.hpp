@@ -56,8 +56,8 @@ struct PagedAttentionArgs {
   void *out;   // [batch, heads, dim]
   float *lse;  // [batch, heads] or null
 };
-// Bytes of workspace that a call needs, 0 when the sizes are refused.
-size_t paged_attention_workspace(const KvCacheArgs &c, int batch, int heads);
+// Bytes of workspace that a call needs (which may be none); 0 when the sizes are refused.
+size_t paged_attention_workspace(const KvCacheArgs &c, const PagedAttentionArgs &a);
 int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *workspace, size_t workspace_bytes,
                     void *stream);
 

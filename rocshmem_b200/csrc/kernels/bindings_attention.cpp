@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -19,7 +20,6 @@
 #include <string>
 #include <tuple>
 #include <utility>
-#include <vector>
 
 #include "attention_kernels.hpp"
 
@@ -200,41 +200,66 @@ std::pair<Tensor, Tensor> py_qk_norm_rope(const Tensor &q, const Tensor &k, cons
   return {q_out, k_out};
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> py_qk_norm_rope_backward(const Tensor &gq, const Tensor &gk, const Tensor &q,
-                                                                    const Tensor &k, const Tensor &q_weight,
-                                                                    const Tensor &k_weight, const Tensor &positions,
-                                                                    const Tensor &table, double eps, bool interleaved) {
-  const NormRopeArgs a = norm_rope_args(q, k, q_weight, k_weight, positions, table, eps, interleaved);
-  const Here here(q);
-  // Gradients come in any layout (an expanded one behind a sum, for instance); the kernel reads plain rows.
-  auto plain = [](const Tensor &g, const Tensor &like) {
-    if (g.sizes() != like.sizes() || g.scalar_type() != like.scalar_type() || g.device() != like.device()) {
-      bad_value("qk_norm_rope: a gradient does not match its output");
-    }
-    return g.is_contiguous() && aligned(g) ? g : g.clone(at::MemoryFormat::Contiguous);
-  };
-  const Tensor pq = plain(gq, q), pk = plain(gk, k);
-  Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
-  Tensor dwq = at::empty(q_weight.sizes(), q_weight.options()), dwk = at::empty(k_weight.sizes(), k_weight.options());
-  Tensor workspace = at::empty({static_cast<int64_t>(qk_norm_rope_workspace(a.dim))}, table.options());
-  check(qk_norm_rope_backward(a, data(pq), data(pk), data(dq), data(dk), data(dwq), data(dwk),
-                              static_cast<float *>(data(workspace)), here.stream), "qk_norm_rope_backward");
-  return {dq, dk, dwq, dwk};
-}
-
 // A leaf whose gradients an eager graph, alive at the time, accumulates on another stream cannot take part in a captured
 // backward pass: the engine would make that stream wait for the captured one, which ends the process. Refused instead.
-void check_capture(const std::vector<Tensor> &tensors) {
-  for (const Tensor &t : tensors) {
-    if (!t.requires_grad() || !t.is_leaf()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+void check_capture(void *stream, int device, std::initializer_list<const Tensor *> tensors) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  check(cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &status), "qk_norm_rope");
+  if (status == cudaStreamCaptureStatusNone) return;
+  for (const Tensor *t : tensors) {
+    if (!t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
     if (!node) continue;
-    const auto stream = node->stream();
-    if (stream.has_value() && *stream != c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap()) {
+    const auto of_node = node->stream();
+    if (of_node.has_value() && *of_node != c10::cuda::getCurrentCUDAStream(device).unwrap()) {
       throw std::runtime_error("qk_norm_rope: a graph of the same leaves from outside the capture is alive; drop it (its outputs "
                                "and losses) before a backward pass is captured");
     }
   }
+}
+
+struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k,
+                                                const Tensor &q_weight, const Tensor &k_weight, const Tensor &positions,
+                                                const Tensor &table, double eps, bool interleaved) {
+    ctx->save_for_backward({q, k, q_weight, k_weight, positions, table});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    auto both = py_qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved);
+    return {both.first, both.second};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    if (at::GradMode::is_enabled()) throw std::runtime_error("qk_norm_rope can be differentiated once: create_graph is refused");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &q_weight = saved[2], &k_weight = saved[3], &table = saved[5];
+    const NormRopeArgs a = norm_rope_args(q, k, q_weight, k_weight, saved[4], table, ctx->saved_data["eps"].toDouble(),
+                                          ctx->saved_data["interleaved"].toBool());
+    const Here here(q);
+    // Gradients come in any layout (an expanded one behind a sum, for instance); the kernel reads plain rows.
+    auto plain = [](const Tensor &g) { return g.is_contiguous() && aligned(g) ? g : g.clone(at::MemoryFormat::Contiguous); };
+    const Tensor gq = plain(grads[0]), gk = plain(grads[1]);
+    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
+    Tensor dwq = at::empty(q_weight.sizes(), q_weight.options()), dwk = at::empty(k_weight.sizes(), k_weight.options());
+    Tensor workspace = at::empty({static_cast<int64_t>(qk_norm_rope_workspace(a.dim))}, table.options());
+    check(qk_norm_rope_backward(a, data(gq), data(gk), data(dq), data(dk), data(dwq), data(dwk),
+                                static_cast<float *>(data(workspace)), here.stream), "qk_norm_rope_backward");
+    return {dq, dk, dwq, dwk, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::pair<Tensor, Tensor> py_qk_norm_rope_any(const Tensor &q, const Tensor &k, const Tensor &q_weight, const Tensor &k_weight,
+                                              const Tensor &positions, const Tensor &table, double eps, bool interleaved) {
+  if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || q_weight.requires_grad() || k_weight.requires_grad())) {
+    return py_qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved);
+  }
+  norm_rope_args(q, k, q_weight, k_weight, positions, table, eps, interleaved);  // refused before a graph is begun
+  {
+    const Here here(q);
+    check_capture(here.stream, q.device().index(), {&q, &k, &q_weight, &k_weight});
+  }
+  auto both = NormRopeFunction::apply(q, k, q_weight, k_weight, positions, table, eps, interleaved);
+  return {both[0], both[1]};
 }
 
 // ---- the paged cache --------------------------------------------------------------------------------------------------
@@ -374,12 +399,13 @@ std::pair<Tensor, OptTensor> py_paged_attention(const Tensor &q, const Cache &c,
   Tensor out = out_given ? *out_given : at::empty(q.sizes(), q.options());
   OptTensor lse = lse_given;
   if (!lse && want_lse) lse = at::empty(q.sizes().slice(0, 2), fp32);
-  const size_t bytes = paged_attention_workspace(p.cache, p.args.batch, p.args.heads);
-  Tensor workspace = at::empty({static_cast<int64_t>(bytes / 4 + 1)}, fp32);
+  const size_t bytes = paged_attention_workspace(p.cache, p.args);
+  Tensor workspace;
+  if (bytes > 0) workspace = at::empty({static_cast<int64_t>(bytes / 4)}, fp32);
   p.args.out = data(out);
   p.args.out_type = code(out.scalar_type());
   p.args.lse = lse ? static_cast<float *>(data(*lse)) : nullptr;
-  check(paged_attention(p.cache, p.args, data(workspace), bytes, here.stream), "paged_attention");
+  check(paged_attention(p.cache, p.args, bytes > 0 ? data(workspace) : nullptr, bytes, here.stream), "paged_attention");
   return {out, lse};
 }
 
@@ -427,9 +453,7 @@ PYBIND11_MODULE(_A, m) {
     cache_args(c);
     return c;
   }));
-  m.def("qk_norm_rope", &py_qk_norm_rope);
-  m.def("qk_norm_rope_backward", &py_qk_norm_rope_backward);
-  m.def("check_capture", &check_capture);
+  m.def("qk_norm_rope", &py_qk_norm_rope_any);
   m.def("kv_cache_write", &py_kv_cache_write);
   m.def("kv_cache_read", &py_kv_cache_read);
   m.def("check_paged", [](const Tensor &q, const Cache &c, const Tensor &table, const Tensor &lengths,

@@ -462,7 +462,7 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
             for (int j = 0; j < NT; ++j) {
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                float x = s[i][j][2 * r + c] * q_scale[j][c] * f;
+                float x = s[i][j][2 * r + c] * (q_scale[j][c] * f);
                 if (p.softcap > 0.f) x = cap2(x, cap_in, cap_back);
                 x = seen ? x : -INFINITY;
                 s[i][j][2 * r + c] = x;
@@ -866,22 +866,29 @@ auto with_shape(int dim, int group, int cache_type, F f) {
   return dim == 64 ? modes(Int<64>{}) : dim == 96 ? modes(Int<96>{}) : dim == 128 ? modes(Int<128>{}) : modes(Int<256>{});
 }
 
+int pairs_of(const Params &p) { return p.batch * p.kv_heads * p.chunks; }
+
+// The lengths are on the device: what counts on the host is the most that they can be.
+int longest_of(const Params &p) { return p.window > 0 ? std::min(p.window, p.capacity) : p.capacity; }
+
+// A block for each pair, no more than SMs. From half the SMs on there is less to split: twice the keys (128 pairs of 1024
+// keys: 14.4 us against 18.0; of 2048: 24.7 and 26.8).
+template <typename S>
+bool is_short(const Params &p) {
+  const int pairs = pairs_of(p), sms = device_sm_count();
+  return pairs <= sms && longest_of(p) <= kShortKeys * S::kTeam * (2 * pairs > sms ? 2 : 1);
+}
+
 template <int D, int NT, int MODE, int GROUPS>
 int launch_join(const Params &p, cudaStream_t s) {
   constexpr int kLanes = 256 / GROUPS;
-  const dim3 grid(static_cast<unsigned>(p.batch) * p.kv_heads * p.chunks, (Shape<D, NT, MODE>::kFrags * 32 + kLanes - 1) / kLanes);
+  const dim3 grid(static_cast<unsigned>(pairs_of(p)), (Shape<D, NT, MODE>::kFrags * 32 + kLanes - 1) / kLanes);
   return launch_after(paged_join_kernel<D, NT, MODE, GROUPS>, grid, 256, s, p);
 }
 
 template <int D, int NT, int MODE>
 int launch(Params p, cudaStream_t s) {
   using S = Shape<D, NT, MODE>;
-  // The lengths are on the device: what counts is the most that they can be.
-  const int longest = p.window > 0 ? std::min(p.window, p.capacity) : p.capacity;
-  const int pairs = p.batch * p.kv_heads * p.chunks;
-  // A block for each pair, no more than SMs. From half the SMs on there is less to split: twice the keys (128 pairs of 1024
-  // keys: 14.4 us against 18.0; of 2048: 24.7 and 26.8).
-  const bool is_short = pairs <= device_sm_count() && longest <= kShortKeys * S::kTeam * (2 * pairs > device_sm_count() ? 2 : 1);
   // The attribute belongs to the device's context: set once for each device.
   static std::atomic<uint64_t> ready{0};
   int dev = 0;
@@ -897,14 +904,15 @@ int launch(Params p, cudaStream_t s) {
   }
   p.blocks = device_sm_count() * S::kBlocks;
   p.least = kLeastKeys / S::kKeys;
-  if (is_short) {
+  const int pairs = pairs_of(p);
+  if (is_short<S>(p)) {
     paged_short_kernel<D, NT, MODE><<<pairs, 32 * S::kTeam, S::kTeam * S::kSmem, s>>>(p);
     return cudaGetLastError();
   }
   paged_kernel<D, NT, MODE><<<p.blocks, 32, S::kSmem, s>>>(p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  if (longest <= S::kKeys) return 0;  // no pair has two tiles: nothing to join
+  if (longest_of(p) <= S::kKeys) return 0;  // no pair has two tiles: nothing to join
   // Many parts of each of a few pairs are shared by eight sets of threads (8 pairs of 148 parts: 35 us the whole call, with one set
   // 62); few parts of many pairs are not worth the exchange (128 pairs of 9 parts: 73 us with one set, 76 with eight).
   const int shares = p.blocks;
@@ -912,41 +920,17 @@ int launch(Params p, cudaStream_t s) {
 }
 
 // The pairs' spans, in whole 16 bytes.
-size_t span_bytes(const KvCacheArgs &c, int batch, int heads) {
-  const int group = heads / c.kv_heads, each = heads_per_unit(group, c.dim);
-  return (static_cast<size_t>(batch) * c.kv_heads * ((group + each - 1) / each) + 1) / 2 * 16;
-}
+size_t span_bytes(const Params &p) { return (static_cast<size_t>(pairs_of(p)) + 1) / 2 * 16; }
 
-bool refuse_sizes(const KvCacheArgs &c, int batch, int heads) {
-  return (c.dim != 64 && c.dim != 96 && c.dim != 128 && c.dim != 256) || batch < 0 || heads < 1 || c.kv_heads < 1 ||
-         heads % c.kv_heads || c.pages < 0 || c.page_shift < 0 || c.page_shift > 20 ||
+bool refuse_call(const KvCacheArgs &c, const PagedAttentionArgs &a) {
+  return (c.dim != 64 && c.dim != 96 && c.dim != 128 && c.dim != 256) || a.batch < 0 || a.heads < 1 || c.kv_heads < 1 ||
+         a.heads % c.kv_heads || c.pages < 0 || c.page_shift < 0 || c.page_shift > 20 || a.window < 0 || a.max_pages < 0 ||
          (static_cast<long long>(c.pages) * c.kv_heads << c.page_shift) > 0x7fffffffll ||
-         static_cast<long long>(batch) * c.kv_heads * ((heads / c.kv_heads + 7) / 8) > 0x7fffffffll;
+         static_cast<long long>(a.batch) * c.kv_heads * ((a.heads / c.kv_heads + 7) / 8) > 0x7fffffffll ||
+         (static_cast<long long>(a.max_pages) << c.page_shift) > 0x7fffffffll - 256;
 }
 
-}  // namespace
-}  // namespace attn
-
-using namespace attn;
-
-size_t paged_attention_workspace(const KvCacheArgs &c, int batch, int heads) {
-  if (refuse_sizes(c, batch, heads)) return 0;
-  return with_shape(c.dim, heads / c.kv_heads, c.type, [&](auto d, auto nt, auto mode) -> size_t {
-    using S = Shape<decltype(d)::value, decltype(nt)::value, decltype(mode)::value>;
-    return span_bytes(c, batch, heads) + static_cast<size_t>(device_sm_count()) * S::kBlocks * 2 * S::kPart * 4;
-  });
-}
-
-int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *workspace, size_t workspace_bytes,
-                    void *stream) {
-  if (refuse_sizes(c, a.batch, a.heads) || (c.type == ATTN_E4M3 && c.pages > 0 && (!c.k_scale || !c.v_scale)) ||
-      (a.q_type != ATTN_BF16 && a.q_type != ATTN_F16) || (c.type != ATTN_E4M3 && c.type != a.q_type) ||
-      (a.out_type != a.q_type && a.out_type != ATTN_F32) || a.window < 0 || a.max_pages < 0 ||
-      (static_cast<long long>(a.max_pages) << c.page_shift) > 0x7fffffffll - 256 ||
-      workspace_bytes < paged_attention_workspace(c, a.batch, a.heads)) {
-    return cudaErrorInvalidValue;
-  }
-  if (a.batch == 0) return 0;
+Params params_of(const KvCacheArgs &c, const PagedAttentionArgs &a) {
   Params p{};
   p.q = a.q;
   p.q_token = a.q_token;
@@ -966,10 +950,6 @@ int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *wor
   p.pages = c.pages;
   p.shift = c.page_shift;
   p.capacity = c.pages > 0 ? a.max_pages << c.page_shift : 0;  // without pages there is not even an address to skip
-  // A warp counts its tiles (of 16 keys at least) in 32 bits.
-  if (static_cast<long long>(a.batch) * c.kv_heads * p.chunks > 0x7fffffffll * device_sm_count() / (p.capacity / 16 + 1)) {
-    return cudaErrorInvalidValue;
-  }
   p.window = a.window;
   p.scale = a.scale;
   p.softcap = a.softcap;
@@ -977,8 +957,36 @@ int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *wor
   p.lse = a.lse;
   p.q_bf16 = a.q_type == ATTN_BF16;
   p.out_f32 = a.out_type == ATTN_F32;
+  return p;
+}
+
+}  // namespace
+}  // namespace attn
+
+using namespace attn;
+
+size_t paged_attention_workspace(const KvCacheArgs &c, const PagedAttentionArgs &a) {
+  if (refuse_call(c, a)) return 0;
+  const Params p = params_of(c, a);
+  return with_shape(c.dim, p.group, c.type, [&](auto d, auto nt, auto mode) -> size_t {
+    using S = Shape<decltype(d)::value, decltype(nt)::value, decltype(mode)::value>;
+    return is_short<S>(p) ? 0 : span_bytes(p) + static_cast<size_t>(device_sm_count()) * S::kBlocks * 2 * S::kPart * 4;
+  });
+}
+
+int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *workspace, size_t workspace_bytes,
+                    void *stream) {
+  if (refuse_call(c, a) || (c.type == ATTN_E4M3 && c.pages > 0 && (!c.k_scale || !c.v_scale)) ||
+      (a.q_type != ATTN_BF16 && a.q_type != ATTN_F16) || (c.type != ATTN_E4M3 && c.type != a.q_type) ||
+      (a.out_type != a.q_type && a.out_type != ATTN_F32) || workspace_bytes < paged_attention_workspace(c, a)) {
+    return cudaErrorInvalidValue;
+  }
+  if (a.batch == 0) return 0;
+  Params p = params_of(c, a);
+  // A warp counts its tiles (of 16 keys at least) in 32 bits.
+  if (pairs_of(p) > 0x7fffffffll * device_sm_count() / (p.capacity / 16 + 1)) return cudaErrorInvalidValue;
   p.spans = static_cast<int2 *>(workspace);
-  p.partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + span_bytes(c, a.batch, a.heads));
+  p.partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + span_bytes(p));
   return with_shape(c.dim, p.group, c.type, [&](auto d, auto nt, auto mode) -> int {
     return launch<decltype(d)::value, decltype(nt)::value, decltype(mode)::value>(p, static_cast<cudaStream_t>(stream));
   });

@@ -76,19 +76,6 @@ def rope_table(num_positions: int, rotary_dim: int, base: float = 10000.0, devic
     return torch.cat([angle.cos(), angle.sin()], dim=1).float()
 
 
-class _NormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, positions, table, eps, interleaved):
-        ctx.save_for_backward(q, k, q_weight, k_weight, positions, table)
-        ctx.options = (eps, interleaved)
-        return _native.load_attention().qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq, gk):
-        return (*_native.load_attention().qk_norm_rope_backward(gq, gk, *ctx.saved_tensors, *ctx.options), None, None, None, None)
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
                  positions: torch.Tensor, table: torch.Tensor, eps: float = 1e-6, interleaved: bool = False,
                  stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -101,16 +88,12 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     ``(2 i, 2 i + 1)``. ``positions [T]`` int32 or int64: a negative one marks padding, whose rows become zeros and have no
     gradient; one past the table makes its token's rows NaN.
 
-    Differentiable once with respect to ``q``, ``k`` and both weights; the weights' gradients are the same in every run. A
-    backward pass can be captured into a CUDA graph with its forward pass; while an eager graph of the same leaves is alive, the
-    captured forward pass is refused."""
+    Differentiable once (``create_graph`` is refused) with respect to ``q``, ``k`` and both weights; the weights' gradients are
+    the same in every run. A backward pass can be captured into a CUDA graph with its forward pass; while an eager graph of the
+    same leaves is alive, the captured forward pass is refused."""
     if stream is not None:
         with _On(stream, q, k, q_weight, k_weight, positions, table):
             return qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved)
-    if (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad) and torch.is_grad_enabled():
-        if q.is_cuda and torch.cuda.is_current_stream_capturing():
-            _native.load_attention().check_capture([q, k, q_weight, k_weight])
-        return _NormRope.apply(q, k, q_weight, k_weight, positions, table, eps, interleaved)
     return _native.load_attention().qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved)
 
 

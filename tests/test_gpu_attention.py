@@ -197,6 +197,19 @@ def test_norm_rope_empty_and_repeatable():
     assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
+def test_norm_rope_refuses_a_second_derivative():
+    at, q, k, wq, wk, pos, table = norm_rope_case(5, 2, 1, 64, 64, F32, F32, False, False, seed=2)
+    leaves = [t.detach().requires_grad_() for t in (q, k, wq, wk)]
+    out = at.qk_norm_rope(*leaves, pos, table)
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        torch.autograd.grad(out, leaves, [torch.ones_like(x) for x in out], create_graph=True)
+    out = at.qk_norm_rope(*leaves, pos, table)
+    torch.autograd.backward(out, [torch.ones_like(x) for x in out])
+    assert all(t.grad is not None and t.grad.shape == t.shape for t in leaves)
+    frozen = at.qk_norm_rope(leaves[0].detach(), leaves[1].detach(), leaves[2], wk.detach(), pos, table)
+    assert torch.equal(torch.autograd.grad(frozen[0].sum() + frozen[1].sum(), leaves[2])[0], leaves[2].grad)
+
+
 # ---- the cache --------------------------------------------------------------------------------------------------
 
 def random_cache(g, pages, size, heads, dim, dtype):
