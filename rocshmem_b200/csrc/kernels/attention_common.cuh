@@ -94,7 +94,9 @@ template <typename T>
 __device__ __forceinline__ Raw4<T> load4(const T *p) {
   return *reinterpret_cast<const Raw4<T> *>(p);
 }
-__device__ __forceinline__ void unpack4(const Raw4<float> &r, float2 *x) { x[0] = make_float2(r.a.x, r.a.y), x[1] = make_float2(r.a.z, r.a.w); }
+__device__ __forceinline__ void unpack4(const Raw4<float> &r, float2 *x) {
+  x[0] = make_float2(r.a.x, r.a.y), x[1] = make_float2(r.a.z, r.a.w);
+}
 __device__ __forceinline__ void unpack4(const Raw4<__nv_bfloat16> &r, float2 *x) {
   x[0] = make_float2(__uint_as_float(r.a.x << 16), __uint_as_float(r.a.x & 0xffff0000u));
   x[1] = make_float2(__uint_as_float(r.a.y << 16), __uint_as_float(r.a.y & 0xffff0000u));
@@ -103,14 +105,18 @@ __device__ __forceinline__ void unpack4(const Raw4<__half> &r, float2 *x) {
   x[0] = __half22float2(*reinterpret_cast<const __half2 *>(&r.a.x));
   x[1] = __half22float2(*reinterpret_cast<const __half2 *>(&r.a.y));
 }
-__device__ __forceinline__ void store4(float *p, const float2 *x) { *reinterpret_cast<float4 *>(p) = make_float4(x[0].x, x[0].y, x[1].x, x[1].y); }
+__device__ __forceinline__ void store4(float *p, const float2 *x) {
+  *reinterpret_cast<float4 *>(p) = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
+}
 __device__ __forceinline__ void store4(__nv_bfloat16 *p, const float2 *x) {
   const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0].x, x[0].y), hi = __floats2bfloat162_rn(x[1].x, x[1].y);
-  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo),
+      *reinterpret_cast<const uint32_t *>(&hi));
 }
 __device__ __forceinline__ void store4(__half *p, const float2 *x) {
   const __half2 lo = __floats2half2_rn(x[0].x, x[0].y), hi = __floats2half2_rn(x[1].x, x[1].y);
-  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo),
+      *reinterpret_cast<const uint32_t *>(&hi));
 }
 
 // One rounding to the nearest value of the type, ties to even.
@@ -169,8 +175,8 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// The largest magnitude among the row's elements, of which the lane holds eight: that of the bits, so that a NaN or infinity
-// is it. 16-bit types compare two elements in one instruction.
+// The largest magnitude among the row's elements, of which the lane holds eight: that of the bits, so that a NaN or
+// infinity is it. 16-bit types compare two elements in one instruction.
 template <int LANES>
 __device__ __forceinline__ float group_top(const Raw8<float> &r) {
   const float v[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
@@ -183,13 +189,16 @@ __device__ __forceinline__ float group_top(const Raw8<float> &r) {
 }
 template <int LANES>
 __device__ __forceinline__ uint32_t group_top16(const uint4 &r) {
-  uint32_t top = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+  uint32_t top = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu),
+      __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
 #pragma unroll
   for (int o = LANES / 2; o; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
   return max(top & 0xffffu, top >> 16);
 }
 template <int LANES>
-__device__ __forceinline__ float group_top(const Raw8<__nv_bfloat16> &r) { return __uint_as_float(group_top16<LANES>(r.a) << 16); }
+__device__ __forceinline__ float group_top(const Raw8<__nv_bfloat16> &r) {
+  return __uint_as_float(group_top16<LANES>(r.a) << 16);
+}
 template <int LANES>
 __device__ __forceinline__ float group_top(const Raw8<__half> &r) {
   return __half2float(__ushort_as_half(static_cast<unsigned short>(group_top16<LANES>(r.a))));
@@ -200,8 +209,8 @@ struct Int {
   static constexpr int value = V;
 };
 
-// Launches a kernel that may be set up while the one before it on the stream is running; it has to wait for that one's end
-// (griddepcontrol.wait) before it reads.
+// Launches a kernel that may be set up while the one before it on the stream is running; it has to wait for that one's
+// end (griddepcontrol.wait) before it reads.
 template <typename... KArgs>
 cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, unsigned threads, cudaStream_t s,
                          typename same_as_kernel<KArgs>::type... args) {

@@ -1,9 +1,9 @@
 // Operators around attention that pass over their rows once: norm and rotation of query and key heads (forward and
 // backward), writes into and reads from a paged cache, the join of partial attention results.
 //
-// All of them are bound by memory. A row (one head of one token) lies in 8, 16 or 32 neighbouring lanes, eight elements a
-// lane; sums over a row by shuffles, nothing in shared memory but the weights' gradients.
-// No counterpart exists in the reference.
+// All of them are bound by memory. A row (one head of one token) lies in 8, 16 or 32 neighbouring lanes, eight elements
+// a lane; sums over a row by shuffles, nothing in shared memory but the weights' gradients. No counterpart exists in
+// the reference.
 #include "attention_common.cuh"
 
 namespace rocshmem {
@@ -32,9 +32,9 @@ struct NormRope {
   int wide_positions;
 };
 
-// The eight elements of a lane: two pieces of four, so that both elements of each of its pairs are among them and the rotation needs
-// no exchange. Pairs (i, i + rotary / 2): the first lanes have a piece of either half, those behind eight neighbours that
-// are not rotated. Pairs (2i, 2i + 1): eight neighbours.
+// The eight elements of a lane: two pieces of four, so that both elements of each of its pairs are among them and the
+// rotation needs no exchange. Pairs (i, i + rotary / 2): the first lanes have a piece of either half, those behind
+// eight neighbours that are not rotated. Pairs (2i, 2i + 1): eight neighbours.
 template <bool INTERLEAVED>
 struct Place {
   int e0, e1;
@@ -63,10 +63,12 @@ template <bool INTERLEAVED>
 struct Turn {
   float2 c[INTERLEAVED ? 4 : 2], s[INTERLEAVED ? 4 : 2];
   __device__ __forceinline__ void load(const float *row, int rotary, int lane) {
-    const float4 cv = *reinterpret_cast<const float4 *>(row + 4 * lane), sv = *reinterpret_cast<const float4 *>(row + rotary / 2 + 4 * lane);
+    const float4 cv = *reinterpret_cast<const float4 *>(row + 4 * lane);
+    const float4 sv = *reinterpret_cast<const float4 *>(row + rotary / 2 + 4 * lane);
     if constexpr (INTERLEAVED) {
       c[0] = both(cv.x), c[1] = both(cv.y), c[2] = both(cv.z), c[3] = both(cv.w);
-      s[0] = make_float2(-sv.x, sv.x), s[1] = make_float2(-sv.y, sv.y), s[2] = make_float2(-sv.z, sv.z), s[3] = make_float2(-sv.w, sv.w);
+      s[0] = make_float2(-sv.x, sv.x), s[1] = make_float2(-sv.y, sv.y);
+      s[2] = make_float2(-sv.z, sv.z), s[3] = make_float2(-sv.w, sv.w);
     } else {
       c[0] = make_float2(cv.x, cv.y), c[1] = make_float2(cv.z, cv.w);
       s[0] = make_float2(sv.x, sv.y), s[1] = make_float2(sv.z, sv.w);
@@ -83,7 +85,8 @@ __device__ __forceinline__ void rotate(float2 (&x)[4], const Turn<INTERLEAVED> &
       const float2 s = BACK ? make_float2(a.s[i].y, a.s[i].x) : a.s[i];
       x[i] = fma2(make_float2(x[i].y, x[i].x), s, mul2(x[i], a.c[i]));
     } else {
-      const float2 n = make_float2(-a.s[i].x, -a.s[i].y), s = BACK ? n : a.s[i], ns = BACK ? a.s[i] : n, u = x[i], v = x[2 + i];
+      const float2 n = make_float2(-a.s[i].x, -a.s[i].y), s = BACK ? n : a.s[i], ns = BACK ? a.s[i] : n;
+      const float2 u = x[i], v = x[2 + i];
       x[i] = fma2(v, ns, mul2(u, a.c[i]));
       x[2 + i] = fma2(u, s, mul2(v, a.c[i]));
     }
@@ -103,11 +106,12 @@ struct Side {
         head(is_q ? a.q_head : a.k_head), heads(is_q ? a.q_heads : a.k_heads) {}
 };
 
-// 16384 tokens x (32 + 8) heads of 128, bf16: 61.5 us for 344 MB (5.6 TB/s; a device copy: 6.4), with two thirds of the issue
-// slots and half of the integer pipe busy. Four rows in flight and five blocks an SM: with three blocks 71 us, with six,
-// which spill, 90; two rows 73, eight 65. One rounding: that of the result.
+// 16384 tokens x (32 + 8) heads of 128, bf16: 61.5 us for 344 MB (5.6 TB/s; a device copy: 6.4), with two thirds of the
+// issue slots and half of the integer pipe busy. Four rows in flight and five blocks an SM: with three blocks 71 us,
+// with six, which spill, 90; two rows 73, eight 65. One rounding: that of the result.
 template <typename T, typename W, int LANES, int ROWS, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5) norm_rope_kernel(NormRope<T, W> a, unsigned q_items, unsigned items,
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5) norm_rope_kernel(NormRope<T, W> a,
+    unsigned q_items, unsigned items,
                                                                                        Divisor q_chunks, Divisor k_chunks, T *q_out, T *k_out) {
   const int lane = threadIdx.x % LANES;
   const Place<INTERLEAVED> at(lane, a.dim, a.rotary);
@@ -116,7 +120,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5) norm_rope_ke
   const bool is_q = mine < q_items;
   const Side<T, W> side(a, is_q);
   const unsigned item = is_q ? mine : min(mine, items - 1) - q_items, t = divide(item, is_q ? q_chunks : k_chunks);
-  const int h0 = (item - t * (is_q ? q_chunks.d : k_chunks.d)) * ROWS, left = mine < items && at.in_row ? side.heads - h0 : 0;
+  const int h0 = (item - t * (is_q ? q_chunks.d : k_chunks.d)) * ROWS;
+  const int left = mine < items && at.in_row ? side.heads - h0 : 0;
   const long long pos = load_index(a.positions, a.wide_positions, t);
   const T *const rows = side.x + t * side.token + h0 * side.head;
   RawRow<T> raw[ROWS];
@@ -155,16 +160,19 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5) norm_rope_ke
   }
 }
 
-// With g the gradient of the output rotated back, n = x r and a = w g: dx = r (a - n mean(a n)), dw = sum of g n. The norm
-// is computed again (x is read anyway). Blocks below q_blocks have the queries, the others the keys, in proportion. Each
-// group of lanes keeps the sums of its columns of the weight in registers over all its rows; a block adds those up in a fixed
-// order, and norm_rope_weights_kernel adds the blocks' sums, so that the gradients are the same in every run.
+// With g the gradient of the output rotated back, n = x r and a = w g: dx = r (a - n mean(a n)), dw = sum of g n. The
+// norm is computed again (x is read anyway). Blocks below q_blocks have the queries, the others the keys, in
+// proportion. Each group of lanes keeps the sums of its columns of the weight in registers over all its rows; a block
+// adds those up in a fixed order, and norm_rope_weights_kernel adds the blocks' sums, so that the gradients are the
+// same in every run.
 //
-// The case above: 101 us for 512 MB (5.1 TB/s), both kernels. 61 % of the issue slots; what is left is the latency of an item's
-// position, then its angles. Two rows in flight and three blocks an SM: four rows 113, four blocks (spilling) 114, one row in four
-// blocks 138; positions looked up an item ahead 115; items of eight heads 104; more blocks than fit at once 106 - 121.
+// The case above: 101 us for 512 MB (5.1 TB/s), both kernels. 61 % of the issue slots; what is left is the latency of
+// an item's position, then its angles. Two rows in flight and three blocks an SM: four rows 113, four blocks (spilling)
+// 114, one row in four blocks 138; positions looked up an item ahead 115; items of eight heads 104; more blocks than
+// fit at once 106 - 121.
 template <typename T, typename W, int LANES, int ROWS, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads, 3) norm_rope_backward_kernel(NormRope<T, W> a, unsigned q_items, unsigned items,
+__global__ void __launch_bounds__(kThreads, 3) norm_rope_backward_kernel(NormRope<T, W> a, unsigned q_items,
+    unsigned items,
                                                                          int q_blocks, const T *gq, const T *gk, T *dq,
                                                                          T *dk, float *partial) {
   extern __shared__ float sums[];  // [groups][dim]
@@ -184,8 +192,8 @@ __global__ void __launch_bounds__(kThreads, 3) norm_rope_backward_kernel(NormRop
     unpack4(load4(side.weight + at.e0), w);
     unpack4(load4(side.weight + at.e1), w + 2);
   }
-  // The same number of rounds for all groups of a block, for the shuffles; a group behind the last item has no rows. Token
-  // and chunk move by the step's quotient and remainder.
+  // The same number of rounds for all groups of a block, for the shuffles; a group behind the last item has no rows.
+  // Token and chunk move by the step's quotient and remainder.
   const unsigned start = block * kGroups + group, step_t = step / chunks, step_c = step - step_t * chunks;
   unsigned t = start / chunks, chunk = start - t * chunks;
   for (unsigned base = block * kGroups; base < n_items; base += step) {
@@ -299,34 +307,42 @@ struct Row {
   int head;
   bool is_v;
 };
-__device__ __forceinline__ Row row_of(unsigned group, int tokens_each, const Divisor &each) {  // each: two times the heads
+// each: two times the heads
+__device__ __forceinline__ Row row_of(unsigned group, int tokens_each, const Divisor &each) {
   const unsigned chunk = divide(group, each), h = group - chunk * each.d, heads = each.d / 2;
   return Row{static_cast<long long>(chunk) * tokens_each, static_cast<int>(h < heads ? h : h - heads), h >= heads};
 }
 
-// The cache rows of the group's tokens: lane r looks up token r and hands it to the others. All lanes of the warp call it.
+// The cache rows of the group's tokens: lane r looks up token r and hands it to the others. All lanes of the warp call
+// it.
 template <int LANES, int ROWS, typename C>
-__device__ __forceinline__ void look_up_rows(const C &c, const Row &w, const void *slots, int wide_slots, int tokens, int (&row)[ROWS]) {
+__device__ __forceinline__ void look_up_rows(const C &c, const Row &w, const void *slots, int wide_slots, int tokens,
+    int (&row)[ROWS]) {
   const int lane = threadIdx.x % LANES;
   int mine = -1;
   if (lane < ROWS && w.token + lane < tokens) {
-    mine = slot_row(load_index(slots, wide_slots, static_cast<int>(w.token) + lane), c.slots, c.shift, c.kv_heads, w.head);
+    mine = slot_row(load_index(slots, wide_slots, static_cast<int>(w.token) + lane), c.slots, c.shift, c.kv_heads,
+        w.head);
   }
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) row[r] = __shfl_sync(0xffffffffu, mine, r, LANES);
 }
 
-// A group of lanes takes one head's row (of k or of v) of ROWS neighbouring tokens, their loads first. Neighbouring groups
-// take the token's other heads: reads are contiguous across a block, and a head's rows go to neighbouring places of its page.
+// A group of lanes takes one head's row (of k or of v) of ROWS neighbouring tokens, their loads first. Neighbouring
+// groups take the token's other heads: reads are contiguous across a block, and a head's rows go to neighbouring places
+// of its page.
 //
-// e4m3: with m the largest magnitude of the row, codes are x * (448 / m) and the factor m / 448. m is held above 2^-110,
-// below which 448 / m would overflow. The largest magnitude is that of the bits, so that a NaN or infinity becomes m, and
-// with it the factor: such a row reads back as NaN. Rounding to 4 bits is what the cache is for; the factor is fp32.
+// e4m3: with m the largest magnitude of the row, codes are x * (448 / m) and the factor m / 448. m is held above
+// 2^-110, below which 448 / m would overflow. The largest magnitude is that of the bits, so that a NaN or infinity
+// becomes m, and with it the factor: such a row reads back as NaN. Rounding to 4 bits is what the cache is for; the
+// factor is fp32.
 //
-// 32768 tokens x 8 heads of 128, bf16 to e4m3: 39 us for 204 MB (5.2 TB/s), bound by the integer pipe (68 % busy before a lane
-// looked up a token's row for the others and divisions became multiplications, 42 us); to bf16 43 us for 269 MB (6.2 TB/s).
+// 32768 tokens x 8 heads of 128, bf16 to e4m3: 39 us for 204 MB (5.2 TB/s), bound by the integer pipe (68 % busy before
+// a lane looked up a token's row for the others and divisions became multiplications, 42 us); to bf16 43 us for 269 MB
+// (6.2 TB/s).
 template <typename T, typename C, int LANES, int ROWS>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 6) kv_write_kernel(Cache<C> c, const T *k, const T *v, long long k_token,
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 6) kv_write_kernel(Cache<C> c, const T *k,
+    const T *v, long long k_token,
                                                             long long k_head, long long v_token, long long v_head,
                                                             const void *slots, int wide_slots, int tokens) {
   constexpr bool kQuantize = sizeof(C) == 1;
@@ -351,7 +367,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 6) kv_write_ker
     unpack8(raw[r], x);
     if constexpr (kQuantize) {
       const float top = group_top<LANES>(raw[r]);
-      const float m = top < INFINITY ? fmaxf(top, 0x1p-110f) : __int_as_float(0x7fc00000);  // the comparison fails for NaN too
+      // the comparison fails for NaN too
+      const float m = top < INFINITY ? fmaxf(top, 0x1p-110f) : __int_as_float(0x7fc00000);
       const float inv = 448.0f / m;
       if (to[r] >= 0) {
         if (in_row) {
@@ -414,8 +431,8 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(Cache<C> c, T *k_out,
 
 // ---- the join of partial results ---------------------------------------------------------------------------------
 
-// out = sum w_i o_i / sum w_i with w_i = exp(lse_i - max). A part whose lse is -inf has seen nothing and
-// does not count, whatever its rows hold. Eight parts of 512 x 64 rows of 128 in fp32: 26.6 us for 144 MB (5.4 TB/s), bound by
+// out = sum w_i o_i / sum w_i with w_i = exp(lse_i - max). A part whose lse is -inf has seen nothing and does not
+// count, whatever its rows hold. Eight parts of 512 x 64 rows of 128 in fp32: 26.6 us for 144 MB (5.4 TB/s), bound by
 // the memory's latency; the first parts' loads are on their way while the maximum is found.
 template <typename T, typename O, int LANES>
 __global__ void __launch_bounds__(kThreads) join_kernel(const T *outs, const float *lses, long long out_part,
@@ -467,7 +484,9 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const T *outs, const flo
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = acc[e] * inv;
   if (in_row) store8(out + row * dim + 8 * lane, x);
-  if (lane == 0 && lse != nullptr) lse[row] = bad ? __int_as_float(0x7fc00000) : total > 0.f ? base + logf(total) : -INFINITY;
+  if (lane == 0 && lse != nullptr) {
+    lse[row] = bad ? __int_as_float(0x7fc00000) : total > 0.f ? base + logf(total) : -INFINITY;
+  }
 }
 
 // ---- choice of the instantiation ---------------------------------------------------------------------------------
@@ -498,7 +517,8 @@ int with_lanes(int dim, F f) {
 
 bool bad_rows(int dim) { return dim < 8 || dim > 256 || dim % 8; }
 
-// Blocks of a launch with one group of lanes for each of `items`; 0 when the kernels could not number the groups in 32 bits.
+// Blocks of a launch with one group of lanes for each of `items`; 0 when the kernels could not number the groups in 32
+// bits.
 unsigned blocks_for(long long items, int lanes) {
   const long long per = kThreads / lanes, n = (items + per - 1) / per;
   return n * per > 0x7fffffffll ? 0u : static_cast<unsigned>(n);
@@ -508,13 +528,16 @@ unsigned blocks_for(long long items, int lanes) {
 long long groups_at_once(int lanes) { return static_cast<long long>(device_sm_count()) * (2048 / lanes); }
 
 // Items of `rows` heads.
-long long items_of(int tokens, int heads, int rows) { return static_cast<long long>(tokens) * ((heads + rows - 1) / rows); }
+long long items_of(int tokens, int heads, int rows) {
+  return static_cast<long long>(tokens) * ((heads + rows - 1) / rows);
+}
 
 int backward_blocks() { return device_sm_count() * 3; }
 
 template <typename T, typename W>
 NormRope<T, W> norm_rope_args(const NormRopeArgs &a) {
-  return NormRope<T, W>{static_cast<const T *>(a.q), static_cast<const T *>(a.k), a.q_token, a.q_head, a.k_token, a.k_head,
+  return NormRope<T, W>{static_cast<const T *>(a.q), static_cast<const T *>(a.k), a.q_token, a.q_head, a.k_token,
+      a.k_head,
                         static_cast<const W *>(a.q_weight), static_cast<const W *>(a.k_weight), a.positions, a.table,
                         a.tokens, a.q_heads, a.k_heads, a.dim, a.rotary, a.table_rows, a.eps, 1.f / static_cast<float>(a.dim),
                         a.wide_positions};
@@ -572,11 +595,13 @@ int qk_norm_rope(const NormRopeArgs &a, void *q_out, void *k_out, void *stream) 
       constexpr int kLanes = decltype(l)::value;
       auto launch = [&](auto rows, auto pairs) -> int {
         constexpr int kRows = decltype(rows)::value;
-        const long long q_items = items_of(a.tokens, a.q_heads, kRows), items = q_items + items_of(a.tokens, a.k_heads, kRows);
+        const long long q_items = items_of(a.tokens, a.q_heads, kRows);
+        const long long items = q_items + items_of(a.tokens, a.k_heads, kRows);
         const unsigned blocks = blocks_for(items, kLanes);
         if (!blocks) return cudaErrorInvalidValue;
         norm_rope_kernel<T, W, kLanes, kRows, decltype(pairs)::value != 0>
-            <<<blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(norm_rope_args<T, W>(a), static_cast<unsigned>(q_items),
+            <<<blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(norm_rope_args<T, W>(a),
+                static_cast<unsigned>(q_items),
                                                                          static_cast<unsigned>(items), divisor((a.q_heads + kRows - 1) / kRows),
                                                                          divisor((a.k_heads + kRows - 1) / kRows),
                                                                          static_cast<T *>(q_out), static_cast<T *>(k_out));
@@ -602,12 +627,15 @@ int qk_norm_rope_backward(const NormRopeArgs &a, const void *gq, const void *gk,
       constexpr int kLanes = decltype(l)::value;
       constexpr int kRows = 2;
       const cudaStream_t s = static_cast<cudaStream_t>(stream);
-      const long long q_items = items_of(a.tokens, a.q_heads, kRows), items = q_items + items_of(a.tokens, a.k_heads, kRows);
+      const long long q_items = items_of(a.tokens, a.q_heads, kRows);
+      const long long items = q_items + items_of(a.tokens, a.k_heads, kRows);
       const long long per = kThreads / kLanes;
       if (items > 0x7fffffffll - backward_blocks() * per) return cudaErrorInvalidValue;
       // Blocks in proportion to the items of queries and keys, at least one for either.
-      const int blocks = static_cast<int>(std::max<long long>(2, std::min<long long>(backward_blocks(), (items + per - 1) / per)));
-      const int q_blocks = static_cast<int>(std::min<long long>(std::max<long long>(q_items * blocks / std::max(items, 1ll), 1), blocks - 1));
+      const long long wanted = std::min<long long>(backward_blocks(), (items + per - 1) / per);
+      const int blocks = static_cast<int>(std::max<long long>(2, wanted));
+      const long long q_share = q_items * blocks / std::max(items, 1ll);
+      const int q_blocks = static_cast<int>(std::min<long long>(std::max<long long>(q_share, 1), blocks - 1));
       auto launch = [&](auto pairs) -> int {
         norm_rope_backward_kernel<T, W, kLanes, kRows, decltype(pairs)::value != 0>
             <<<blocks, kThreads, kThreads / kLanes * a.dim * sizeof(float), s>>>(
@@ -617,7 +645,8 @@ int qk_norm_rope_backward(const NormRopeArgs &a, const void *gq, const void *gk,
       };
       const int e = a.interleaved ? launch(Int<1>{}) : launch(Int<0>{});
       if (e != cudaSuccess) return e;
-      return launch_after(norm_rope_weights_kernel<W>, dim3((a.dim + 31) / 32, 2), 1024, s, workspace, q_blocks, blocks, a.dim,
+      return launch_after(norm_rope_weights_kernel<W>, dim3((a.dim + 31) / 32, 2), 1024, s, workspace, q_blocks,
+          blocks, a.dim,
                           static_cast<W *>(dq_weight), static_cast<W *>(dk_weight));
     });
   });
@@ -638,7 +667,8 @@ int kv_cache_write(const KvCacheArgs &c, const void *k, const void *v, long long
         const long long rows = static_cast<long long>(tokens) * 2 * c.kv_heads;
         auto launch = [&](auto n) -> int {
           constexpr int kRows = decltype(n)::value;
-          const unsigned blocks = blocks_for((static_cast<long long>(tokens) + kRows - 1) / kRows * 2 * c.kv_heads, kLanes);
+          const unsigned blocks = blocks_for((static_cast<long long>(tokens) + kRows - 1) / kRows * 2 * c.kv_heads,
+              kLanes);
           if (!blocks) return cudaErrorInvalidValue;
           kv_write_kernel<T, C, kLanes, kRows><<<blocks, kThreads, 0, s>>>(
               cache, static_cast<const T *>(k), static_cast<const T *>(v), k_token, k_head, v_token, v_head, slots,
@@ -665,7 +695,8 @@ int kv_cache_read(const KvCacheArgs &c, void *k_out, void *v_out, const void *sl
         const long long rows = static_cast<long long>(tokens) * 2 * c.kv_heads;
         auto launch = [&](auto n) -> int {
           constexpr int kRows = decltype(n)::value;
-          const unsigned blocks = blocks_for((static_cast<long long>(tokens) + kRows - 1) / kRows * 2 * c.kv_heads, kLanes);
+          const unsigned blocks = blocks_for((static_cast<long long>(tokens) + kRows - 1) / kRows * 2 * c.kv_heads,
+              kLanes);
           if (!blocks) return cudaErrorInvalidValue;
           kv_read_kernel<T, C, kLanes, kRows><<<blocks, kThreads, 0, s>>>(cache, static_cast<T *>(k_out),
                                                                          static_cast<T *>(v_out), slots, wide_slots, tokens);

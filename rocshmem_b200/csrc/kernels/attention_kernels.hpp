@@ -11,8 +11,8 @@ namespace kernels {
 
 enum AttnType : int { ATTN_BF16 = 0, ATTN_F16 = 1, ATTN_F32 = 2, ATTN_E4M3 = 3 };
 
-// Queries and keys of one call of the norm + rotation: rows of `dim` elements at base + t * token + h * head (strides in
-// elements); outputs are contiguous [tokens, heads, dim].
+// Queries and keys of one call of the norm + rotation: rows of `dim` elements at base + t * token + h * head (strides
+// in elements); outputs are contiguous [tokens, heads, dim].
 struct NormRopeArgs {
   const void *q, *k;
   long long q_token, q_head, k_token, k_head;
@@ -36,7 +36,8 @@ struct KvCacheArgs {
   float *k_scale, *v_scale;
   int pages, kv_heads, page_shift, dim, type;
 };
-// Rows k[t, h, :], v[t, h, :] (strides in elements) go to slots[t] (32- or 64-bit); slots outside the cache are skipped.
+// Rows k[t, h, :], v[t, h, :] (strides in elements) go to slots[t] (32- or 64-bit); slots outside the cache are
+// skipped.
 int kv_cache_write(const KvCacheArgs &c, const void *k, const void *v, long long k_token, long long k_head,
                    long long v_token, long long v_head, const void *slots, int wide_slots, int tokens, int type,
                    void *stream);
@@ -61,7 +62,8 @@ size_t paged_attention_workspace(const KvCacheArgs &c, const PagedAttentionArgs 
 int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *workspace, size_t workspace_bytes,
                     void *stream);
 
-// outs [parts, rows, dim] (part stride in elements), lses [parts, rows] (part stride in elements) -> out [rows, dim], lse [rows].
+// outs [parts, rows, dim] (part stride in elements), lses [parts, rows] (part stride in elements) -> out [rows, dim],
+// lse [rows].
 int attention_join(const void *outs, const float *lses, long long out_part, long long lse_part, int parts,
                    long long rows, int dim, int in_type, int out_type, void *out, float *lse, void *stream);
 

@@ -3,9 +3,9 @@
 //
 // The tiles of all (sequence, unit) pairs stand in one line: sequence by sequence, within it unit by unit (a unit is a
 // key head and up to 8 * NT of its query heads), within that tile by tile. Warp c of the grid takes the share [c * per,
-// (c + 1) * per) of the line, whatever pairs its tiles belong to. A pair that lies in one share is finished there; one that
-// lies in several leaves a partial result in each of them. A share has at most two such pairs, its first and its last, so
-// two places a share hold all partial results whatever the lengths are.
+// (c + 1) * per) of the line, whatever pairs its tiles belong to. A pair that lies in one share is finished there; one
+// that lies in several leaves a partial result in each of them. A share has at most two such pairs, its first and its
+// last, so two places a share hold all partial results whatever the lengths are.
 #pragma once
 
 #include <cstdint>
@@ -49,11 +49,12 @@ ATTN_HD Owners owners(long long begin, int n, long long per) { return Owners{beg
 ATTN_HD int place(long long first, long long c) { return c > first ? 0 : 1; }
 
 // The last share that a pair of n tiles lies in which begins in share `share` with `left` of the share's tiles left.
-ATTN_HD int last_share(int share, int n, int left, int per) { return n > left ? share + (n - left + per - 1) / per : share; }
+ATTN_HD int last_share(int share, int n, int left, int per) { return n > left ? share + (n - left + per - 1) / per
+    : share; }
 
-// Division of numbers below 2^31 by one divisor, by a multiplication (Granlund and Montgomery): with l = ceil(log2 d) and m =
-// floor(2^32 (2^l - d) / d) + 1, n / d = (floor(m n / 2^32) + n) >> l. A division proper takes 20 instructions, as many as a
-// fifth of what a row of a cache write needs.
+// Division of numbers below 2^31 by one divisor, by a multiplication (Granlund and Montgomery): with l = ceil(log2 d)
+// and m = floor(2^32 (2^l - d) / d) + 1, n / d = (floor(m n / 2^32) + n) >> l. A division proper takes 20 instructions,
+// as many as a fifth of what a row of a cache write needs.
 struct Divisor {
   uint32_t d, m, l;
 };
@@ -73,7 +74,8 @@ ATTN_HD int page_row(int page, int num_pages, int pos, int shift, int kv_heads, 
   return ((page * kv_heads + head) << shift) + (pos & ((1 << shift) - 1));
 }
 
-// The same for a flat slot (page * page_size + offset), or -1 for a slot outside the cache, which has at most 2^31 - 1 rows.
+// The same for a flat slot (page * page_size + offset), or -1 for a slot outside the cache, which has at most 2^31 - 1
+// rows.
 ATTN_HD int slot_row(long long slot, int num_slots, int shift, int kv_heads, int head) {
   if (slot < 0 || slot >= num_slots) return -1;
   const int s = static_cast<int>(slot);

@@ -1,6 +1,7 @@
 // Python bindings of the attention operators. Unlike the library's other bindings they take torch tensors: checks,
 // outputs, workspaces and launches of a call are done here, because in Python they take 20 us and more, several times
-// what the kernels of a decode step take. What is refused raises ValueError or TypeError before anything touches a device.
+// what the kernels of a decode step take. What is refused raises ValueError or TypeError before anything touches a
+// device.
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
@@ -69,7 +70,8 @@ struct Strides {
 };
 Strides rows(const Tensor &t, const char *name, int64_t heads = -1, int64_t dim = -1) {
   if (t.dim() != 3 || (heads >= 0 && t.size(1) != heads) || (dim >= 0 && t.size(2) != dim)) {
-    bad_value(name, " must be [tokens, ", heads >= 0 ? text(heads) : "heads", ", ", dim >= 0 ? text(dim) : "dim", "], got ", t.sizes());
+    bad_value(name, " must be [tokens, ", heads >= 0 ? text(heads) : "heads", ", ", dim >= 0 ? text(dim) : "dim",
+        "], got ", t.sizes());
   }
   const int64_t vec = 16 / static_cast<int64_t>(t.element_size());
   const Strides s{t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0};
@@ -90,7 +92,9 @@ int index(const Tensor &t, const char *name, int64_t count) {
 void no_grad(const char *what, std::initializer_list<const Tensor *> tensors) {
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor *t : tensors) {
-    if (t->requires_grad()) bad_value(what, " has no backward pass: call it under torch.no_grad(), or detach its inputs");
+    if (t->requires_grad()) {
+      bad_value(what, " has no backward pass: call it under torch.no_grad(), or detach its inputs");
+    }
   }
 }
 
@@ -128,7 +132,8 @@ void result(const Tensor &t, const char *name, at::IntArrayRef shape, std::initi
             std::initializer_list<const Tensor *> inputs) {
   bool ok = t.sizes() == shape && t.is_contiguous() && aligned(t), typed = false;
   for (at::ScalarType s : types) typed = typed || t.scalar_type() == s;
-  if (!ok || !typed) bad_value(name, " must be a contiguous, 16-byte aligned tensor of shape ", shape, " and type ", *types.begin(),
+  if (!ok || !typed) bad_value(name, " must be a contiguous, 16-byte aligned tensor of shape ", shape, " and type ",
+      *types.begin(),
                                types.size() > 1 ? " or float" : "", ", got ", t.sizes(), " ", t.scalar_type());
   for (const Tensor *x : inputs) {
     if (x != nullptr && overlap(t, *x)) bad_value(name, " shares memory with an input");
@@ -150,7 +155,8 @@ NormRopeArgs norm_rope_args(const Tensor &q, const Tensor &k, const Tensor &q_we
   }
   if (D % 8 || D < 8 || D > 256) bad_value("the head dimension must be a multiple of 8 up to 256, got ", D);
   for (const auto &[w, name] : {std::make_pair(&q_weight, "q_weight"), std::make_pair(&k_weight, "k_weight")}) {
-    if ((w->scalar_type() != q.scalar_type() && w->scalar_type() != at::kFloat) || w->scalar_type() != q_weight.scalar_type()) {
+    if ((w->scalar_type() != q.scalar_type() && w->scalar_type() != at::kFloat) ||
+        w->scalar_type() != q_weight.scalar_type()) {
       bad_type(name, " must be ", q.scalar_type(), " or fp32, both weights the same");
     }
     if (w->dim() != 1 || w->size(0) != D || !w->is_contiguous() || !aligned(*w)) {
@@ -191,7 +197,8 @@ NormRopeArgs norm_rope_args(const Tensor &q, const Tensor &k, const Tensor &q_we
   return a;
 }
 
-std::pair<Tensor, Tensor> py_qk_norm_rope(const Tensor &q, const Tensor &k, const Tensor &q_weight, const Tensor &k_weight,
+std::pair<Tensor, Tensor> py_qk_norm_rope(const Tensor &q, const Tensor &k, const Tensor &q_weight,
+    const Tensor &k_weight,
                                           const Tensor &positions, const Tensor &table, double eps, bool interleaved) {
   const NormRopeArgs a = norm_rope_args(q, k, q_weight, k_weight, positions, table, eps, interleaved);
   const Here here(q);
@@ -200,8 +207,9 @@ std::pair<Tensor, Tensor> py_qk_norm_rope(const Tensor &q, const Tensor &k, cons
   return {q_out, k_out};
 }
 
-// A leaf whose gradients an eager graph, alive at the time, accumulates on another stream cannot take part in a captured
-// backward pass: the engine would make that stream wait for the captured one, which ends the process. Refused instead.
+// A leaf whose gradients an eager graph, alive at the time, accumulates on another stream cannot take part in a
+// captured backward pass: the engine would make that stream wait for the captured one, which ends the process. Refused
+// instead.
 void check_capture(void *stream, int device, std::initializer_list<const Tensor *> tensors) {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   check(cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &status), "qk_norm_rope");
@@ -229,15 +237,20 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
     return {both.first, both.second};
   }
 
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-    if (at::GradMode::is_enabled()) throw std::runtime_error("qk_norm_rope can be differentiated once: create_graph is refused");
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+      torch::autograd::variable_list grads) {
+    if (at::GradMode::is_enabled()) {
+      throw std::runtime_error("qk_norm_rope can be differentiated once: create_graph is refused");
+    }
     const auto saved = ctx->get_saved_variables();
     const Tensor &q = saved[0], &k = saved[1], &q_weight = saved[2], &k_weight = saved[3], &table = saved[5];
     const NormRopeArgs a = norm_rope_args(q, k, q_weight, k_weight, saved[4], table, ctx->saved_data["eps"].toDouble(),
                                           ctx->saved_data["interleaved"].toBool());
     const Here here(q);
     // Gradients come in any layout (an expanded one behind a sum, for instance); the kernel reads plain rows.
-    auto plain = [](const Tensor &g) { return g.is_contiguous() && aligned(g) ? g : g.clone(at::MemoryFormat::Contiguous); };
+    auto plain = [](const Tensor &g) {
+      return g.is_contiguous() && aligned(g) ? g : g.clone(at::MemoryFormat::Contiguous);
+    };
     const Tensor gq = plain(grads[0]), gk = plain(grads[1]);
     Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
     Tensor dwq = at::empty(q_weight.sizes(), q_weight.options()), dwk = at::empty(k_weight.sizes(), k_weight.options());
@@ -248,9 +261,11 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
   }
 };
 
-std::pair<Tensor, Tensor> py_qk_norm_rope_any(const Tensor &q, const Tensor &k, const Tensor &q_weight, const Tensor &k_weight,
+std::pair<Tensor, Tensor> py_qk_norm_rope_any(const Tensor &q, const Tensor &k, const Tensor &q_weight,
+    const Tensor &k_weight,
                                               const Tensor &positions, const Tensor &table, double eps, bool interleaved) {
-  if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || q_weight.requires_grad() || k_weight.requires_grad())) {
+  if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || q_weight.requires_grad() ||
+      k_weight.requires_grad())) {
     return py_qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved);
   }
   norm_rope_args(q, k, q_weight, k_weight, positions, table, eps, interleaved);  // refused before a graph is begun
@@ -262,7 +277,7 @@ std::pair<Tensor, Tensor> py_qk_norm_rope_any(const Tensor &q, const Tensor &k, 
   return {both[0], both[1]};
 }
 
-// ---- the paged cache --------------------------------------------------------------------------------------------------
+// ---- the paged cache ------------------------------------------------------------------------------------------------
 
 struct Cache {
   Tensor k, v;
@@ -276,11 +291,15 @@ KvCacheArgs cache_args(const Cache &c) {
     bad_value("KvCache: k and v must both be [pages, kv_heads, page_size, head_dim] in bf16, fp16 or e4m3");
   }
   const int64_t pages = k.size(0), heads = k.size(1), size = k.size(2), dim = k.size(3);
-  if (size < 1 || size > (1 << 20) || (size & (size - 1))) bad_value("KvCache: the page size must be a power of two up to 2^20, got ", size);
+  if (size < 1 || size > (1 << 20) || (size & (size - 1))) {
+    bad_value("KvCache: the page size must be a power of two up to 2^20, got ", size);
+  }
   if (heads < 1 || heads > (1 << 20) || pages > INT32_MAX || dim % 8 || dim < 8 || dim > 256) {
     bad_value("KvCache: at least one head, head_dim a multiple of 8 up to 256");
   }
-  if (pages * heads * size > INT32_MAX) bad_value("KvCache: at most 2^31 - 1 rows (pages * kv_heads * page_size), got ", pages * heads * size);
+  if (pages * heads * size > INT32_MAX) {
+    bad_value("KvCache: at most 2^31 - 1 rows (pages * kv_heads * page_size), got ", pages * heads * size);
+  }
   const bool scaled = k.scalar_type() == at::kFloat8_e4m3fn;
   for (const OptTensor *s : {&c.k_scale, &c.v_scale}) {
     if (scaled && (!s->has_value() || (*s)->scalar_type() != at::kFloat || (*s)->sizes() != k.sizes().slice(0, 3))) {
@@ -314,7 +333,9 @@ void py_kv_cache_write(const Cache &c, const Tensor &k, const Tensor &v, const T
   no_grad("kv_cache_write", {&k, &v});
   on_one_device("kv_cache_write", {&k, &v, &slots, &c.k});
   for (const Tensor *t : {&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)}) {
-    if (t != nullptr && (overlap(*t, k) || overlap(*t, v))) bad_value("kv_cache_write: k or v shares memory with the cache");
+    if (t != nullptr && (overlap(*t, k) || overlap(*t, v))) {
+      bad_value("kv_cache_write: k or v shares memory with the cache");
+    }
   }
   const Here here(k);
   check(kv_cache_write(a, data(k), data(v), sk.token, sk.head, sv.token, sv.head, data(slots), wide,
@@ -331,7 +352,8 @@ std::pair<Tensor, Tensor> py_kv_cache_read(const Cache &c, const Tensor &slots, 
   const Here here(slots);
   const auto options = c.k.options().dtype(dtype);
   Tensor k = at::empty({T, a.kv_heads, a.dim}, options), v = at::empty({T, a.kv_heads, a.dim}, options);
-  check(kv_cache_read(a, data(k), data(v), data(slots), wide, static_cast<int>(T), code(dtype), here.stream), "kv_cache_read");
+  check(kv_cache_read(a, data(k), data(v), data(slots), wide, static_cast<int>(T), code(dtype), here.stream),
+      "kv_cache_read");
   return {k, v};
 }
 
@@ -347,23 +369,34 @@ Paged check_paged(const Tensor &q, const Cache &c, const Tensor &block_table, co
                   std::optional<double> scale, double softcap, int64_t window) {
   Paged p{cache_args(c), {}};
   if (!is_half(q.scalar_type()) || (p.cache.type != ATTN_E4M3 && p.cache.type != code(q.scalar_type()))) {
-    bad_type("q must be bf16 or fp16, and of the cache's type unless that is e4m3: got ", q.scalar_type(), " and ", c.k.scalar_type());
+    bad_type("q must be bf16 or fp16, and of the cache's type unless that is e4m3: got ", q.scalar_type(), " and ",
+        c.k.scalar_type());
   }
   const Strides s = rows(q, "q", -1, p.cache.dim);
   const int64_t B = q.size(0), H = q.size(1), D = q.size(2);
-  if (H < 1 || H % p.cache.kv_heads) bad_value("the ", H, " query heads must be a multiple of the cache's ", p.cache.kv_heads);
-  if (D != 64 && D != 96 && D != 128 && D != 256) bad_value("paged_attention: the head dimension must be 64, 96, 128 or 256, got ", D);
-  if (block_table.scalar_type() != at::kInt || lengths.scalar_type() != at::kInt) bad_type("block_table and lengths must be int32");
+  if (H < 1 || H % p.cache.kv_heads) {
+    bad_value("the ", H, " query heads must be a multiple of the cache's ", p.cache.kv_heads);
+  }
+  if (D != 64 && D != 96 && D != 128 && D != 256) {
+    bad_value("paged_attention: the head dimension must be 64, 96, 128 or 256, got ", D);
+  }
+  if (block_table.scalar_type() != at::kInt || lengths.scalar_type() != at::kInt) {
+    bad_type("block_table and lengths must be int32");
+  }
   if (block_table.dim() != 2 || block_table.size(0) != B || (block_table.size(1) > 1 && block_table.stride(1) != 1)) {
     bad_value("block_table must be [", B, ", pages] with contiguous rows");
   }
-  if (lengths.dim() != 1 || lengths.size(0) != B || !lengths.is_contiguous()) bad_value("lengths must be contiguous [", B, "]");
+  if (lengths.dim() != 1 || lengths.size(0) != B || !lengths.is_contiguous()) {
+    bad_value("lengths must be contiguous [", B, "]");
+  }
   const double f = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(D));
   if (!(f > 0 && f < 1e30) || !(softcap >= 0 && softcap < 1e30) || window < 0) {
     bad_value("scale must be positive, softcap and window not negative");
   }
   const int64_t most = block_table.size(1) * c.k.size(2);
-  if (most > INT32_MAX - 256) bad_value("paged_attention: a sequence's pages hold at most 2^31 - 257 tokens, got ", most);
+  if (most > INT32_MAX - 256) {
+    bad_value("paged_attention: a sequence's pages hold at most 2^31 - 257 tokens, got ", most);
+  }
   PagedAttentionArgs &a = p.args;
   a.q = data(q);
   a.q_token = s.token;
@@ -386,7 +419,8 @@ std::pair<Tensor, OptTensor> py_paged_attention(const Tensor &q, const Cache &c,
                                                 int64_t window, const OptTensor &out_given, const OptTensor &lse_given,
                                                 bool want_lse) {
   Paged p = check_paged(q, c, block_table, lengths, scale, softcap, window);
-  const std::initializer_list<const Tensor *> inputs = {&q, &block_table, &lengths, &c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)};
+  const std::initializer_list<const Tensor *> inputs = {&q, &block_table, &lengths, &c.k, &c.v, or_null(c.k_scale),
+      or_null(c.v_scale)};
   if (out_given) {
     result(*out_given, "out", q.sizes(), {q.scalar_type(), at::kFloat}, inputs);
     if (lse_given && overlap(*out_given, *lse_given)) bad_value("out shares memory with lse");
@@ -409,9 +443,12 @@ std::pair<Tensor, OptTensor> py_paged_attention(const Tensor &q, const Cache &c,
   return {out, lse};
 }
 
-std::pair<Tensor, Tensor> py_attention_join(const Tensor &outs, const Tensor &lses, std::optional<at::ScalarType> dtype_given,
+std::pair<Tensor, Tensor> py_attention_join(const Tensor &outs, const Tensor &lses,
+    std::optional<at::ScalarType> dtype_given,
                                             const OptTensor &out_given) {
-  if (!is_float(outs.scalar_type()) || lses.scalar_type() != at::kFloat) bad_type("outs must be bf16, fp16 or fp32, lses fp32");
+  if (!is_float(outs.scalar_type()) || lses.scalar_type() != at::kFloat) {
+    bad_type("outs must be bf16, fp16 or fp32, lses fp32");
+  }
   if (outs.dim() != 4 || lses.sizes() != outs.sizes().slice(0, 3) || outs.size(0) < 1 || outs.size(0) > INT32_MAX) {
     bad_value("outs must be [n, B, H, D] and lses [n, B, H], got ", outs.sizes(), " and ", lses.sizes());
   }
@@ -438,7 +475,8 @@ std::pair<Tensor, Tensor> py_attention_join(const Tensor &outs, const Tensor &ls
   const Here here(outs);
   Tensor out = out_given ? *out_given : at::empty(outs.sizes().slice(1), outs.options().dtype(dtype));
   Tensor lse = at::empty(lses.sizes().slice(1), lses.options());
-  check(attention_join(data(outs), static_cast<const float *>(data(lses)), outs_part, lse_part, static_cast<int>(n), B * H,
+  check(attention_join(data(outs), static_cast<const float *>(data(lses)), outs_part, lse_part, static_cast<int>(n),
+      B * H,
                        static_cast<int>(D), code(outs.scalar_type()), code(dtype), data(out),
                        static_cast<float *>(data(lse)), here.stream), "attention_join");
   return {out, lse};
@@ -448,7 +486,8 @@ std::pair<Tensor, Tensor> py_attention_join(const Tensor &outs, const Tensor &ls
 
 PYBIND11_MODULE(_A, m) {
   m.doc() = "Attention operators on torch tensors";
-  py::class_<Cache>(m, "Cache").def(py::init([](const Tensor &k, const Tensor &v, const OptTensor &ks, const OptTensor &vs) {
+  py::class_<Cache>(m, "Cache").def(py::init([](const Tensor &k, const Tensor &v, const OptTensor &ks,
+      const OptTensor &vs) {
     Cache c{k, v, ks, vs};
     cache_args(c);
     return c;

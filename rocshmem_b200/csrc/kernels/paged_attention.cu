@@ -2,11 +2,12 @@
 //
 //   s_j = scale q.k_j  (capped: c tanh(s_j / c)),   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   lse = m + log sum
 //
-// A key and a value are read once and used by the 1 - 16 query heads that share them, so memory bounds the kernel: about 23
-// bytes a cycle and SM have to arrive, and the arithmetic only has to keep up. The products run on warp-level matrix
-// instructions with the KEYS as the tile's 16 rows and the query heads as its 8 columns: a group of up to eight heads
-// wastes nothing (with the heads as rows, half and more of each instruction would be padding), and 16 keys a warp are
-// enough to feed it. tcgen05 needs 128 rows to a tile and accumulators in TMEM; it has nothing to give where the tensor pipe idles.
+// A key and a value are read once and used by the 1 - 16 query heads that share them, so memory bounds the kernel:
+// about 23 bytes a cycle and SM have to arrive, and the arithmetic only has to keep up. The products run on warp-level
+// matrix instructions with the KEYS as the tile's 16 rows and the query heads as its 8 columns: a group of up to eight
+// heads wastes nothing (with the heads as rows, half and more of each instruction would be padding), and 16 keys a warp
+// are enough to feed it. tcgen05 needs 128 rows to a tile and accumulators in TMEM; it has nothing to give where the
+// tensor pipe idles.
 //
 //   S^T [16 keys, 8 heads] = K [16, D] Q^T [D, 8]          A = K rows as they lie, B = queries, kept in registers
 //   O^T [D, 8 heads]      += V^T [D, 16 keys] P^T [16, 8]  A = V transposed on the way out of shared memory
@@ -14,18 +15,19 @@
 // The accumulator layout of S^T differs from the operand layout of P^T by a transposition of 8 x 8 blocks (movmatrix).
 // Both products have a head's values in the same lanes, so rescaling O by the change of the maximum needs no exchange.
 //
-// Blocks are single warps that work on their own. The line of all tiles (attention_plan.hpp) is dealt to them in equal shares; a
-// warp streams its tiles through a ring of stages (cp.async; rows behind the end, of bad pages and before the window
-// arrive as zeros and score -inf) with a running maximum and sum, and its loads run ahead from one pair into the next. There is no
-// barrier. A pair that lies in several shares leaves unnormalised partial results, which paged_join_kernel adds in the order of the
-// shares: results do not depend on which warp is done first.
+// Blocks are single warps that work on their own. The line of all tiles (attention_plan.hpp) is dealt to them in equal
+// shares; a warp streams its tiles through a ring of stages (cp.async; rows behind the end, of bad pages and before the
+// window arrive as zeros and score -inf) with a running maximum and sum, and its loads run ahead from one pair into the
+// next. There is no barrier. A pair that lies in several shares leaves unnormalised partial results, which
+// paged_join_kernel adds in the order of the shares: results do not depend on which warp is done first.
 //
-// e4m3 caches: codes become fp16 exactly (cvt), a key's factor multiplies its score, a value's factor its probability. They are
-// bound by instructions as much as by memory: 32 keys a step need 650 (two steps of 16 keys took 15 % longer).
+// e4m3 caches: codes become fp16 exactly (cvt), a key's factor multiplies its score, a value's factor its probability.
+// They are bound by instructions as much as by memory: 32 keys a step need 650 (two steps of 16 keys took 15 % longer).
 //
-// Measured on one B200, 128 elements a head: 64 sequences of 1024 - 4096 tokens, 32 / 8 heads, bf16, 116 us for 676 MB (5.8 TB/s; a
-// device copy: 6.4); two sequences of 130 - 520 thousand, 64 / 8 heads, e4m3, 307 us for 1.94 GB (6.3). Without the join, 111 and
-// 302. What is left in the first is the start, 4 us until data arrives, and the SMs that end last (see Shape).
+// Measured on one B200, 128 elements a head: 64 sequences of 1024 - 4096 tokens, 32 / 8 heads, bf16, 116 us for 676 MB
+// (5.8 TB/s; a device copy: 6.4); two sequences of 130 - 520 thousand, 64 / 8 heads, e4m3, 307 us for 1.94 GB (6.3).
+// Without the join, 111 and 302. What is left in the first is the start, 4 us until data arrives, and the SMs that end
+// last (see Shape).
 #include "attention_common.cuh"
 
 #include <atomic>
@@ -37,8 +39,9 @@ namespace attn {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// Probabilities are at most 1. Where they are rounded to fp16 they are scaled by 2^14 first, so that one down to 2^-28 of
-// the largest keeps all its bits and none above 2^-39 is lost from a long sum; the factor is in the sum as well and cancels.
+// Probabilities are at most 1. Where they are rounded to fp16 they are scaled by 2^14 first, so that one down to 2^-28
+// of the largest keeps all its bits and none above 2^-39 is lost from a long sum; the factor is in the sum as well and
+// cancels.
 constexpr float kF16Shift = 14.f;
 
 enum Mode : int { MODE_BF16 = 0, MODE_F16 = 1, MODE_E4M3 = 2 };
@@ -108,9 +111,9 @@ __device__ __forceinline__ float reciprocal(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// c tanh(x / c) in base 2, with in = 1 / c and back = c log2(e). Up to one, where most scores are, tanh y is Lambert's continued
-// fraction y / (1 + y^2 / (3 + y^2 / (5 + y^2 / (7 + y^2 / 9)))) as a quotient (off by 6e-8 of it at most), beyond 1 - 2 / (exp(2y) +
-// 1), whose error there is one of the last bits too. tanhf cost a fifth of the kernel's time.
+// c tanh(x / c) in base 2, with in = 1 / c and back = c log2(e). Up to one, where most scores are, tanh y is Lambert's
+// continued fraction y / (1 + y^2 / (3 + y^2 / (5 + y^2 / (7 + y^2 / 9)))) as a quotient (off by 6e-8 of it at most),
+// beyond 1 - 2 / (exp(2y) + 1), whose error there is one of the last bits too. tanhf cost a fifth of the kernel's time.
 __device__ __forceinline__ float cap2(float x, float in, float back) {
   const float y = x * in, y2 = y * y;
   const float near = y * fmaf(y2 + 105.f, y2, 945.f) * reciprocal(fmaf(fmaf(15.f, y2, 420.f), y2, 945.f));
@@ -119,8 +122,8 @@ __device__ __forceinline__ float cap2(float x, float in, float back) {
 }
 
 // Shared memory and tile sizes of one instantiation. Rows are padded so that the accesses of a fragment fall into
-// different banks: 16 bytes for 16-bit rows (ldmatrix), for e4m3 32 bytes a key row (8 bytes a lane from four rows) and 16 a value row
-// (up to 16 bytes a lane from every other row). With 96 e4m3 elements a key row already has that stride.
+// different banks: 16 bytes for 16-bit rows (ldmatrix), for e4m3 32 bytes a key row (8 bytes a lane from four rows) and
+// 16 a value row (up to 16 bytes a lane from every other row). With 96 e4m3 elements a key row already has that stride.
 template <int D, int NT, int MODE>
 struct Shape {
   static constexpr int kElem = MODE == MODE_E4M3 ? 1 : 2;
@@ -129,21 +132,24 @@ struct Shape {
   static constexpr int kPitchK = kRowBytes + (MODE == MODE_E4M3 ? (D == 96 ? 0 : 32) : 16);
   static constexpr int kPitchV = kRowBytes + 16;
   static constexpr int kScales = MODE == MODE_E4M3 ? 2 * kKeys * 4 : 0;
-  static constexpr int kStage = kKeys * (kPitchK + kPitchV) + kScales + 16;  // one warp's stage; its last word: which rows are seen
+  // one warp's stage; its last word: which rows are seen
+  static constexpr int kStage = kKeys * (kPitchK + kPitchV) + kScales + 16;
   static constexpr int kHeads = 8 * NT;
   static constexpr int kFrags = D / 16 * NT;               // of O^T, four values a lane
   static constexpr int kPart = kFrags * 128 + 2 * kHeads;  // floats of a partial result: O^T, maxima (base 2), sums
-  // Two stages: one tile on its way while the other is used. e4m3 is bound by instructions and takes as many warps as its
-  // registers allow. 16-bit caches are bound by memory and want 64 - 70 KB on their way for each SM, no more: SMs of
-  // large GPCs get less of the bandwidth than others, and the further the queues reach, the later they end (128 elements,
-  // 64 sequences, blocks x stages an SM: 8 x 2 119 us, 12 x 2 123, 5 x 4 123, 8 x 3 127).
+  // Two stages: one tile on its way while the other is used. e4m3 is bound by instructions and takes as many warps as
+  // its registers allow. 16-bit caches are bound by memory and want 64 - 70 KB on their way for each SM, no more: SMs
+  // of large GPCs get less of the bandwidth than others, and the further the queues reach, the later they end (128
+  // elements, 64 sequences, blocks x stages an SM: 8 x 2 119 us, 12 x 2 123, 5 x 4 123, 8 x 3 127).
   static constexpr int kStages = 2;
   static constexpr int kWarpsByRegisters = NT == 2 ? (D == 64 ? 12 : 8) : D == 64 ? 16 : D == 96 ? 12 : 8;
   static constexpr int kWarpsByBytes = 70 * 1024 / kStage;
-  static constexpr int kBlocks = MODE == MODE_E4M3 || kWarpsByBytes > kWarpsByRegisters ? kWarpsByRegisters : kWarpsByBytes;
+  static constexpr int kBlocks =
+      MODE == MODE_E4M3 || kWarpsByBytes > kWarpsByRegisters ? kWarpsByRegisters : kWarpsByBytes;
   static constexpr int kSmem = kStages * kStage;
   static constexpr int kTeam = 8 * kSmem <= 226 * 1024 ? 8 : 4;  // warps of a block of paged_short_kernel
-  static_assert(kBlocks * (kSmem + 1024) <= 228 * 1024 && kPitchK % 16 == 0 && kPitchV % 16 == 0 && kStage % 16 == 0, "alignment");
+  static_assert(kBlocks * (kSmem + 1024) <= 228 * 1024 && kPitchK % 16 == 0 && kPitchV % 16 == 0 && kStage % 16 == 0,
+      "alignment");
 };
 
 struct Params {
@@ -207,9 +213,11 @@ __device__ __forceinline__ void store_out(const Params &p, long long at, float x
   else store1(static_cast<__half *>(p.out) + at, x);
 }
 
-// For the two heads of a lane's columns in group j: the factor that makes sums of p v results, and, by one lane each, the lse.
+// For the two heads of a lane's columns in group j: the factor that makes sums of p v results, and, by one lane each,
+// the lse.
 template <int NT>
-__device__ __forceinline__ void finish(const Params &p, long long row0, int n_heads, int j, int lane, const float (&m)[2],
+__device__ __forceinline__ void finish(const Params &p, long long row0, int n_heads, int j, int lane,
+    const float (&m)[2],
                                        const float (&l)[2], float (&inv)[2]) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -256,8 +264,9 @@ __device__ __forceinline__ void store_fragment(const Params &p, long long row0, 
   }
 }
 
-// Streams the tiles of a warp's share, from `cur` on. done(...) is called at the end of every pair, or of the share's part of
-// one, with the accumulators of O^T (e4m3: in units of cv), maxima and sums of the lane's columns, and whether the pair begins and ends here.
+// Streams the tiles of a warp's share, from `cur` on. done(...) is called at the end of every pair, or of the share's
+// part of one, with the accumulators of O^T (e4m3: in units of cv), maxima and sums of the lane's columns, and whether
+// the pair begins and ends here.
 template <int D, int NT, int MODE, typename F>
 __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cur, int lane, F done) {
   using S = Shape<D, NT, MODE>;
@@ -297,7 +306,7 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
       const unsigned r = kEven ? i * kEach + my_row : at / kChunks, c = kEven ? 0 : at % kChunks;
       const int from = __shfl_sync(0xffffffffu, row, r);
       const uint32_t bytes = from < 0 ? 0 : 16;
-      const unsigned long long off = static_cast<unsigned long long>(static_cast<uint32_t>(max(from, 0))) * S::kRowBytes;
+      const unsigned long long off = static_cast<unsigned long long>(static_cast<unsigned>(max(from, 0))) * S::kRowBytes;
       const uint32_t to_k = kEven ? i * kEach * S::kPitchK : r * S::kPitchK + c * 16;
       const uint32_t to_v = kEven ? i * kEach * S::kPitchV : r * S::kPitchV + c * 16;
       copy16(my_to + at_stage + to_k, my_k + off + c * 16, bytes);
@@ -328,7 +337,8 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
 
   // ---- pairs ----
   const float cap_in = 1.f / p.softcap, cap_back = p.softcap * kLog2e;
-  const int k_lane = (lane % 16) * S::kPitchK + (lane / 16) * 16;                       // ldmatrix: 16 keys x 16 elements
+  // ldmatrix: 16 keys x 16 elements
+  const int k_lane = (lane % 16) * S::kPitchK + (lane / 16) * 16;
   const int v_lane = ((lane / 16) * 8 + lane % 8) * S::kPitchV + (lane / 8 % 2) * 16;   // transposed
   while (cur.left > 0) {
     const int b = cur.b, kv = cur.unit / p.chunks, h0 = kv * p.group + cur.unit % p.chunks * S::kHeads;
@@ -558,8 +568,9 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
             }
           }
         } else {
-          // Lane (g, t) reads neighbouring elements of value rows 2t, 2t + 1, 2t + 8, 2t + 9; byte pairs of two rows become
-          // the fragment's registers. Element e of the lane's D / 8 is row g (e even) or g + 8 (e odd) of block e / 2.
+          // Lane (g, t) reads neighbouring elements of value rows 2t, 2t + 1, 2t + 8, 2t + 9; byte pairs of two rows
+          // become the fragment's registers. Element e of the lane's D / 8 is row g (e even) or g + 8 (e odd) of block
+          // e / 2.
           constexpr int kWords = D / 32;
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
@@ -623,7 +634,8 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
 
 // A partial result: fragments as they lie in the lanes, then maxima and sums of the columns.
 template <int D, int NT, int MODE>
-__device__ __forceinline__ void store_part(float *part, int lane, const float (&o)[D / 16][NT][4], const float (&m)[NT][2],
+__device__ __forceinline__ void store_part(float *part, int lane, const float (&o)[D / 16][NT][4],
+    const float (&m)[NT][2],
                                            const float (&l)[NT][2], float cv) {
   using S = Shape<D, NT, MODE>;
   const float f = MODE == MODE_E4M3 ? cv : 1.f;
@@ -639,7 +651,8 @@ __device__ __forceinline__ void store_part(float *part, int lane, const float (&
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       *reinterpret_cast<float2 *>(part + S::kFrags * 128 + 8 * j + 2 * lane) = make_float2(m[j][0], m[j][1]);
-      *reinterpret_cast<float2 *>(part + S::kFrags * 128 + S::kHeads + 8 * j + 2 * lane) = make_float2(l[j][0], l[j][1]);
+      *reinterpret_cast<float2 *>(part + S::kFrags * 128 + S::kHeads + 8 * j + 2 * lane) =
+          make_float2(l[j][0], l[j][1]);
     }
   }
 }
@@ -668,7 +681,8 @@ template <int D, int NT, int MODE>
 __device__ __forceinline__ Joined load_part(const float *part, int at) {
   using S = Shape<D, NT, MODE>;
   const int col = 8 * (at / 32 % NT) + 2 * (at % 4);
-  return Joined{reinterpret_cast<const float4 *>(part)[at], *reinterpret_cast<const float2 *>(part + S::kFrags * 128 + col),
+  return Joined{reinterpret_cast<const float4 *>(part)[at],
+      *reinterpret_cast<const float2 *>(part + S::kFrags * 128 + col),
                 *reinterpret_cast<const float2 *>(part + S::kFrags * 128 + S::kHeads + col)};
 }
 // The result of fragment at / 32. All lanes of the warp call it.
@@ -676,7 +690,8 @@ template <int D, int NT, int MODE>
 __device__ __forceinline__ void store_joined(const Params &p, int b, int unit, int at, const Joined &a) {
   using S = Shape<D, NT, MODE>;
   const int lane = at % 32, d = at / 32 / NT, j = at / 32 % NT;
-  const int kv = unit / p.chunks, h0 = kv * p.group + unit % p.chunks * S::kHeads, n_heads = min(S::kHeads, (kv + 1) * p.group - h0);
+  const int kv = unit / p.chunks, h0 = kv * p.group + unit % p.chunks * S::kHeads;
+  const int n_heads = min(S::kHeads, (kv + 1) * p.group - h0);
   const float v[4] = {a.o.x, a.o.y, a.o.z, a.o.w}, tops[2] = {a.m.x, a.m.y}, sums[2] = {a.l.x, a.l.y};
   float inv[2];
   // One warp for each group of heads writes the lse.
@@ -695,7 +710,9 @@ __global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(
   // ---- the line of tiles ----
   // Lanes take neighbouring sequences, `per_lane` each; a scan over the lanes gives each one its first tile.
   const int per_lane = (p.batch + 31) / 32, b_lo = min(lane * per_lane, p.batch), b_hi = min(b_lo + per_lane, p.batch);
-  auto tiles_at = [&](int b) { return static_cast<long long>(tiles_of(visible(p.lengths[b], p.capacity, p.window), kKeys)) * units; };
+  auto tiles_at = [&](int b) {
+    return static_cast<long long>(tiles_of(visible(p.lengths[b], p.capacity, p.window), kKeys)) * units;
+  };
   long long mine = 0;
   for (int b = b_lo; b < b_hi; ++b) mine += tiles_at(b);
   long long upto = mine;
@@ -745,7 +762,8 @@ __global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(
           make_int2(share, last_share(share, pair.n, pair.left, static_cast<int>(per)));
     }
     if (!(begins && ends)) {
-      store_part<D, NT, MODE>(p.partial + (static_cast<long long>(blockIdx.x) * 2 + (begins ? 1 : 0)) * S::kPart, lane, o, m, l, cv);
+      store_part<D, NT, MODE>(p.partial + (static_cast<long long>(blockIdx.x) * 2 + (begins ? 1 : 0)) * S::kPart,
+          lane, o, m, l, cv);
       return;
     }
     const long long row0 = static_cast<long long>(pair.b) * p.heads + h0;
@@ -778,7 +796,8 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, MODE>::kTeam) paged_short_ke
   float *const part = reinterpret_cast<float *>(ring);
   static_assert(S::kPart * 4 <= S::kSmem, "a part fits the ring");
   if (cur.left > 0) {
-    run_share<D, NT, MODE>(p, ring, cur, lane, [&](const Cursor &, bool, bool, int, int, float (&o)[DK][NT][4], float (&m)[NT][2],
+    run_share<D, NT, MODE>(p, ring, cur, lane,
+        [&](const Cursor &, bool, bool, int, int, float (&o)[DK][NT][4], float (&m)[NT][2],
                                                    float (&l)[NT][2], float cv) {
       copies_wait<0>();
       __syncwarp();
@@ -798,8 +817,8 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, MODE>::kTeam) paged_short_ke
   }
 }
 
-// Adds the partial results of the pairs that several warps share, in the order of the shares. A thread has the four values
-// that a lane had of one fragment; a block GROUPS sets of such threads, which take the parts in turn.
+// Adds the partial results of the pairs that several warps share, in the order of the shares. A thread has the four
+// values that a lane had of one fragment; a block GROUPS sets of such threads, which take the parts in turn.
 template <int D, int NT, int MODE, int GROUPS>
 __global__ void __launch_bounds__(256) paged_join_kernel(const Params p) {
   using S = Shape<D, NT, MODE>;
@@ -841,10 +860,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const Params p) {
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
-// Keys a warp of paged_short_kernel, at most: with more, splitting over more SMs pays for a second launch. 128 elements, bf16,
-// 32 pairs, one launch against two: 128 keys 6.2 us against 9.9, 512 keys 10.3 and 10.3, 1024 keys 14.4 and 11.1.
+// Keys a warp of paged_short_kernel, at most: with more, splitting over more SMs pays for a second launch. 128
+// elements, bf16, 32 pairs, one launch against two: 128 keys 6.2 us against 9.9, 512 keys 10.3 and 10.3, 1024 keys 14.4
+// and 11.1.
 constexpr int kShortKeys = 64;
-// Keys that a share has at least: below that its fixed costs weigh more than the loads that another warp would take over.
+// Keys that a share has at least: below that its fixed costs weigh more than the loads that another warp would take
+// over.
 constexpr int kLeastKeys = 32;
 
 int heads_per_unit(int group, int dim) { return group > 8 && dim <= 128 ? 16 : 8; }
@@ -863,7 +884,8 @@ auto with_shape(int dim, int group, int cache_type, F f) {
     return cache_type == ATTN_BF16 ? heads(d, Int<MODE_BF16>{}) : cache_type == ATTN_F16 ? heads(d, Int<MODE_F16>{})
                                                                                        : heads(d, Int<MODE_E4M3>{});
   };
-  return dim == 64 ? modes(Int<64>{}) : dim == 96 ? modes(Int<96>{}) : dim == 128 ? modes(Int<128>{}) : modes(Int<256>{});
+  return dim == 64 ? modes(Int<64>{}) : dim == 96 ? modes(Int<96>{}) : dim == 128 ? modes(Int<128>{})
+      : modes(Int<256>{});
 }
 
 int pairs_of(const Params &p) { return p.batch * p.kv_heads * p.chunks; }
@@ -871,8 +893,8 @@ int pairs_of(const Params &p) { return p.batch * p.kv_heads * p.chunks; }
 // The lengths are on the device: what counts on the host is the most that they can be.
 int longest_of(const Params &p) { return p.window > 0 ? std::min(p.window, p.capacity) : p.capacity; }
 
-// A block for each pair, no more than SMs. From half the SMs on there is less to split: twice the keys (128 pairs of 1024
-// keys: 14.4 us against 18.0; of 2048: 24.7 and 26.8).
+// A block for each pair, no more than SMs. From half the SMs on there is less to split: twice the keys (128 pairs of
+// 1024 keys: 14.4 us against 18.0; of 2048: 24.7 and 26.8).
 template <typename S>
 bool is_short(const Params &p) {
   const int pairs = pairs_of(p), sms = device_sm_count();
@@ -898,7 +920,8 @@ int launch(Params p, cudaStream_t s) {
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
     e = cudaFuncSetAttribute(paged_kernel<D, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(paged_short_kernel<D, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTeam * S::kSmem);
+    e = cudaFuncSetAttribute(paged_short_kernel<D, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        S::kTeam * S::kSmem);
     if (e != cudaSuccess) return e;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
@@ -913,8 +936,9 @@ int launch(Params p, cudaStream_t s) {
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   if (longest_of(p) <= S::kKeys) return 0;  // no pair has two tiles: nothing to join
-  // Many parts of each of a few pairs are shared by eight sets of threads (8 pairs of 148 parts: 35 us the whole call, with one set
-  // 62); few parts of many pairs are not worth the exchange (128 pairs of 9 parts: 73 us with one set, 76 with eight).
+  // Many parts of each of a few pairs are shared by eight sets of threads (8 pairs of 148 parts: 35 us the whole call,
+  // with one set 62); few parts of many pairs are not worth the exchange (128 pairs of 9 parts: 73 us with one set, 76
+  // with eight).
   const int shares = p.blocks;
   return pairs > shares / 24 ? launch_join<D, NT, MODE, 1>(p, s) : launch_join<D, NT, MODE, 8>(p, s);
 }
@@ -924,7 +948,8 @@ size_t span_bytes(const Params &p) { return (static_cast<size_t>(pairs_of(p)) + 
 
 bool refuse_call(const KvCacheArgs &c, const PagedAttentionArgs &a) {
   return (c.dim != 64 && c.dim != 96 && c.dim != 128 && c.dim != 256) || a.batch < 0 || a.heads < 1 || c.kv_heads < 1 ||
-         a.heads % c.kv_heads || c.pages < 0 || c.page_shift < 0 || c.page_shift > 20 || a.window < 0 || a.max_pages < 0 ||
+         a.heads % c.kv_heads || c.pages < 0 || c.page_shift < 0 || c.page_shift > 20 || a.window < 0
+             || a.max_pages < 0 ||
          (static_cast<long long>(c.pages) * c.kv_heads << c.page_shift) > 0x7fffffffll ||
          static_cast<long long>(a.batch) * c.kv_heads * ((a.heads / c.kv_heads + 7) / 8) > 0x7fffffffll ||
          (static_cast<long long>(a.max_pages) << c.page_shift) > 0x7fffffffll - 256;

@@ -29,7 +29,7 @@ E4M3 = torch.float8_e4m3fn
 E4M3_MAX = 448.0
 
 
-# ---- streams ----------------------------------------------------------------------------------------------------------
+# ---- streams ---------------------------------------------------------------------------------------------------------
 
 class _On:
     """Makes ``stream`` current on the device of ``tensors``, whose memory is kept until the stream is done with it."""
@@ -59,7 +59,7 @@ class _On:
         return self._inner.__exit__(*args)
 
 
-# ---- norm and rotation ------------------------------------------------------------------------------------------------
+# ---- norm and rotation -----------------------------------------------------------------------------------------------
 
 def rope_table(num_positions: int, rotary_dim: int, base: float = 10000.0, device=None,
                frequencies: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -84,20 +84,20 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
 
     bf16, fp16 or fp32; sums, norm and rotation in fp32, rounded once. ``D`` is a multiple of 8 up to 256. Rows may be
     strided (views of a fused projection) as long as each is contiguous and 16-byte aligned. The weights have the rows'
-    type or fp32. ``table [positions, R]`` is :func:`rope_table`'s, ``R`` a multiple of 16. Pairs are ``(i, i + R / 2)``, or with ``interleaved``
-    ``(2 i, 2 i + 1)``. ``positions [T]`` int32 or int64: a negative one marks padding, whose rows become zeros and have no
-    gradient; one past the table makes its token's rows NaN.
+    type or fp32. ``table [positions, R]`` is :func:`rope_table`'s, ``R`` a multiple of 16. Pairs are ``(i, i + R /
+    2)``, or with ``interleaved`` ``(2 i, 2 i + 1)``. ``positions [T]`` int32 or int64: a negative one marks padding,
+    whose rows become zeros and have no gradient; one past the table makes its token's rows NaN.
 
-    Differentiable once (``create_graph`` is refused) with respect to ``q``, ``k`` and both weights; the weights' gradients are
-    the same in every run. A backward pass can be captured into a CUDA graph with its forward pass; while an eager graph of the
-    same leaves is alive, the captured forward pass is refused."""
+    Differentiable once (``create_graph`` is refused) with respect to ``q``, ``k`` and both weights; the weights'
+    gradients are the same in every run. A backward pass can be captured into a CUDA graph with its forward pass; while
+    an eager graph of the same leaves is alive, the captured forward pass is refused."""
     if stream is not None:
         with _On(stream, q, k, q_weight, k_weight, positions, table):
             return qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved)
     return _native.load_attention().qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved)
 
 
-# ---- the paged cache --------------------------------------------------------------------------------------------------
+# ---- the paged cache -------------------------------------------------------------------------------------------------
 
 @dataclass(frozen=True, eq=False)
 class KvCache:
@@ -118,8 +118,8 @@ class KvCache:
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
                  device=None, symmetric: bool = False) -> "KvCache":
-        """A cache of zeros on ``device`` (default: the current CUDA device). ``symmetric``: on the symmetric heap, so that
-        other PEs can put pages into it (collective; give it back with :meth:`free`)."""
+        """A cache of zeros on ``device`` (default: the current CUDA device). ``symmetric``: on the symmetric heap, so
+        that other PEs can put pages into it (collective; give it back with :meth:`free`)."""
         shape = (num_pages, kv_heads, page_size, head_dim)
         if symmetric:
             def zeros(shape, dtype):
@@ -131,7 +131,8 @@ class KvCache:
                 return torch.zeros(shape, dtype=dtype, device=device)
         if dtype != E4M3:
             return cls(zeros(shape, dtype), zeros(shape, dtype))
-        return cls(zeros(shape, dtype), zeros(shape, dtype), zeros(shape[:3], torch.float32), zeros(shape[:3], torch.float32))
+        return cls(zeros(shape, dtype), zeros(shape, dtype), zeros(shape[:3], torch.float32),
+            zeros(shape[:3], torch.float32))
 
     def free(self) -> None:
         """Collective: give a symmetric cache's memory back to the heap."""
@@ -163,10 +164,11 @@ class KvCache:
         return (self.k, self.v) if self.k_scale is None else (self.k, self.v, self.k_scale, self.v_scale)
 
 
-def token_slots(block_table: torch.Tensor, sequences: torch.Tensor, positions: torch.Tensor, page_size: int) -> torch.Tensor:
-    """Slots (int64) of tokens: token ``i`` is position ``positions[i]`` of sequence ``sequences[i]``, whose pages are row
-    ``sequences[i]`` of ``block_table``. -1 for a negative position, one past the table or one without a page. Plain PyTorch,
-    any device, no synchronisation."""
+def token_slots(block_table: torch.Tensor, sequences: torch.Tensor, positions: torch.Tensor,
+    page_size: int) -> torch.Tensor:
+    """Slots (int64) of tokens: token ``i`` is position ``positions[i]`` of sequence ``sequences[i]``, whose pages are
+    row ``sequences[i]`` of ``block_table``. -1 for a negative position, one past the table or one without a page. Plain
+    PyTorch, any device, no synchronisation."""
     at = positions.long()
     known = (at >= 0) & (at < block_table.shape[1] * page_size)
     if block_table.shape[1] == 0:
@@ -176,9 +178,9 @@ def token_slots(block_table: torch.Tensor, sequences: torch.Tensor, positions: t
 
 
 def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, stream=None) -> None:
-    """Writes ``k``, ``v [T, kv_heads, head_dim]`` (bf16, fp16 or fp32; rows may be strided as in :func:`qk_norm_rope`) into
-    the slots ``[T]`` (int32 or int64). Slots outside the cache, negative ones among them, are skipped: padding. The
-    others have to differ from one another.
+    """Writes ``k``, ``v [T, kv_heads, head_dim]`` (bf16, fp16 or fp32; rows may be strided as in :func:`qk_norm_rope`)
+    into the slots ``[T]`` (int32 or int64). Slots outside the cache, negative ones among them, are skipped: padding.
+    The others have to differ from one another.
 
     A 16-bit cache takes the values rounded to its type. In an e4m3 cache a row with the largest magnitude ``m`` becomes
     codes ``x * 448 / m`` with the factor ``m / 448``; a row that holds a NaN or an infinity reads back as NaN."""
@@ -190,8 +192,8 @@ def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torc
 
 def kv_cache_read(cache: KvCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
                   stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """The keys and values of slots ``[T]`` (int32 or int64), each ``[T, kv_heads, head_dim]`` in bf16, fp16 or fp32 (codes
-    times factors in fp32, rounded once). Slots outside the cache give zeros."""
+    """The keys and values of slots ``[T]`` (int32 or int64), each ``[T, kv_heads, head_dim]`` in bf16, fp16 or fp32
+    (codes times factors in fp32, rounded once). Slots outside the cache give zeros."""
     if stream is not None:
         with _On(stream, slots, *cache._tensors()):
             return kv_cache_read(cache, slots, dtype)
@@ -207,19 +209,22 @@ def paged_attention(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor, 
     """Attention of one new token for each sequence: ``q [B, H, D]`` against the first ``lengths[b]`` tokens of sequence
     ``b``, which lie in the pages ``block_table[b]``. Returns ``out [B, H, D]``, with ``return_lse`` ``(out, lse)``.
 
-    ``q`` is bf16 or fp16 and of the cache's type, or either for an e4m3 cache; ``D`` is 64, 96, 128 or 256; ``H`` a multiple of the cache's
-    heads, whose groups share a key head. Scores are ``scale * q.k`` (default ``D ** -0.5``), with ``softcap`` > 0
-    ``softcap * tanh(scale * q.k / softcap)``; ``window`` > 0 leaves the last ``window`` tokens. Sums and softmax are fp32. ``out`` may be given,
-    in q's type or fp32, and ``lse [B, H]`` fp32, the natural logarithm of the sum of the scores' exponentials; neither may share
-    memory with an input. ``block_table [B, pages]`` and ``lengths [B]`` are int32 on the device.
+    ``q`` is bf16 or fp16 and of the cache's type, or either for an e4m3 cache; ``D`` is 64, 96, 128 or 256; ``H`` a
+    multiple of the cache's heads, whose groups share a key head. Scores are ``scale * q.k`` (default ``D ** -0.5``),
+    with ``softcap`` > 0 ``softcap * tanh(scale * q.k / softcap)``; ``window`` > 0 leaves the last ``window`` tokens.
+    Sums and softmax are fp32. ``out`` may be given, in q's type or fp32, and ``lse [B, H]`` fp32, the natural logarithm
+    of the sum of the scores' exponentials; neither may share memory with an input. ``block_table [B, pages]`` and
+    ``lengths [B]`` are int32 on the device.
 
-    Lengths are taken between 0 and the table's end. Tokens in a page that is no page of the cache are not seen. A sequence that sees
-    nothing has zeros and an lse of -inf. Rows that are not seen may hold anything, NaN included; an infinity or NaN in a row
-    that is seen makes the results of its heads NaN, except a score of -inf, which counts for nothing."""
+    Lengths are taken between 0 and the table's end. Tokens in a page that is no page of the cache are not seen. A
+    sequence that sees nothing has zeros and an lse of -inf. Rows that are not seen may hold anything, NaN included; an
+    infinity or NaN in a row that is seen makes the results of its heads NaN, except a score of -inf, which counts for
+    nothing."""
     if stream is not None:
         with _On(stream, q, block_table, lengths, *cache._tensors(), out, lse):
             return paged_attention(q, cache, block_table, lengths, scale, softcap, window, out, lse, return_lse)
-    both = _native.load_attention().paged_attention(q, cache._cache, block_table, lengths, scale, softcap, window, out, lse,
+    both = _native.load_attention().paged_attention(q, cache._cache, block_table, lengths, scale, softcap, window,
+        out, lse,
                                                     return_lse)
     return both if return_lse else both[0]
 
@@ -227,9 +232,10 @@ def paged_attention(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor, 
 def attention_join(outs: torch.Tensor, lses: torch.Tensor, dtype: Optional[torch.dtype] = None,
                    out: Optional[torch.Tensor] = None, stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Joins attention results over disjoint parts of a cache: ``outs [n, B, H, D]`` (bf16, fp16 or fp32) with ``lses
-    [n, B, H]`` fp32, as :func:`paged_attention` returns them for each part. Returns ``(out [B, H, D], lse [B, H])``: the parts'
-    sum weighted by ``exp(lse)``. Every part must be contiguous; the parts may lie apart. ``dtype`` of the result defaults to that
-    of ``out`` if given, else of ``outs``. A part with an lse of -inf does not count, whatever its ``outs`` hold."""
+    [n, B, H]`` fp32, as :func:`paged_attention` returns them for each part. Returns ``(out [B, H, D], lse [B, H])``:
+    the parts' sum weighted by ``exp(lse)``. Every part must be contiguous; the parts may lie apart. ``dtype`` of the
+    result defaults to that of ``out`` if given, else of ``outs``. A part with an lse of -inf does not count, whatever
+    its ``outs`` hold."""
     if stream is not None:
         with _On(stream, outs, lses, out):
             return attention_join(outs, lses, dtype, out)
@@ -238,7 +244,8 @@ def attention_join(outs: torch.Tensor, lses: torch.Tensor, dtype: Optional[torch
 
 # ---- references (plain PyTorch, any device) -------------------------------------------------------------------------
 
-def ref_norm_rope(x: torch.Tensor, weight: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, eps: float = 1e-6,
+def ref_norm_rope(x: torch.Tensor, weight: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
+    eps: float = 1e-6,
                   interleaved: bool = False) -> torch.Tensor:
     """PyTorch reference of :func:`qk_norm_rope` for one of the two tensors, in 64 bits, differentiable."""
     R = table.shape[1]
@@ -269,8 +276,8 @@ def ref_quantize_rows(x: torch.Tensor):
 
 def ref_paged_attention(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor, lengths: torch.Tensor,
                         scale: Optional[float] = None, softcap: float = 0.0, window: int = 0):
-    """PyTorch reference of :func:`paged_attention` in 64 bits, sequence by sequence: ``(out, lse)``. The CPU backend's form
-    of the operator too."""
+    """PyTorch reference of :func:`paged_attention` in 64 bits, sequence by sequence: ``(out, lse)``. The CPU backend's
+    form of the operator too."""
     _native.load_attention().check_paged(q, cache._cache, block_table, lengths, scale, softcap, window)
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     B, H, D = q.shape
@@ -306,5 +313,6 @@ def ref_attention_join(outs: torch.Tensor, lses: torch.Tensor):
     top = l.amax(dim=0)
     w = torch.exp(l - torch.where(top == float("-inf"), 0.0, top))
     total = w.sum(dim=0)
-    out = torch.where(w[..., None] > 0, outs.double() * w[..., None], 0.0).sum(dim=0) / torch.where(total > 0, total, 1.0)[..., None]
+    out = torch.where(w[..., None] > 0, outs.double() * w[..., None], 0.0).sum(dim=0) / torch.where(total > 0, total,
+        1.0)[..., None]
     return out, torch.where(total > 0, top + total.clamp(min=1e-300).log(), float("-inf"))

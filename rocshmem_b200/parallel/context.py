@@ -1,17 +1,17 @@
 """Decoding with a cache that is spread over a team: the counterpart, for one new token, of the sequence-sharded
 prefill of :mod:`rocshmem_b200.parallel.ring`.
 
-Every member keeps the keys and values of some of a sequence's tokens (after ring attention, those of its own part of the
-prompt; the new tokens go to any one member) in a paged cache of its own. For a step every member computes the attention of
-the same queries over its tokens, the partial results and their log-sum-exps are gathered, and every member joins them:
+Every member keeps the keys and values of some of a sequence's tokens (after ring attention, those of its own part of
+the prompt; the new tokens go to any one member) in a paged cache of its own. For a step every member computes the
+attention of the same queries over its tokens, the partial results and their log-sum-exps are gathered, and every member
+joins them:
 
     step = ContextParallelDecode(max_batch=64, heads=32, head_dim=128)
     out = step(q, cache, block_table, lengths)      # cache, block_table and lengths: this member's part
 
 The reference has no attention code; the exchange is its all-gather (``fcollect``,
-``src/ipc/context_ipc_tmpl_device.hpp:436-472``). On GPUs a step is one attention call, one all-gather kernel and one join
-on the current stream; on the CPU backend the same in plain PyTorch over the host-blocking all-gather.
-"""
+``src/ipc/context_ipc_tmpl_device.hpp:503-531``). On GPUs a step is one attention call, one all-gather kernel and one
+join on the current stream; on the CPU backend the same in plain PyTorch over the host-blocking all-gather. """
 from __future__ import annotations
 
 from typing import Optional
@@ -24,8 +24,8 @@ from ..ops import collectives as coll
 
 
 class ContextParallelDecode:
-    """Symmetric buffers for the partial results of one (team, batch, heads) combination; collective to create, to call and
-    to destroy. A team of one needs none and calls :func:`rocshmem_b200.ops.attention.paged_attention` directly."""
+    """Symmetric buffers for the partial results of one (team, batch, heads) combination; collective to create, to call
+    and to destroy. A team of one needs none and calls :func:`rocshmem_b200.ops.attention.paged_attention` directly."""
 
     def __init__(self, max_batch: int, heads: int, head_dim: int, team: Optional[rt.Team] = None):
         if rt.n_local_pes() != 1:
@@ -62,9 +62,9 @@ class ContextParallelDecode:
 
     def __call__(self, q: torch.Tensor, cache: attention.KvCache, block_table: torch.Tensor, lengths: torch.Tensor,
                  scale: Optional[float] = None, softcap: float = 0.0) -> torch.Tensor:
-        """``q [B, heads, head_dim]``, the same on every member; ``cache``, ``block_table [B, pages]`` and ``lengths [B]``
-        describe this member's part and may be empty (a length of zero). Returns the attention over all members' tokens
-        ``[B, heads, head_dim]`` in q's type, the same bits on every member. Arguments as in
+        """``q [B, heads, head_dim]``, the same on every member; ``cache``, ``block_table [B, pages]`` and ``lengths
+        [B]`` describe this member's part and may be empty (a length of zero). Returns the attention over all members'
+        tokens ``[B, heads, head_dim]`` in q's type, the same bits on every member. Arguments as in
         :func:`rocshmem_b200.ops.attention.paged_attention`; sliding windows, which go by positions in the whole
         sequence, are the caller's to express through the parts' block tables and lengths."""
         if q.dim() != 3 or q.shape[1:] != (self.heads, self.head_dim) or q.shape[0] > self.max_batch:
@@ -75,7 +75,8 @@ class ContextParallelDecode:
         if self.n == 1:
             if cuda:
                 return attention.paged_attention(q, cache, block_table, lengths, scale=scale, softcap=softcap)
-            return attention.ref_paged_attention(q, cache, block_table, lengths, scale=scale, softcap=softcap)[0].to(q.dtype)
+            return attention.ref_paged_attention(q, cache, block_table, lengths, scale=scale,
+                softcap=softcap)[0].to(q.dtype)
         if self.mine is None:
             raise RuntimeError("ContextParallelDecode was destroyed")
         B = q.shape[0]

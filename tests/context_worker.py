@@ -1,5 +1,5 @@
-"""One PE of the sequence-sharded decode test (started by test_context_decode.py): the cache of a batch is spread over the
-members, some of which hold nothing of a sequence; every member's result is the attention over all tokens."""
+"""One PE of the sequence-sharded decode test (started by test_context_decode.py): the cache of a batch is spread over
+the members, some of which hold nothing of a sequence; every member's result is the attention over all tokens."""
 import os
 
 import torch

@@ -1,5 +1,6 @@
-// The arithmetic of paged attention's split (attention_plan.hpp) on the CPU: every tile of every pair is taken by exactly
-// one share, in order; partial results of one pair lie in places of their own; rows of pages that do not exist are refused.
+// The arithmetic of paged attention's split (attention_plan.hpp) on the CPU: every tile of every pair is taken by
+// exactly one share, in order; partial results of one pair lie in places of their own; rows of pages that do not exist
+// are refused.
 #include <cstdio>
 #include <cstdlib>
 #include <map>
@@ -58,7 +59,8 @@ void check_division() {
   std::mt19937 rng(9);
   for (uint32_t d = 1; d < 5000; ++d) {
     const Divisor v = divisor(d);
-    for (uint32_t n : {0u, 1u, d - 1, d, d + 1, 2 * d - 1, 2 * d, 0x7fffffffu, 0x7fffffffu - d, 0x7fffffffu / d * d, 0x7fffffffu / d * d - 1,
+    for (uint32_t n : {0u, 1u, d - 1, d, d + 1, 2 * d - 1, 2 * d, 0x7fffffffu, 0x7fffffffu - d, 0x7fffffffu / d * d,
+        0x7fffffffu / d * d - 1,
                        static_cast<uint32_t>(rng() >> 1), static_cast<uint32_t>(rng() >> 9), static_cast<uint32_t>(rng() >> 20)}) {
       if (n <= 0x7fffffffu) CHECK(divide(n, v) == n / d);
     }
@@ -68,7 +70,8 @@ void check_division() {
   }
 }
 
-void check_split(const std::vector<int> &lengths, int capacity, int window, int units, int shares, int least, int tile) {
+void check_split(const std::vector<int> &lengths, int capacity, int window, int units, int shares, int least,
+    int tile) {
   std::vector<long long> bases;
   long long total = 0;
   for (int n : lengths) {

@@ -25,7 +25,8 @@ def test_split_over_blocks_and_rows_of_pages(tmp_path):
 
 
 def norm_rope_args(**over):
-    a = dict(q=torch.zeros(3, 4, 64, dtype=BF16), k=torch.zeros(3, 2, 64, dtype=BF16), q_weight=torch.ones(64, dtype=BF16),
+    a = dict(q=torch.zeros(3, 4, 64, dtype=BF16), k=torch.zeros(3, 2, 64, dtype=BF16),
+        q_weight=torch.ones(64, dtype=BF16),
              k_weight=torch.ones(64, dtype=BF16), positions=torch.zeros(3, dtype=torch.int32), table=torch.zeros(8, 64))
     a.update(over)
     return a
@@ -76,8 +77,10 @@ def kv(dtype=BF16, pages=4, heads=2, size=16, dim=64):
     lambda: kv(dim=60),
     lambda: kv(dim=264),
     lambda: at.KvCache(torch.zeros(4, 2, 16, 64).to(E4M3), torch.zeros(4, 2, 16, 64).to(E4M3)),
-    lambda: at.KvCache(torch.zeros(4, 2, 16, 64).to(E4M3), torch.zeros(4, 2, 16, 64).to(E4M3), torch.ones(4, 2, 8), torch.ones(4, 2, 16)),
-    lambda: at.KvCache(torch.zeros(4, 2, 16, 64, dtype=BF16), torch.zeros(4, 2, 16, 64, dtype=BF16), torch.ones(4, 2, 16), None),
+    lambda: at.KvCache(torch.zeros(4, 2, 16, 64).to(E4M3), torch.zeros(4, 2, 16, 64).to(E4M3), torch.ones(4, 2, 8),
+        torch.ones(4, 2, 16)),
+    lambda: at.KvCache(torch.zeros(4, 2, 16, 64, dtype=BF16), torch.zeros(4, 2, 16, 64, dtype=BF16),
+        torch.ones(4, 2, 16), None),
     lambda: at.KvCache(torch.zeros(4, 2, 64, 16, dtype=BF16).transpose(2, 3), torch.zeros(4, 2, 16, 64, dtype=BF16)),
 ])
 def test_cache_refusals(make):
@@ -106,7 +109,8 @@ def test_cache_shape_properties_and_frozen():
     (dict(), ValueError, "CUDA device"),
 ])
 def test_write_refusals(over, error, match):
-    a = dict(k=torch.zeros(3, 2, 64, dtype=BF16), v=torch.zeros(3, 2, 64, dtype=BF16), slots=torch.zeros(3, dtype=torch.int64))
+    a = dict(k=torch.zeros(3, 2, 64, dtype=BF16), v=torch.zeros(3, 2, 64, dtype=BF16),
+        slots=torch.zeros(3, dtype=torch.int64))
     a.update(over)
     with pytest.raises(error, match=match):
         at.kv_cache_write(kv(), **a)

@@ -1,5 +1,5 @@
-"""Decoding over a cache that is spread over a team (rocshmem_b200.parallel.context): several processes on the CPU backend,
-one process on a GPU, several GPUs where there are any."""
+"""Decoding over a cache that is spread over a team (rocshmem_b200.parallel.context): several processes on the CPU
+backend, one process on a GPU, several GPUs where there are any."""
 import os
 import subprocess
 import sys
@@ -47,8 +47,8 @@ def test_members_join_their_parts_on_gpus():
 
 @pytest.mark.gpu
 def test_parts_in_one_buffer_join_to_the_whole():
-    """What the members of a team of three do between the collectives, with one process's buffer in place of the gathered one: each
-    part is written where the all-gather would put it."""
+    """What the members of a team of three do between the collectives, with one process's buffer in place of the
+    gathered one: each part is written where the all-gather would put it."""
     from rocshmem_b200.ops import attention as at
     from rocshmem_b200.parallel.context import ContextParallelDecode
     step = ContextParallelDecode.__new__(ContextParallelDecode)

@@ -1,6 +1,7 @@
 """Attention operators on a GPU against plain PyTorch in 64 bits.
 
-Tolerances, with u the half step of the result's type (eps / 2) and 2^-23 for one fp32 operation (tensor cores truncate):
+Tolerances, with u the half step of the result's type (eps / 2) and 2^-23 for one fp32 operation (tensor cores
+truncate):
 
 * norm and rotation: the result's rounding, and fp32 sums of D squares, each at most D / 8 + 8 additions deep in a lane and
   across lanes: (D / 8 + 16) 2^-23 of the magnitudes that enter an element;
@@ -117,13 +118,14 @@ def test_norm_rope_and_gradients(T, Hq, Hk, D, R, dtype, weight, interleaved, fu
         near(back[i], dx, HALF_STEP[dtype] * dx.abs() + (D / 4 + 32) * ONE * size + smallest, "input gradient")
         # A sum of T x H terms in fp32; a term itself is a few operations off.
         terms = (a * n.abs()).sum(dim=(0, 1))
-        near(back[2 + i], dw, HALF_STEP[weight] * dw.abs() + (T * x.shape[1] + D / 8 + 64) * ONE * terms, "weight gradient")
+        near(back[2 + i], dw, HALF_STEP[weight] * dw.abs() + (T * x.shape[1] + D / 8 + 64) * ONE * terms,
+            "weight gradient")
 
 
 def test_norm_rope_gradient_against_differences():
-    """The slope of L = sum of g q' + g' k' along a random direction, from two forward passes: central differences are off by
-    h^2 / 6 of the third derivative (a few units for rows of norm 1) and 2^-22 / h of the terms; 1e-3 of the terms covers both
-    at h = 2^-6."""
+    """The slope of L = sum of g q' + g' k' along a random direction, from two forward passes: central differences are
+    off by h^2 / 6 of the third derivative (a few units for rows of norm 1) and 2^-22 / h of the terms; 1e-3 of the
+    terms covers both at h = 2^-6."""
     at, q, k, wq, wk, pos, table = norm_rope_case(40, 4, 2, 64, 64, F32, F32, False, False, seed=5)
     leaves = [t.requires_grad_() for t in (q, k, wq, wk)]
     got = at.qk_norm_rope(*leaves, pos, table)
@@ -416,7 +418,8 @@ def test_paged_attention_caps_and_windows(softcap, window, scale, cache):
 def test_paged_attention_does_not_see_bad_pages_or_bad_lengths():
     from rocshmem_b200.ops import attention as at
     for cache in (BF16, E4M3):
-        c, q, table, ln = paged_case([200, 200, 90, 64, 10], 8, 2, 128, 16, BF16, cache, seed=2, extra_pages=0, poison=False)
+        c, q, table, ln = paged_case([200, 200, 90, 64, 10], 8, 2, 128, 16, BF16, cache, seed=2, extra_pages=0,
+            poison=False)
         table[0, 2], table[0, 5], table[1, :] = -1, c.num_pages, 2 ** 31 - 1
         table[2, 0] = -2 ** 31
         ln[2], ln[3], ln[4] = 10 ** 6, -5, 2 ** 31 - 1
@@ -451,7 +454,8 @@ def test_paged_attention_strides_and_given_results():
 
 
 def test_paged_attention_extreme_values():
-    """Queries and factors far from one, keys and values of the type's largest, scores of -inf, infinities and NaN that are seen."""
+    """Queries and factors far from one, keys and values of the type's largest, scores of -inf, infinities and NaN that
+    are seen."""
     from rocshmem_b200.ops import attention as at
     c, q, table, ln = paged_case([40, 300], 8, 2, 128, 16, BF16, E4M3, seed=3, poison=False)
     c.k_scale.mul_(1e-30)
@@ -545,10 +549,12 @@ def test_streams_are_refused_or_followed():
     assert torch.equal(rk, (codes.float() * factors[..., None]).to(BF16))
 
 
-# ---- join -------------------------------------------------------------------------------------------------------------
+# ---- join ------------------------------------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("n,B,H,D,dtype,out_dtype", [(1, 1, 1, 64, F32, BF16), (2, 3, 8, 128, F32, BF16), (3, 70, 5, 96, BF16, F32),
-                                                      (8, 33, 16, 256, F32, F16), (17, 2, 2, 8, F16, F16), (9, 5, 7, 200, BF16, BF16)])
+@pytest.mark.parametrize("n,B,H,D,dtype,out_dtype",
+    [(1, 1, 1, 64, F32, BF16), (2, 3, 8, 128, F32, BF16), (3, 70, 5, 96, BF16, F32),
+                                                      (8, 33, 16, 256, F32, F16), (17, 2, 2, 8, F16, F16), (9, 5, 7,
+                                                          200, BF16, BF16)])
 def test_attention_join(n, B, H, D, dtype, out_dtype):
     from rocshmem_b200.ops import attention as at
     g = gen(n * D)
@@ -590,8 +596,8 @@ def test_attention_join_of_parts_that_lie_apart_and_of_nan():
 
 @pytest.mark.parametrize("cache,size", [(BF16, 16), (E4M3, 32)])
 def test_prefill_then_decode_steps(cache, size):
-    """Prompts are normed, rotated and written, then tokens are added one by one; each step's result is the attention over
-    all rows so far, as the cache holds them. The cache of one sequence split over two joins to the same."""
+    """Prompts are normed, rotated and written, then tokens are added one by one; each step's result is the attention
+    over all rows so far, as the cache holds them. The cache of one sequence split over two joins to the same."""
     from rocshmem_b200.ops import attention as at
     g = gen(31)
     B, H, K, D = 3, 8, 2, 128
@@ -631,8 +637,8 @@ def test_prefill_then_decode_steps(cache, size):
 # ---- captures, far offsets, odd but allowed arguments ---------------------------------------------------------------
 
 def test_norm_rope_training_step_in_a_graph():
-    """Forward and backward captured together and replayed on new contents; refused while an eager graph of the same leaves
-    is alive."""
+    """Forward and backward captured together and replayed on new contents; refused while an eager graph of the same
+    leaves is alive."""
     at, q, k, wq, wk, pos, table = norm_rope_case(200, 4, 2, 128, 128, BF16, F32, False, False, seed=8)
     leaves = [t.detach().clone().requires_grad_() for t in (q, k, wq, wk)]
     grads = [randn(gen(20 + i), *t.shape, dtype=BF16) for i, t in enumerate((q, k))]
@@ -689,7 +695,8 @@ def test_rows_behind_four_gigabytes(cache):
     small = at.KvCache.allocate(3, size, K, D, cache)
     near_table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
     at.kv_cache_write(small, k, v, at.token_slots(near_table, torch.zeros_like(pos), pos, size))
-    for a, b in zip(at.kv_cache_read(c, slots), at.kv_cache_read(small, at.token_slots(near_table, torch.zeros_like(pos), pos, size))):
+    for a, b in zip(at.kv_cache_read(c, slots),
+        at.kv_cache_read(small, at.token_slots(near_table, torch.zeros_like(pos), pos, size))):
         assert torch.equal(a, b) and (cache == E4M3 or torch.equal(a, k) or torch.equal(a, v))
     q = randn(g, 1, 8, D, dtype=BF16)
     ln = torch.tensor([n], dtype=torch.int32, device="cuda")
@@ -727,12 +734,14 @@ def test_expanded_queries_and_caches_that_are_copied():
         assert torch.equal(at.paged_attention(one, other, table, ln), want)
     assert c != copy.copy(c) and c == c
     with pytest.raises(ValueError, match="gradient"):
-        at.KvCache(torch.zeros(2, 2, 16, 64, dtype=BF16, device="cuda", requires_grad=True), torch.zeros(2, 2, 16, 64, dtype=BF16, device="cuda"))
+        at.KvCache(torch.zeros(2, 2, 16, 64, dtype=BF16, device="cuda", requires_grad=True),
+            torch.zeros(2, 2, 16, 64, dtype=BF16, device="cuda"))
 
 
 @pytest.mark.parametrize("cache", [BF16, E4M3])
 @pytest.mark.parametrize("D", [64, 128, 256])
-@pytest.mark.parametrize("B,K,H,pages", [(1, 1, 1, 1), (2, 2, 12, 7), (37, 4, 16, 20), (37, 4, 16, 33), (149, 1, 8, 5), (5, 1, 40, 16)])
+@pytest.mark.parametrize("B,K,H,pages", [(1, 1, 1, 1), (2, 2, 12, 7), (37, 4, 16, 20), (37, 4, 16, 33), (149, 1, 8,
+    5), (5, 1, 40, 16)])
 def test_paged_attention_one_launch_and_two(cache, D, B, K, H, pages):
     """Calls on both sides of the rule that chooses between a block for each pair and shares of all tiles."""
     from rocshmem_b200.ops import attention as at
