@@ -5,6 +5,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/pybind11.h>
@@ -98,6 +99,16 @@ void no_grad(const char *what, std::initializer_list<const Tensor *> tensors) {
   }
 }
 
+// A dual tensor (forward-mode differentiation) does not require a gradient: its tangent would be dropped without a word.
+void no_tangent(const char *what, std::initializer_list<const Tensor *> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor *t : tensors) {
+    if (t != nullptr && t->_fw_grad(/*level=*/0).defined()) {
+      bad_value(what, " has no forward-mode derivative: pass primals (torch.autograd.forward_ad.unpack_dual)");
+    }
+  }
+}
+
 void on_one_device(const char *what, std::initializer_list<const Tensor *> tensors) {
   const at::Device device = (*tensors.begin())->device();
   if (!device.is_cuda()) bad_value(what, ": tensors must be on a CUDA device");
@@ -171,6 +182,7 @@ NormRopeArgs norm_rope_args(const Tensor &q, const Tensor &k, const Tensor &q_we
     bad_value("the table's rows must have a multiple of 16 elements up to ", D, ", got ", table.sizes());
   }
   const int wide = index(positions, "positions", T);
+  no_tangent("qk_norm_rope", {&q, &k, &q_weight, &k_weight, &table});
   on_one_device("qk_norm_rope", {&q, &k, &q_weight, &k_weight, &positions, &table});
   NormRopeArgs a{};
   a.q = data(q);
@@ -315,6 +327,7 @@ KvCacheArgs cache_args(const Cache &c) {
   for (const Tensor *t : {&c.k, &c.v}) {
     if (t->requires_grad()) bad_value("KvCache: the cache is written in place and cannot require a gradient");
   }
+  no_tangent("KvCache", {&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)});
   int shift = 0;
   while ((int64_t{1} << shift) < size) ++shift;
   return KvCacheArgs{data(k), data(v), scaled ? static_cast<float *>(data(*c.k_scale)) : nullptr,
@@ -331,6 +344,7 @@ void py_kv_cache_write(const Cache &c, const Tensor &k, const Tensor &v, const T
   if (v.size(0) != k.size(0)) bad_value("k and v must have the same tokens, got ", k.size(0), " and ", v.size(0));
   const int wide = index(slots, "slots", k.size(0));
   no_grad("kv_cache_write", {&k, &v});
+  no_tangent("kv_cache_write", {&k, &v});
   on_one_device("kv_cache_write", {&k, &v, &slots, &c.k});
   for (const Tensor *t : {&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)}) {
     if (t != nullptr && (overlap(*t, k) || overlap(*t, v))) {
@@ -427,6 +441,7 @@ std::pair<Tensor, OptTensor> py_paged_attention(const Tensor &q, const Cache &c,
   }
   if (lse_given) result(*lse_given, "lse", q.sizes().slice(0, 2), {at::kFloat}, inputs);
   no_grad("paged_attention", {&q});
+  no_tangent("paged_attention", {&q, or_null(out_given), or_null(lse_given)});
   on_one_device("paged_attention", {&q, &block_table, &lengths, &c.k, or_null(out_given), or_null(lse_given)});
   const Here here(q);
   const auto fp32 = q.options().dtype(at::kFloat);
@@ -471,6 +486,7 @@ std::pair<Tensor, Tensor> py_attention_join(const Tensor &outs, const Tensor &ls
   if (!is_float(dtype)) bad_type("dtype must be bf16, fp16 or fp32, got ", dtype);
   if (out_given) result(*out_given, "out", outs.sizes().slice(1), {dtype}, {&outs, &lses});
   no_grad("attention_join", {&outs, &lses});
+  no_tangent("attention_join", {&outs, &lses, or_null(out_given)});
   on_one_device("attention_join", {&outs, &lses, or_null(out_given)});
   const Here here(outs);
   Tensor out = out_given ? *out_given : at::empty(outs.sizes().slice(1), outs.options().dtype(dtype));

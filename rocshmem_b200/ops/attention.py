@@ -88,8 +88,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     2)``, or with ``interleaved`` ``(2 i, 2 i + 1)``. ``positions [T]`` int32 or int64: a negative one marks padding,
     whose rows become zeros and have no gradient; one past the table makes its token's rows NaN.
 
-    Differentiable once (``create_graph`` is refused) with respect to ``q``, ``k`` and both weights; the weights'
-    gradients are the same in every run. A backward pass can be captured into a CUDA graph with its forward pass; while
+    Differentiable once (``create_graph`` and forward-mode derivatives are refused) with respect to ``q``, ``k`` and
+    both weights; the weights' gradients are the same in every run. A backward pass can be captured into a CUDA graph with its forward pass; while
     an eager graph of the same leaves is alive, the captured forward pass is refused."""
     if stream is not None:
         with _On(stream, q, k, q_weight, k_weight, positions, table):

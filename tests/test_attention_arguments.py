@@ -1,0 +1,84 @@
+"""Attention operators without a GPU: calls that would drop a derivative, write over what somebody else keeps, or mean
+something else than they say. All are refused before anything touches a device, so CPU tensors show it: what passes
+every check ends with the refusal of the CPU device."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from rocshmem_b200.ops import attention as at
+
+BF16, F16, F32, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
+
+
+def zeros(*shape, dtype=BF16, **kw):
+    return torch.zeros(*shape, dtype=dtype, **kw)
+
+
+def cache(dtype=BF16, pages=4, heads=2, size=16, dim=64):
+    return at.KvCache.allocate(pages, size, heads, dim, dtype, device="cpu")
+
+
+def norm_rope(**over):
+    a = dict(q=zeros(3, 4, 64, dtype=F32), k=zeros(3, 2, 64, dtype=F32), q_weight=torch.ones(64),
+             k_weight=torch.ones(64), positions=torch.zeros(3, dtype=torch.int32), table=torch.zeros(8, 64))
+    a.update(over)
+    return at.qk_norm_rope(**a)
+
+
+def write(c=None, **over):
+    a = dict(k=zeros(3, 2, 64), v=zeros(3, 2, 64), slots=torch.arange(3))
+    a.update(over)
+    return at.kv_cache_write(c or cache(), **a)
+
+
+def attend(c=None, **over):
+    a = dict(q=zeros(2, 4, 64), block_table=torch.zeros(2, 2, dtype=torch.int32),
+             lengths=torch.zeros(2, dtype=torch.int32))
+    a.update(over)
+    return at.paged_attention(cache=c or cache(), **a)
+
+
+def join(**over):
+    a = dict(outs=torch.zeros(2, 3, 4, 64), lses=torch.zeros(2, 3, 4))
+    a.update(over)
+    return at.attention_join(**a)
+
+
+# ---- forward-mode derivatives ---------------------------------------------------------------------------------------
+
+def dual(x):
+    return fwd.make_dual(x, torch.ones_like(x))
+
+
+@pytest.mark.parametrize("call", [
+    lambda: norm_rope(q=dual(zeros(3, 4, 64, dtype=F32))),
+    lambda: norm_rope(k=dual(zeros(3, 2, 64, dtype=F32))),
+    lambda: norm_rope(q_weight=dual(torch.ones(64))),
+    lambda: norm_rope(k_weight=dual(torch.ones(64))),
+    lambda: norm_rope(table=dual(torch.zeros(8, 64))),
+    lambda: write(k=dual(zeros(3, 2, 64))),
+    lambda: write(v=dual(zeros(3, 2, 64))),
+    lambda: at.KvCache(dual(zeros(4, 2, 16, 64)), zeros(4, 2, 16, 64)),
+    lambda: at.KvCache(zeros(4, 2, 16, 64, dtype=E4M3), zeros(4, 2, 16, 64, dtype=E4M3), torch.ones(4, 2, 16),
+                       dual(torch.ones(4, 2, 16))),
+    lambda: attend(q=dual(zeros(2, 4, 64))),
+    lambda: attend(out=dual(zeros(2, 4, 64))),
+    lambda: attend(lse=dual(torch.zeros(2, 4))),
+    lambda: join(outs=dual(torch.zeros(2, 3, 4, 64))),
+    lambda: join(lses=dual(torch.zeros(2, 3, 4))),
+    lambda: join(out=dual(torch.zeros(3, 4, 64))),
+])
+def test_dual_tensors_are_refused(call):
+    with fwd.dual_level():
+        with pytest.raises(ValueError, match="no forward-mode derivative"):
+            call()
+
+
+def test_primals_within_a_dual_level_pass():
+    with fwd.dual_level():
+        for call in (norm_rope, write, attend, join):
+            with pytest.raises(ValueError, match="CUDA device"):
+                call()
+        q = fwd.unpack_dual(dual(zeros(2, 4, 64))).primal
+        with pytest.raises(ValueError, match="CUDA device"):
+            attend(q=q)
