@@ -65,6 +65,19 @@ bool is_half(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
 bool aligned(const Tensor &t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
 void *data(const Tensor &t) { return const_cast<void *>(t.const_data_ptr()); }
 
+// Tensors inside a torch.func transform are wrappers without memory of their own. Called before an address is taken.
+void no_transform(const char *what, std::initializer_list<const Tensor *> tensors) {
+  static const c10::DispatchKeySet wrappers({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+      c10::DispatchKey::Functionalize});
+  for (const Tensor *t : tensors) {
+    if (t != nullptr && t->key_set().has_any(wrappers)) {
+      bad_value(what, " cannot be called inside a torch.func transform (vmap, grad, jvp and the like)");
+    }
+  }
+}
+
+const Tensor *or_null(const OptTensor &t) { return t.has_value() ? &*t : nullptr; }
+
 // Strides of dimensions 0 and 1 of t [tokens, heads, dim], whose rows the kernels read 16 bytes at a time.
 struct Strides {
   int64_t token, head;
@@ -117,8 +130,6 @@ void on_one_device(const char *what, std::initializer_list<const Tensor *> tenso
   }
 }
 
-const Tensor *or_null(const OptTensor &t) { return t.has_value() ? &*t : nullptr; }
-
 // The inputs' device for the duration of a call, and its current stream.
 struct Here {
   explicit Here(const Tensor &t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
@@ -155,6 +166,7 @@ void result(const Tensor &t, const char *name, at::IntArrayRef shape, std::initi
 
 NormRopeArgs norm_rope_args(const Tensor &q, const Tensor &k, const Tensor &q_weight, const Tensor &k_weight,
                             const Tensor &positions, const Tensor &table, double eps, bool interleaved) {
+  no_transform("qk_norm_rope", {&q, &k, &q_weight, &k_weight, &positions, &table});
   if (!is_float(q.scalar_type()) || k.scalar_type() != q.scalar_type()) {
     bad_type("q and k must both be bf16, fp16 or fp32, got ", q.scalar_type(), " and ", k.scalar_type());
   }
@@ -298,6 +310,7 @@ struct Cache {
 
 KvCacheArgs cache_args(const Cache &c) {
   const Tensor &k = c.k, &v = c.v;
+  no_transform("KvCache", {&k, &v, or_null(c.k_scale), or_null(c.v_scale)});
   if (k.dim() != 4 || v.sizes() != k.sizes() || k.scalar_type() != v.scalar_type() ||
       !(is_half(k.scalar_type()) || k.scalar_type() == at::kFloat8_e4m3fn)) {
     bad_value("KvCache: k and v must both be [pages, kv_heads, page_size, head_dim] in bf16, fp16 or e4m3");
@@ -337,6 +350,7 @@ KvCacheArgs cache_args(const Cache &c) {
 
 void py_kv_cache_write(const Cache &c, const Tensor &k, const Tensor &v, const Tensor &slots) {
   const KvCacheArgs a = cache_args(c);
+  no_transform("kv_cache_write", {&k, &v, &slots});
   if (!is_float(k.scalar_type()) || v.scalar_type() != k.scalar_type()) {
     bad_type("k and v must both be bf16, fp16 or fp32, got ", k.scalar_type(), " and ", v.scalar_type());
   }
@@ -358,6 +372,7 @@ void py_kv_cache_write(const Cache &c, const Tensor &k, const Tensor &v, const T
 
 std::pair<Tensor, Tensor> py_kv_cache_read(const Cache &c, const Tensor &slots, at::ScalarType dtype) {
   const KvCacheArgs a = cache_args(c);
+  no_transform("kv_cache_read", {&slots});
   if (!is_float(dtype)) bad_type("dtype must be bf16, fp16 or fp32, got ", dtype);
   if (slots.dim() != 1 || slots.size(0) > INT32_MAX) bad_value("slots must be [T]");
   const int64_t T = slots.size(0);
@@ -382,6 +397,7 @@ struct Paged {
 Paged check_paged(const Tensor &q, const Cache &c, const Tensor &block_table, const Tensor &lengths,
                   std::optional<double> scale, double softcap, int64_t window) {
   Paged p{cache_args(c), {}};
+  no_transform("paged_attention", {&q, &block_table, &lengths});
   if (!is_half(q.scalar_type()) || (p.cache.type != ATTN_E4M3 && p.cache.type != code(q.scalar_type()))) {
     bad_type("q must be bf16 or fp16, and of the cache's type unless that is e4m3: got ", q.scalar_type(), " and ",
         c.k.scalar_type());
@@ -435,6 +451,7 @@ std::pair<Tensor, OptTensor> py_paged_attention(const Tensor &q, const Cache &c,
   Paged p = check_paged(q, c, block_table, lengths, scale, softcap, window);
   const std::initializer_list<const Tensor *> inputs = {&q, &block_table, &lengths, &c.k, &c.v, or_null(c.k_scale),
       or_null(c.v_scale)};
+  no_transform("paged_attention", {or_null(out_given), or_null(lse_given)});
   if (out_given) {
     result(*out_given, "out", q.sizes(), {q.scalar_type(), at::kFloat}, inputs);
     if (lse_given && overlap(*out_given, *lse_given)) bad_value("out shares memory with lse");
@@ -461,6 +478,7 @@ std::pair<Tensor, OptTensor> py_paged_attention(const Tensor &q, const Cache &c,
 std::pair<Tensor, Tensor> py_attention_join(const Tensor &outs, const Tensor &lses,
     std::optional<at::ScalarType> dtype_given,
                                             const OptTensor &out_given) {
+  no_transform("attention_join", {&outs, &lses, or_null(out_given)});
   if (!is_float(outs.scalar_type()) || lses.scalar_type() != at::kFloat) {
     bad_type("outs must be bf16, fp16 or fp32, lses fp32");
   }

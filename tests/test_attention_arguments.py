@@ -82,3 +82,25 @@ def test_primals_within_a_dual_level_pass():
         q = fwd.unpack_dual(dual(zeros(2, 4, 64))).primal
         with pytest.raises(ValueError, match="CUDA device"):
             attend(q=q)
+
+
+# ---- torch.func transforms ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("call", [
+    lambda: torch.func.vmap(lambda q: norm_rope(q=q))(zeros(2, 3, 4, 64, dtype=F32)),
+    lambda: torch.func.grad(lambda q: norm_rope(q=q)[0].sum())(zeros(3, 4, 64, dtype=F32)),
+    lambda: torch.func.jvp(lambda t: norm_rope(table=t)[0], (torch.zeros(8, 64),), (torch.ones(8, 64),)),
+    lambda: torch.func.functionalize(lambda w: norm_rope(q_weight=w)[0])(torch.ones(64)),
+    lambda: torch.func.vmap(lambda k: write(k=k) or k)(zeros(2, 3, 2, 64)),
+    lambda: torch.func.vmap(lambda slots: at.kv_cache_read(cache(), slots)[0])(torch.zeros(2, 3, dtype=torch.int64)),
+    lambda: torch.func.vmap(lambda k: at.KvCache(k, zeros(4, 2, 16, 64)) and k)(zeros(2, 4, 2, 16, 64)),
+    lambda: torch.func.vmap(lambda q: attend(q=q))(zeros(3, 2, 4, 64)),
+    lambda: torch.func.grad(lambda q: attend(q=q).float().sum())(zeros(2, 4, 64)),
+    lambda: torch.func.vmap(lambda out: attend(out=out))(zeros(3, 2, 4, 64)),
+    lambda: torch.func.vmap(lambda n: attend(lengths=n))(torch.zeros(3, 2, dtype=torch.int32)),
+    lambda: torch.func.vmap(lambda outs: join(outs=outs)[0])(torch.zeros(5, 2, 3, 4, 64)),
+    lambda: torch.func.jvp(lambda l: join(lses=l)[1], (torch.zeros(2, 3, 4),), (torch.ones(2, 3, 4),)),
+])
+def test_transforms_are_refused_by_the_operators_themselves(call):
+    with pytest.raises(ValueError, match="torch.func transform"):
+        call()
