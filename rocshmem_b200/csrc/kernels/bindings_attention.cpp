@@ -194,6 +194,9 @@ NormRopeArgs norm_rope_args(const Tensor &q, const Tensor &k, const Tensor &q_we
     bad_value("the table's rows must have a multiple of 16 elements up to ", D, ", got ", table.sizes());
   }
   const int wide = index(positions, "positions", T);
+  if (at::GradMode::is_enabled() && table.requires_grad()) {
+    bad_value("qk_norm_rope has no gradient for its table: detach it");
+  }
   no_tangent("qk_norm_rope", {&q, &k, &q_weight, &k_weight, &table});
   on_one_device("qk_norm_rope", {&q, &k, &q_weight, &k_weight, &positions, &table});
   NormRopeArgs a{};

@@ -89,7 +89,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     whose rows become zeros and have no gradient; one past the table makes its token's rows NaN.
 
     Differentiable once (``create_graph`` and forward-mode derivatives are refused) with respect to ``q``, ``k`` and
-    both weights; the weights' gradients are the same in every run. A backward pass can be captured into a CUDA graph with its forward pass; while
+    both weights; the weights' gradients are the same in every run. A ``table`` that requires a gradient is refused. A backward pass can be captured into a CUDA graph with its forward pass; while
     an eager graph of the same leaves is alive, the captured forward pass is refused."""
     if stream is not None:
         with _On(stream, q, k, q_weight, k_weight, positions, table):

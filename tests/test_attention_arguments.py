@@ -104,3 +104,19 @@ def test_primals_within_a_dual_level_pass():
 def test_transforms_are_refused_by_the_operators_themselves(call):
     with pytest.raises(ValueError, match="torch.func transform"):
         call()
+
+
+# ---- gradients that no operator computes ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("leaves", [False, True])
+def test_a_table_that_requires_a_gradient_is_refused(leaves):
+    """Alone its gradient would be cut off, beside trained inputs it would be undefined: frequencies that never train."""
+    frequencies = torch.full((32,), 0.5, requires_grad=True)
+    table = at.rope_table(8, 64, frequencies=frequencies)
+    assert table.requires_grad
+    q = zeros(3, 4, 64, dtype=F32, requires_grad=leaves)
+    with pytest.raises(ValueError, match="gradient for its table"):
+        norm_rope(q=q, table=table)
+    for fine in (lambda: norm_rope(q=q, table=table.detach()), torch.no_grad()(lambda: norm_rope(q=q, table=table))):
+        with pytest.raises(ValueError, match="CUDA device"):
+            fine()
