@@ -340,8 +340,8 @@ KvCacheArgs cache_args(const Cache &c) {
       bad_value("KvCache: tensors must be contiguous, 16-byte aligned and on one device");
     }
   }
-  for (const Tensor *t : {&c.k, &c.v}) {
-    if (t->requires_grad()) bad_value("KvCache: the cache is written in place and cannot require a gradient");
+  for (const Tensor *t : {&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)}) {
+    if (t != nullptr && t->requires_grad()) bad_value("KvCache: the cache is written in place and cannot require a gradient");
   }
   no_tangent("KvCache", {&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)});
   int shift = 0;

@@ -120,3 +120,17 @@ def test_a_table_that_requires_a_gradient_is_refused(leaves):
     for fine in (lambda: norm_rope(q=q, table=table.detach()), torch.no_grad()(lambda: norm_rope(q=q, table=table))):
         with pytest.raises(ValueError, match="CUDA device"):
             fine()
+
+
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_factors_that_require_a_gradient_are_refused(which):
+    """At construction, and at a call where they came to require one later."""
+    c = cache(E4M3)
+    parts = dict(k=c.k, v=c.v, k_scale=c.k_scale, v_scale=c.v_scale)
+    parts[which] = torch.zeros(4, 2, 16, requires_grad=True)
+    with pytest.raises(ValueError, match="cannot require a gradient"):
+        at.KvCache(**parts)
+    getattr(c, which).requires_grad_()
+    for call in (write, attend, lambda c: at.kv_cache_read(c, torch.arange(3))):
+        with pytest.raises(ValueError, match="cannot require a gradient"):
+            call(c)
