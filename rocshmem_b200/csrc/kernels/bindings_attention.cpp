@@ -106,8 +106,8 @@ int index(const Tensor &t, const char *name, int64_t count) {
 void no_grad(const char *what, std::initializer_list<const Tensor *> tensors) {
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor *t : tensors) {
-    if (t->requires_grad()) {
-      bad_value(what, " has no backward pass: call it under torch.no_grad(), or detach its inputs");
+    if (t != nullptr && t->requires_grad()) {
+      bad_value(what, " has no backward pass: call it under torch.no_grad(), or detach its tensors");
     }
   }
 }
@@ -460,7 +460,7 @@ std::pair<Tensor, OptTensor> py_paged_attention(const Tensor &q, const Cache &c,
     if (lse_given && overlap(*out_given, *lse_given)) bad_value("out shares memory with lse");
   }
   if (lse_given) result(*lse_given, "lse", q.sizes().slice(0, 2), {at::kFloat}, inputs);
-  no_grad("paged_attention", {&q});
+  no_grad("paged_attention", {&q, or_null(out_given), or_null(lse_given)});
   no_tangent("paged_attention", {&q, or_null(out_given), or_null(lse_given)});
   on_one_device("paged_attention", {&q, &block_table, &lengths, &c.k, or_null(out_given), or_null(lse_given)});
   const Here here(q);
@@ -506,7 +506,7 @@ std::pair<Tensor, Tensor> py_attention_join(const Tensor &outs, const Tensor &ls
   const at::ScalarType dtype = dtype_given ? *dtype_given : out_given ? out_given->scalar_type() : outs.scalar_type();
   if (!is_float(dtype)) bad_type("dtype must be bf16, fp16 or fp32, got ", dtype);
   if (out_given) result(*out_given, "out", outs.sizes().slice(1), {dtype}, {&outs, &lses});
-  no_grad("attention_join", {&outs, &lses});
+  no_grad("attention_join", {&outs, &lses, or_null(out_given)});
   no_tangent("attention_join", {&outs, &lses, or_null(out_given)});
   on_one_device("attention_join", {&outs, &lses, or_null(out_given)});
   const Here here(outs);

@@ -134,3 +134,17 @@ def test_factors_that_require_a_gradient_are_refused(which):
     for call in (write, attend, lambda c: at.kv_cache_read(c, torch.arange(3))):
         with pytest.raises(ValueError, match="cannot require a gradient"):
             call(c)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: attend(out=zeros(2, 4, 64, requires_grad=True)),
+    lambda: attend(out=zeros(2, 4, 64, requires_grad=True) * 2),
+    lambda: attend(lse=torch.zeros(2, 4, requires_grad=True)),
+    lambda: join(out=torch.zeros(3, 4, 64, requires_grad=True)),
+])
+def test_given_results_that_require_a_gradient_are_refused(call):
+    """A result written over a tensor that autograd follows would leave the graph with another tensor's gradient."""
+    with pytest.raises(ValueError, match="no backward pass"):
+        call()
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
+        call()
