@@ -137,6 +137,14 @@ struct Here {
   void *stream;
 };
 
+// Tells autograd that tensors were written through their addresses, so that a backward pass that has saved one of them
+// is refused as after any other operation in place. Inference tensors have no version.
+void written(std::initializer_list<const Tensor *> tensors) {
+  for (const Tensor *t : tensors) {
+    if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  }
+}
+
 // Whether the address ranges of two tensors meet.
 bool overlap(const Tensor &a, const Tensor &b) {
   if (a.numel() == 0 || b.numel() == 0) return false;
@@ -371,6 +379,7 @@ void py_kv_cache_write(const Cache &c, const Tensor &k, const Tensor &v, const T
   const Here here(k);
   check(kv_cache_write(a, data(k), data(v), sk.token, sk.head, sv.token, sv.head, data(slots), wide,
                        static_cast<int>(k.size(0)), code(k.scalar_type()), here.stream), "kv_cache_write");
+  written({&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)});
 }
 
 std::pair<Tensor, Tensor> py_kv_cache_read(const Cache &c, const Tensor &slots, at::ScalarType dtype) {
@@ -475,6 +484,7 @@ std::pair<Tensor, OptTensor> py_paged_attention(const Tensor &q, const Cache &c,
   p.args.out_type = code(out.scalar_type());
   p.args.lse = lse ? static_cast<float *>(data(*lse)) : nullptr;
   check(paged_attention(p.cache, p.args, bytes > 0 ? data(workspace) : nullptr, bytes, here.stream), "paged_attention");
+  written({or_null(out_given), or_null(lse_given)});
   return {out, lse};
 }
 
@@ -516,6 +526,7 @@ std::pair<Tensor, Tensor> py_attention_join(const Tensor &outs, const Tensor &ls
       B * H,
                        static_cast<int>(D), code(outs.scalar_type()), code(dtype), data(out),
                        static_cast<float *>(data(lse)), here.stream), "attention_join");
+  written({or_null(out_given)});
   return {out, lse};
 }
 

@@ -1,0 +1,71 @@
+"""Attention operators on a GPU, beside test_gpu_attention.py: tensors that are written in place."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, E4M3 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, dtype=F32, scale=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+# ---- tensors that are written in place ------------------------------------------------------------------------------
+
+def small_call(cache_dtype=BF16):
+    from rocshmem_b200.ops import attention as at
+    g = gen(1)
+    c = at.KvCache.allocate(4, 16, 2, 64, cache_dtype)
+    k, v, q = (randn(g, 3, 2, 64, dtype=BF16) for _ in range(3))
+    at.kv_cache_write(c, k, v, torch.arange(3, device="cuda"))
+    table = torch.arange(3, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    lengths = torch.tensor([3, 0, 1], dtype=torch.int32, device="cuda")
+    return at, c, k, v, q, table, lengths
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+def test_autograd_sees_what_a_cache_write_changes(cache):
+    """A product saves the cache's values (or factors) for its backward pass; after a write that pass is refused."""
+    at, c, k, v, *_ = small_call(cache)
+    for i, kept in enumerate((c.k, c.v) if cache == BF16 else (c.k_scale, c.v_scale)):
+        x = torch.ones(kept.shape, device="cuda", dtype=kept.dtype, requires_grad=True)
+        product = (x * kept).sum()
+        at.kv_cache_write(c, k, v, torch.arange(3, device="cuda"))
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            product.backward()
+        product = (x * kept).sum()
+        at.kv_cache_read(c, torch.arange(3, device="cuda"))      # reads change nothing
+        product.backward()
+        assert torch.equal(x.grad, kept)
+
+
+def test_autograd_sees_given_results():
+    at, c, _, _, q, table, lengths = small_call()
+    out, lse = torch.ones(3, 2, 64, dtype=BF16, device="cuda"), torch.ones(3, 2, device="cuda")
+    for kept, call in ((out, lambda: at.paged_attention(q, c, table, lengths, out=out)),
+                       (lse, lambda: at.paged_attention(q, c, table, lengths, lse=lse)),
+                       (out, lambda: at.attention_join(q[None], torch.zeros(1, 3, 2, device="cuda"), out=out))):
+        x = torch.ones_like(kept, requires_grad=True)
+        product = (x * kept).sum()
+        call()
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            product.backward()
+
+
+def test_tensors_made_in_inference_mode_are_written_inside_and_outside_of_it():
+    """They have no version to advance."""
+    with torch.inference_mode():
+        at, c, k, v, q, table, lengths = small_call()
+        out, lse = torch.zeros(3, 2, 64, dtype=BF16, device="cuda"), torch.zeros(3, 2, device="cuda")
+        want = at.paged_attention(q, c, table, lengths)
+        at.paged_attention(q, c, table, lengths, out=out, lse=lse)
+        assert torch.equal(out, want)
+    at.kv_cache_write(c, k, v, torch.arange(3, device="cuda"))
+    at.paged_attention(q, c, table, lengths, out=out, lse=lse)
+    joined, _ = at.attention_join(out[None], lse[None], out=torch.empty_like(out))
+    assert torch.equal(out, want) and torch.equal(joined, want)
