@@ -370,12 +370,19 @@ void py_kv_cache_write(const Cache &c, const Tensor &k, const Tensor &v, const T
   const int wide = index(slots, "slots", k.size(0));
   no_grad("kv_cache_write", {&k, &v});
   no_tangent("kv_cache_write", {&k, &v});
-  on_one_device("kv_cache_write", {&k, &v, &slots, &c.k});
-  for (const Tensor *t : {&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)}) {
-    if (t != nullptr && (overlap(*t, k) || overlap(*t, v))) {
-      bad_value("kv_cache_write: k or v shares memory with the cache");
+  const std::initializer_list<const Tensor *> parts = {&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)};
+  for (const Tensor *t : parts) {
+    if (t == nullptr) continue;
+    if (overlap(*t, k) || overlap(*t, v) || overlap(*t, slots)) {
+      bad_value("kv_cache_write: k, v or slots shares memory with the cache");
+    }
+    for (const Tensor *other : parts) {
+      if (other != nullptr && other != t && overlap(*t, *other)) {
+        bad_value("kv_cache_write: the cache's tensors share memory with one another");
+      }
     }
   }
+  on_one_device("kv_cache_write", {&k, &v, &slots, &c.k});
   const Here here(k);
   check(kv_cache_write(a, data(k), data(v), sk.token, sk.head, sv.token, sv.head, data(slots), wide,
                        static_cast<int>(k.size(0)), code(k.scalar_type()), here.stream), "kv_cache_write");

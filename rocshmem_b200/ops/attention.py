@@ -180,7 +180,8 @@ def token_slots(block_table: torch.Tensor, sequences: torch.Tensor, positions: t
 def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, stream=None) -> None:
     """Writes ``k``, ``v [T, kv_heads, head_dim]`` (bf16, fp16 or fp32; rows may be strided as in :func:`qk_norm_rope`)
     into the slots ``[T]`` (int32 or int64). Slots outside the cache, negative ones among them, are skipped: padding.
-    The others have to differ from one another.
+    The others have to differ from one another. Neither the inputs nor the cache's own tensors may share memory with
+    another tensor of the cache (a cache whose keys are its values can be read, but not written).
 
     A 16-bit cache takes the values rounded to its type. In an e4m3 cache a row with the largest magnitude ``m`` becomes
     codes ``x * 448 / m`` with the factor ``m / 448``; a row that holds a NaN or an infinity reads back as NaN."""

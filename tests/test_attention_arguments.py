@@ -148,3 +148,28 @@ def test_given_results_that_require_a_gradient_are_refused(call):
         call()
     with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
         call()
+
+
+# ---- shared memory --------------------------------------------------------------------------------------------------
+
+def test_writes_into_tensors_that_share_memory_are_refused():
+    """Keys and values of one call would be written to the same rows by different threads, in no order."""
+    one = zeros(5, 2, 16, 64)
+    codes, factors = zeros(4, 2, 16, 64, dtype=E4M3), [torch.ones(4, 2, 16) for _ in range(2)]
+    shared = [at.KvCache(one[:4], one[:4]), at.KvCache(one[:4], one[1:]),
+              at.KvCache(codes, codes, *factors),
+              at.KvCache(codes, codes.clone(), factors[0], factors[0]),
+              at.KvCache(codes, codes.clone(), codes.view(F32).view(-1)[:128].view(4, 2, 16), factors[0])]
+    for c in shared:
+        with pytest.raises(ValueError, match="share memory with one another"):
+            write(c)
+        with pytest.raises(ValueError, match="CUDA device"):       # read they may be
+            at.kv_cache_read(c, torch.arange(3))
+    c = cache()
+    rows = c.k.view(-1)[:3 * 2 * 64].view(3, 2, 64)
+    for over in (dict(k=rows), dict(v=rows), dict(slots=c.v.view(torch.int64).view(-1)[:3])):
+        with pytest.raises(ValueError, match="shares memory with the cache"):
+            write(c, **over)
+    apart = at.KvCache(one[:2], one[2:4])
+    with pytest.raises(ValueError, match="CUDA device"):
+        write(apart)
