@@ -407,6 +407,8 @@ std::pair<Tensor, Tensor> py_kv_cache_read(const Cache &c, const Tensor &slots, 
 
 // ---- attention over the cache -------------------------------------------------------------------------------------
 
+constexpr double kSmallest = 1e-30;
+
 struct Paged {
   KvCacheArgs cache;
   PagedAttentionArgs args;
@@ -441,6 +443,11 @@ Paged check_paged(const Tensor &q, const Cache &c, const Tensor &block_table, co
   const double f = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(D));
   if (!(f > 0 && f < 1e30) || !(softcap >= 0 && softcap < 1e30) || window < 0) {
     bad_value("scale must be positive, softcap and window not negative");
+  }
+  // The kernels take both as fp32 and the cap's reciprocal: what would become zero there, no cap at all, or lose digits is
+  // refused.
+  if (f < kSmallest || (softcap > 0 && softcap < kSmallest)) {
+    bad_value("scale and softcap (unless it is 0) must be at least ", kSmallest, ", got ", f, " and ", softcap);
   }
   const int64_t most = block_table.size(1) * c.k.size(2);
   if (most > INT32_MAX - 256) {

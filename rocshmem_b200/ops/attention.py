@@ -213,6 +213,7 @@ def paged_attention(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor, 
     ``q`` is bf16 or fp16 and of the cache's type, or either for an e4m3 cache; ``D`` is 64, 96, 128 or 256; ``H`` a
     multiple of the cache's heads, whose groups share a key head. Scores are ``scale * q.k`` (default ``D ** -0.5``),
     with ``softcap`` > 0 ``softcap * tanh(scale * q.k / softcap)``; ``window`` > 0 leaves the last ``window`` tokens.
+    ``scale`` and ``softcap`` lie between 1e-30 and 1e30.
     Sums and softmax are fp32. ``out`` may be given, in q's type or fp32, and ``lse [B, H]`` fp32, the natural logarithm
     of the sum of the scores' exponentials; neither may share memory with an input. ``block_table [B, pages]`` and
     ``lengths [B]`` are int32 on the device.

@@ -173,3 +173,16 @@ def test_writes_into_tensors_that_share_memory_are_refused():
     apart = at.KvCache(one[:2], one[2:4])
     with pytest.raises(ValueError, match="CUDA device"):
         write(apart)
+
+
+# ---- numbers that are another number in the kernels' type -----------------------------------------------------------
+
+@pytest.mark.parametrize("over", [dict(softcap=1e-50), dict(softcap=1e-40), dict(softcap=1e-31), dict(scale=1e-50),
+                                  dict(scale=1e-40), dict(softcap=1e31), dict(scale=float("inf"))])
+def test_scales_and_caps_out_of_range_are_refused(over):
+    """A cap that becomes zero in 32 bits was no cap."""
+    with pytest.raises(ValueError, match="scale"):
+        attend(**over)
+    for fine in (dict(softcap=1e-30), dict(scale=1e-30), dict(softcap=0.0), dict(softcap=9e29), dict(scale=9e29)):
+        with pytest.raises(ValueError, match="CUDA device"):
+            attend(**fine)
