@@ -201,6 +201,11 @@ NormRopeArgs norm_rope_args(const Tensor &q, const Tensor &k, const Tensor &q_we
   if (R % 16 || R < 16 || R > D || table.size(0) < 1 || table.size(0) > INT32_MAX) {
     bad_value("the table's rows must have a multiple of 16 elements up to ", D, ", got ", table.sizes());
   }
+  // In the kernels' type: an eps that becomes zero there makes rows of zeros NaN.
+  const float eps32 = static_cast<float>(eps);
+  if (!(eps >= 0 && std::isfinite(eps32) && (eps32 > 0 || eps == 0))) {
+    bad_value("eps must not be negative, and a finite fp32 number that is not zero unless it is 0 itself, got ", eps);
+  }
   const int wide = index(positions, "positions", T);
   if (at::GradMode::is_enabled() && table.requires_grad()) {
     bad_value("qk_norm_rope has no gradient for its table: detach it");
@@ -224,7 +229,7 @@ NormRopeArgs norm_rope_args(const Tensor &q, const Tensor &k, const Tensor &q_we
   a.dim = static_cast<int>(D);
   a.rotary = static_cast<int>(R);
   a.table_rows = static_cast<int>(table.size(0));
-  a.eps = static_cast<float>(eps);
+  a.eps = eps32;
   a.interleaved = interleaved;
   a.type = code(q.scalar_type());
   a.weight_type = code(q_weight.scalar_type());

@@ -186,3 +186,13 @@ def test_scales_and_caps_out_of_range_are_refused(over):
     for fine in (dict(softcap=1e-30), dict(scale=1e-30), dict(softcap=0.0), dict(softcap=9e29), dict(scale=9e29)):
         with pytest.raises(ValueError, match="CUDA device"):
             attend(**fine)
+
+
+@pytest.mark.parametrize("eps", [-1e-6, float("nan"), float("inf"), -float("inf"), 1e39, 1e-50, 5e-324])
+def test_eps_out_of_range_is_refused(eps):
+    """One below zero or NaN gives NaN; one that becomes zero in 32 bits makes rows of zeros NaN, which have a norm."""
+    with pytest.raises(ValueError, match="eps"):
+        norm_rope(eps=eps)
+    for fine in (0.0, 0, 1e-45, 1e-6, 1e-3, 3e38):
+        with pytest.raises(ValueError, match="CUDA device"):
+            norm_rope(eps=fine)
