@@ -5,7 +5,7 @@ Four artefacts, all inside the package directory so that they travel with a sour
 * ``lib/librocshmem_b200.so`` - host runtime (C++) plus every CUDA kernel of the library;
 * ``_C.<abi>.so``             - pybind11 bindings, linked against the library;
 * ``_A.<abi>.so``             - bindings of the attention operators, which take torch tensors (the only part that is
-                                compiled against torch's headers);
+                                compiled against torch's headers, and which fits no other version of torch);
 * ``_testk.<abi>.so``         - kernels of the functional test-suite that exercise the device API
                                 from user code, linked against the same library (built on demand).
 
@@ -16,6 +16,7 @@ GPU. Run ``python -m rocshmem_b200._build`` or call :func:`build`.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -62,6 +63,22 @@ def _pybind_include() -> str:
 def _torch_dir() -> Path:
     from importlib.util import find_spec
     return Path(find_spec("torch").origin).resolve().parent
+
+
+def _torch_version() -> str:
+    """The installed torch's version, without importing it (a build does not need torch to load)."""
+    found = re.search(r"^__version__\s*=\s*['\"]([^'\"]+)['\"]", (_torch_dir() / "version.py").read_text(), re.M)
+    if not found:
+        raise RuntimeError("no version in torch/version.py")
+    return found.group(1)
+
+
+def attention_torch() -> str | None:
+    """The version of torch that the built ``_A`` was compiled against (a text inside it), ``None`` without a build.
+    Read from the file: loading an extension into another torch than its own is what must not happen."""
+    ext = PKG / f"_A{EXT}"
+    found = re.search(rb"rocshmem_b200\._A for torch ([0-9A-Za-z.+_-]+)", ext.read_bytes()) if ext.exists() else None
+    return found.group(1).decode() if found else None
 
 
 def _rel(p: Path) -> str:
@@ -127,7 +144,10 @@ def _ninja_text(with_tests: bool) -> str:
     for src in TORCH_CPP:
         obj = _rel(OBJ / (src.replace("/", "_") + ".o"))
         lines.append(f"build {obj}: cxx {_rel(CSRC / src)}")
-        lines.append(f"  extra = $pyflags -isystem {torch_dir}/include -isystem {torch_dir}/include/torch/csrc/api/include")
+        # -MMD leaves system headers out of the dependencies: the version in the command is what rebuilds the object
+        # after a change of torch.
+        lines.append(f"  extra = $pyflags -isystem {torch_dir}/include -isystem {torch_dir}/include/torch/csrc/api/include "
+                     f"-DROCSHMEM_TORCH_VERSION={_torch_version()}")
         torch_objs.append(obj)
     ext_a = _rel(PKG / f"_A{EXT}")
     lines.append(f"build {ext_a}: linkext {' '.join(torch_objs)} | {lib}")
@@ -170,8 +190,11 @@ def build(with_tests: bool = True, verbose: bool = False, jobs: int | None = Non
         print(proc.stdout)
 
 
-def is_built(with_tests: bool = False) -> bool:
-    ok = all(f.exists() for f in (LIBDIR / "librocshmem_b200.so", PKG / f"_C{EXT}", PKG / f"_A{EXT}"))
+def is_built(with_tests: bool = False, with_attention: bool = True) -> bool:
+    """Whether the artefacts are there; the attention operators' bindings, for the installed torch."""
+    ok = all(f.exists() for f in (LIBDIR / "librocshmem_b200.so", PKG / f"_C{EXT}"))
+    if with_attention:
+        ok = ok and attention_torch() == _torch_version()
     if with_tests:
         ok = ok and (PKG / f"_testk{EXT}").exists()
     return ok

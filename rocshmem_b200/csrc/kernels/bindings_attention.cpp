@@ -551,8 +551,14 @@ std::pair<Tensor, Tensor> py_attention_join(const Tensor &outs, const Tensor &ls
 
 }  // namespace
 
+#define ROCSHMEM_TEXT_OF(x) #x
+#define ROCSHMEM_TEXT(x) ROCSHMEM_TEXT_OF(x)
+// The version that these objects fit. Read from the file before it is loaded.
+const char kBuiltFor[] = "rocshmem_b200._A for torch " ROCSHMEM_TEXT(ROCSHMEM_TORCH_VERSION);
+
 PYBIND11_MODULE(_A, m) {
   m.doc() = "Attention operators on torch tensors";
+  m.attr("built_for") = kBuiltFor;
   py::class_<Cache>(m, "Cache").def(py::init([](const Tensor &k, const Tensor &v, const OptTensor &ks,
       const OptTensor &vs) {
     Cache c{k, v, ks, vs};
