@@ -62,7 +62,11 @@ def _pybind_include() -> str:
 
 def _torch_dir() -> Path:
     from importlib.util import find_spec
-    return Path(find_spec("torch").origin).resolve().parent
+    found = find_spec("torch")
+    if found is None or found.origin is None:
+        raise RuntimeError("torch not found: the attention operators are compiled against the torch that they will run "
+                           "with; build where it is installed (pip install --no-build-isolation)")
+    return Path(found.origin).resolve().parent
 
 
 def _torch_version() -> str:
@@ -151,7 +155,8 @@ def _ninja_text(with_tests: bool) -> str:
         torch_objs.append(obj)
     ext_a = _rel(PKG / f"_A{EXT}")
     lines.append(f"build {ext_a}: linkext {' '.join(torch_objs)} | {lib}")
-    lines.append(f"  libs = -L{torch_dir}/lib -lc10 -lc10_cuda -ltorch_cpu -ltorch_python -Xlinker -rpath -Xlinker {torch_dir}/lib")
+    # No run path to torch's libraries: torch is imported before the extension, which finds them loaded.
+    lines.append(f"  libs = -L{torch_dir}/lib -lc10 -lc10_cuda -ltorch_cpu -ltorch_python")
     targets = [ext, ext_a]
     tests_src = PKG.parent / "tests" / "csrc" / "test_kernels.cu"
     if with_tests and tests_src.exists():

@@ -56,3 +56,21 @@ print("refused")
     env = dict(os.environ, ROCSHMEM_B200_NO_AUTOBUILD="1", PYTHONPATH=ROOT)
     out = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and out.stdout.strip() == "refused", out.stderr
+
+
+def test_an_isolated_build_is_refused(monkeypatch):
+    """It would compile against a torch of its own, in a folder that is deleted afterwards."""
+    import importlib.util
+    import tomllib
+    with open(os.path.join(ROOT, "pyproject.toml"), "rb") as f:
+        assert not any(r.startswith("torch") for r in tomllib.load(f)["build-system"]["requires"])
+    find = importlib.util.find_spec
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: None if name == "torch" else find(name, *a))
+    with pytest.raises(RuntimeError, match="no-build-isolation"):
+        _build._ninja_text(with_tests=False)
+
+
+def test_the_extension_has_no_run_path_to_a_torch():
+    text = _build._ninja_text(with_tests=False)
+    libs = [line for line in text.splitlines() if line.lstrip().startswith("libs =")]
+    assert len(libs) == 1 and "rpath" not in libs[0]
