@@ -165,15 +165,15 @@ class KvCache:
 
 
 def token_slots(block_table: torch.Tensor, sequences: torch.Tensor, positions: torch.Tensor,
-    page_size: int) -> torch.Tensor:
+                page_size: int) -> torch.Tensor:
     """Slots (int64) of tokens: token ``i`` is position ``positions[i]`` of sequence ``sequences[i]``, whose pages are
-    row ``sequences[i]`` of ``block_table``. -1 for a negative position, one past the table or one without a page. Plain
-    PyTorch, any device, no synchronisation."""
-    at = positions.long()
-    known = (at >= 0) & (at < block_table.shape[1] * page_size)
-    if block_table.shape[1] == 0:
+    row ``sequences[i]`` of ``block_table``. -1 for a sequence that the table does not have, a negative position, one
+    past the table or one without a page. Plain PyTorch, any device, no synchronisation."""
+    at, row = positions.long(), sequences.long()
+    known = (at >= 0) & (at < block_table.shape[1] * page_size) & (row >= 0) & (row < block_table.shape[0])
+    if block_table.numel() == 0:
         return torch.full_like(at, -1)
-    page = block_table[sequences.long(), torch.where(known, at, 0) // page_size].long()
+    page = block_table[torch.where(known, row, 0), torch.where(known, at, 0) // page_size].long()
     return torch.where(known & (page >= 0), page * page_size + at % page_size, -1)
 
 

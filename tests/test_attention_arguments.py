@@ -196,3 +196,18 @@ def test_eps_out_of_range_is_refused(eps):
     for fine in (0.0, 0, 1e-45, 1e-6, 1e-3, 3e38):
         with pytest.raises(ValueError, match="CUDA device"):
             norm_rope(eps=fine)
+
+
+# ---- slots ----------------------------------------------------------------------------------------------------------
+
+def test_slots_of_sequences_that_the_table_does_not_have():
+    """A negative sequence (padding of a batch) is not the last one counted from the end, whose tokens a write would
+    replace, and one past the table is no index out of range, which on a GPU ends the process."""
+    table = torch.tensor([[4, 2, -1], [0, 7, 1]], dtype=torch.int32)
+    seq = torch.tensor([-1, -2, 2, 2 ** 31 - 1, 0, 1, -2 ** 31])
+    pos = torch.tensor([0, 17, 0, 5, 17, 33, 0])
+    for s, p in ((seq, pos), (seq.int(), pos.int())):
+        got = at.token_slots(table, s, p, 16)
+        assert got.dtype == torch.int64 and got.tolist() == [-1, -1, -1, -1, 33, 17, -1]
+    assert at.token_slots(table[:0], seq, pos, 16).tolist() == [-1] * 7
+    assert at.token_slots(table, seq[:0], pos[:0], 16).tolist() == []
