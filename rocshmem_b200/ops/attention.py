@@ -65,9 +65,12 @@ def rope_table(num_positions: int, rotary_dim: int, base: float = 10000.0, devic
                frequencies: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The table ``[num_positions, rotary_dim]`` fp32 that :func:`qk_norm_rope` reads: row ``p`` holds the cosines and
     then the sines of ``p * frequency_i``, ``i < rotary_dim / 2``. ``frequencies`` (scaled ones, for instance) default
-    to ``base ** (-2 i / rotary_dim)``. Angles are computed in 64 bits: those of far positions keep no digits in 32."""
+    to ``base ** (-2 i / rotary_dim)``. Angles are computed in 64 bits: those of far positions keep no digits in 32. The
+    table lies on ``device``, by default where the frequencies do."""
     if rotary_dim % 2 or rotary_dim < 2 or num_positions < 1:
         raise ValueError("rope_table: rotary_dim must be even, num_positions positive")
+    if frequencies is not None and device is None:
+        device = frequencies.device
     if frequencies is None:
         frequencies = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
     if tuple(frequencies.shape) != (rotary_dim // 2,):

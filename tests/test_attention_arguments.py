@@ -211,3 +211,14 @@ def test_slots_of_sequences_that_the_table_does_not_have():
         assert got.dtype == torch.int64 and got.tolist() == [-1, -1, -1, -1, 33, 17, -1]
     assert at.token_slots(table[:0], seq, pos, 16).tolist() == [-1] * 7
     assert at.token_slots(table, seq[:0], pos[:0], 16).tolist() == []
+
+
+# ---- the table of angles --------------------------------------------------------------------------------------------
+
+def test_a_table_lies_where_its_frequencies_do():
+    """Without a device of its own (here one without memory stands for the GPU)."""
+    f = torch.full((16,), 0.5)
+    assert at.rope_table(8, 32, frequencies=f.to("meta")).device.type == "meta"
+    assert at.rope_table(8, 32, frequencies=f).device.type == "cpu"
+    assert at.rope_table(8, 32, frequencies=f, device="meta").device.type == "meta"
+    assert at.rope_table(8, 32).device.type == "cpu" and at.rope_table(8, 32, device="meta").device.type == "meta"
