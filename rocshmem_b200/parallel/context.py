@@ -65,8 +65,9 @@ class ContextParallelDecode:
         """``q [B, heads, head_dim]``, the same on every member; ``cache``, ``block_table [B, pages]`` and ``lengths
         [B]`` describe this member's part and may be empty (a length of zero). Returns the attention over all members'
         tokens ``[B, heads, head_dim]`` in q's type, the same bits on every member. Arguments as in
-        :func:`rocshmem_b200.ops.attention.paged_attention`; sliding windows, which go by positions in the whole
-        sequence, are the caller's to express through the parts' block tables and lengths."""
+        :func:`rocshmem_b200.ops.attention.paged_attention`. There is no sliding window: a member does not know which
+        positions of the whole sequence its tokens have, and a block table can leave out whole pages only, while a
+        window's edge mostly lies inside one."""
         if q.dim() != 3 or q.shape[1:] != (self.heads, self.head_dim) or q.shape[0] > self.max_batch:
             raise ValueError(f"q must be [batch <= {self.max_batch}, {self.heads}, {self.head_dim}], got {tuple(q.shape)}")
         if q.shape[0] == 0:
