@@ -221,6 +221,14 @@ def paged_attention(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor, 
     of the sum of the scores' exponentials; neither may share memory with an input. ``block_table [B, pages]`` and
     ``lengths [B]`` are int32 on the device.
 
+    The kernel is chosen by the block table's width (or the window), the most that the lengths on the device can be: a
+    batch of short sequences, and a captured graph of one, is faster with the table cut to the pages that it can need
+    (``block_table[:, :n]``): 4 sequences of up to 300 tokens 8.3 us on the device, with a table 16 or 256 times as wide
+    10.3; 16 of up to 64 tokens 6.3 and 10.0.
+
+    Sums are fp32 and hold up to 2^14 times a value: results are finite as long as the magnitudes of a sequence's values
+    add up to less than 1e34.
+
     Lengths are taken between 0 and the table's end. Tokens in a page that is no page of the cache are not seen. A
     sequence that sees nothing has zeros and an lse of -inf. Rows that are not seen may hold anything, NaN included; an
     infinity or NaN in a row that is seen makes the results of its heads NaN, except a score of -inf, which counts for
