@@ -107,8 +107,10 @@ struct Side {
 };
 
 // 16384 tokens x (32 + 8) heads of 128, bf16: 61.5 us for 344 MB (5.6 TB/s; a device copy: 6.4), with two thirds of the
-// issue slots and half of the integer pipe busy. Four rows in flight and five blocks an SM: with three blocks 71 us,
-// with six, which spill, 90; two rows 73, eight 65. One rounding: that of the result.
+// issue slots and half of the integer pipe busy; fp32, 8192 tokens: 57 us for 340 MB (5.9). Four rows in flight and five
+// blocks an SM, for which the 16-bit form with pairs of halves spills 16 - 20 bytes a thread; without spills, with four
+// blocks, it takes 70 us, with three 69, with six, which spill more, 90; two rows 73, eight 65. One rounding: that of
+// the result.
 template <typename T, typename W, int LANES, int ROWS, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5) norm_rope_kernel(NormRope<T, W> a,
     unsigned q_items, unsigned items,
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5) norm_rope_ke
 // adds those up in a fixed order, and norm_rope_weights_kernel adds the blocks' sums, so that the gradients are the
 // same in every run.
 //
-// The case above: 101 us for 512 MB (5.1 TB/s), both kernels. 61 % of the issue slots; what is left is the latency of
+// The case above: 101 us for 512 MB (5.1 TB/s), both kernels, without the host. 61 % of the issue slots; what is left is the latency of
 // an item's position, then its angles. Two rows in flight and three blocks an SM: four rows 113, four blocks (spilling)
 // 114, one row in four blocks 138; positions looked up an item ahead 115; items of eight heads 104; more blocks than
 // fit at once 106 - 121.

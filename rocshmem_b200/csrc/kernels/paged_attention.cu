@@ -24,10 +24,14 @@
 // e4m3 caches: codes become fp16 exactly (cvt), a key's factor multiplies its score, a value's factor its probability.
 // They are bound by instructions as much as by memory: 32 keys a step need 650 (two steps of 16 keys took 15 % longer).
 //
-// Measured on one B200, 128 elements a head: 64 sequences of 1024 - 4096 tokens, 32 / 8 heads, bf16, 116 us for 676 MB
-// (5.8 TB/s; a device copy: 6.4); two sequences of 130 - 520 thousand, 64 / 8 heads, e4m3, 307 us for 1.94 GB (6.3).
-// Without the join, 111 and 302. What is left in the first is the start, 4 us until data arrives, and the SMs that end
-// last (see Shape).
+// Measured on one B200, 128 elements a head, launches one after the other without the host: 64 sequences of 1024 - 4096
+// tokens, 32 / 8 heads, bf16, 117 us for 675 MB (5.8 TB/s; a device copy: 6.4); two sequences of 130 - 520 thousand,
+// 64 / 8 heads, e4m3, 312 us for 1.94 GB (6.2). Public calls in a loop: 118 us for 670 MB (5.7) and 328 us for 2.03 GB
+// (6.2). The join takes 5 us of it. What is left in the first is the start, 4 us until data arrives, and the SMs that
+// end last (see Shape). Farther from memory: 16 heads a key head in e4m3 (54 us for a floor of 27: the softmax's
+// arithmetic at two warps a scheduler) and in bf16 with 64 elements (42 for 26), one sequence of 32768 tokens (35 for
+// 21: start, join), 256 sequences of 512 tokens (72 for 54, e4m3 51 for 28: each pair begins with a wait for its
+// queries).
 #include "attention_common.cuh"
 
 #include <atomic>
@@ -361,8 +365,9 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
         }
         q_scale[j][0] = q_scale[j][1] = 1.f;
       } else {
-        // A head's largest magnitude brought to [1, 2) by a power of two: bf16 values then fit fp16 exactly, down to
-        // 2^-24 of the largest.
+        // A head's largest magnitude brought to [1, 2) by a power of two. bf16 values (8 bits) then fit fp16 exactly
+        // down to 2^-17, fp16 values (11 bits) down to 2^-14; what is smaller is rounded to steps of 2^-24, off by 2^-25
+        // at most, half of what fp32 would round off the largest element's product.
         uint4 raw[D / 32];
         uint32_t top = 0;
 #pragma unroll
@@ -528,7 +533,9 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
         }
         if constexpr (MODE == MODE_E4M3) v_unit = 1.f / cv;
         // P^T, as a value rounded to the operand's type and the rounded rest: of one part alone the rounding of
-        // bf16 (2^-8) or fp16 (2^-11) would be as large as that of the result.
+        // bf16 (2^-8) or fp16 (2^-11) would be as large as that of the result. Two are off by 2^-17 and 2^-23. The second
+        // costs nothing where memory bounds (one part, 64 sequences of 1024 - 4096 tokens: 117 us both), 8 % with 16
+        // heads a key head in e4m3 (54.0 against 49.7).
         uint32_t pf[MT][NT][2], pr[MT][NT][2];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
@@ -861,8 +868,14 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const Params p) {
 // ---- host side ----------------------------------------------------------------------------------------------------
 
 // Keys a warp of paged_short_kernel, at most: with more, splitting over more SMs pays for a second launch. 128
-// elements, bf16, 32 pairs, one launch against two: 128 keys 6.2 us against 9.9, 512 keys 10.3 and 10.3, 1024 keys 14.4
+// elements, bf16, 32 pairs, one launch against two: 128 keys 6.2 us against 9.8, 512 keys 10.3 and 10.3, 1024 keys 14.4
 // and 11.1.
+//
+// Over a grid of 1 - 32 sequences of 16 - 2048 keys, 64, 128 and 256 elements, bf16 and e4m3, 4 and 16 heads a key head,
+// the rule takes the faster form, or one within 8 % of it, in 308 of 336 cases. It is off most for more pairs than SMs
+// of 64 elements, of which an SM holds several blocks (256 pairs of 128 keys: two launches 9.8 us, one would take 6.2),
+// and at its upper end for few pairs that two launches would split further (4 pairs of 512 keys with 16 heads: one
+// launch 12.3 us, two 8.8; 8 pairs with 4 heads 10.3 and 8.2; 256 elements in e4m3 14.9 and 11.1).
 constexpr int kShortKeys = 64;
 // Keys that a share has at least: below that its fixed costs weigh more than the loads that another warp would take
 // over.
@@ -894,7 +907,7 @@ int pairs_of(const Params &p) { return p.batch * p.kv_heads * p.chunks; }
 int longest_of(const Params &p) { return p.window > 0 ? std::min(p.window, p.capacity) : p.capacity; }
 
 // A block for each pair, no more than SMs. From half the SMs on there is less to split: twice the keys (128 pairs of
-// 1024 keys: 14.4 us against 18.0; of 2048: 24.7 and 26.8).
+// 1024 keys: 14.4 us against 18.2; of 2048, which take two launches: 24.7 and 26.9).
 template <typename S>
 bool is_short(const Params &p) {
   const int pairs = pairs_of(p), sms = device_sm_count();
@@ -936,9 +949,10 @@ int launch(Params p, cudaStream_t s) {
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   if (longest_of(p) <= S::kKeys) return 0;  // no pair has two tiles: nothing to join
-  // Many parts of each of a few pairs are shared by eight sets of threads (8 pairs of 148 parts: 35 us the whole call,
-  // with one set 62); few parts of many pairs are not worth the exchange (128 pairs of 9 parts: 73 us with one set, 76
-  // with eight).
+  // Many parts of each of a few pairs are shared by eight sets of threads (8 pairs of 32768 keys, 148 parts: 35 us the
+  // whole call, with one set 56); few parts of many pairs are not worth the exchange (512 pairs of 2048 keys: 68 us with
+  // one set, 76 with eight). The two are level at 128 pairs for 128 elements (2048 keys: 26.8 and 26.5), so that between
+  // 50 and 128 pairs, which have one set, eight would be up to a quarter faster (64 pairs of 2048 keys: 20.4 and 16.4).
   const int shares = p.blocks;
   return pairs > shares / 24 ? launch_join<D, NT, MODE, 1>(p, s) : launch_join<D, NT, MODE, 8>(p, s);
 }
