@@ -34,12 +34,15 @@ from rocshmem_b200.ops import collectives as coll  # noqa: E402
 from rocshmem_b200.ops import attention, gemm, moe  # noqa: E402
 
 
-def timed(fn, reps, flush):
+def timed(fn, reps, flush, fills=1):
+    """Microseconds of a call. The GPU is filling ``flush`` while the host issues the call; ``fills`` more than one for
+    calls whose host time is longer than one fill and would be measured otherwise."""
     fn()
     torch.cuda.synchronize()
     total = 0.0
     for _ in range(reps):
-        flush.fill_(1)
+        for _ in range(fills):
+            flush.fill_(1)
         a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         a.record()
         fn()
@@ -170,7 +173,7 @@ def tour_attention(reps, flush, rows):
     leaves = [t.clone().requires_grad_() for t in (q, k, wq, wk)]
     out = attention.qk_norm_rope(*leaves, pos, table)
     gq, gk = randn(T, H, D), randn(T, K, D)
-    add("norm and rotation, backward", timed(lambda: torch.autograd.grad(out, leaves, (gq, gk), retain_graph=True), reps, flush), 3 * n)
+    add("norm and rotation, backward", timed(lambda: torch.autograd.grad(out, leaves, (gq, gk), retain_graph=True), reps, flush, fills=8), 3 * n)
     slots = torch.randperm(T, generator=g, device="cuda")
     for dtype, label, width in ((torch.bfloat16, "bf16", 2 * D), (torch.float8_e4m3fn, "e4m3", D + 4)):
         pages = 64 * 128
