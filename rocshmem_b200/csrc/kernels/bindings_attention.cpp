@@ -145,18 +145,21 @@ void written(std::initializer_list<const Tensor *> tensors) {
   }
 }
 
-// Whether the address ranges of two tensors meet.
-bool overlap(const Tensor &a, const Tensor &b) {
-  if (a.numel() == 0 || b.numel() == 0) return false;
-  auto span = [](const Tensor &t) {
+// The addresses of a tensor's elements, first to last; nothing for one without elements.
+struct Range {
+  uintptr_t first = 0, end = 0;
+  Range() = default;
+  explicit Range(const Tensor &t) {
+    if (t.numel() == 0) return;
     int64_t last = 0;
-    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-    const uintptr_t p = reinterpret_cast<uintptr_t>(t.const_data_ptr());
-    return std::make_pair(p, p + static_cast<uintptr_t>(last + 1) * t.element_size());
-  };
-  const auto x = span(a), y = span(b);
-  return x.first < y.second && y.first < x.second;
-}
+    const auto sizes = t.sizes(), strides = t.strides();
+    for (size_t i = 0; i < sizes.size(); ++i) last += (sizes[i] - 1) * strides[i];
+    first = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+    end = first + static_cast<uintptr_t>(last + 1) * t.element_size();
+  }
+  bool meets(const Range &o) const { return first < o.end && o.first < end; }
+};
+bool overlap(const Tensor &a, const Tensor &b) { return Range(a).meets(Range(b)); }
 
 void result(const Tensor &t, const char *name, at::IntArrayRef shape, std::initializer_list<at::ScalarType> types,
             std::initializer_list<const Tensor *> inputs) {
@@ -375,17 +378,19 @@ void py_kv_cache_write(const Cache &c, const Tensor &k, const Tensor &v, const T
   const int wide = index(slots, "slots", k.size(0));
   no_grad("kv_cache_write", {&k, &v});
   no_tangent("kv_cache_write", {&k, &v});
-  const std::initializer_list<const Tensor *> parts = {&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)};
-  for (const Tensor *t : parts) {
+  const Range in[3] = {Range(k), Range(v), Range(slots)};
+  Range parts[4];
+  int n = 0;
+  for (const Tensor *t : {&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)}) {
     if (t == nullptr) continue;
-    if (overlap(*t, k) || overlap(*t, v) || overlap(*t, slots)) {
-      bad_value("kv_cache_write: k, v or slots shares memory with the cache");
+    const Range r(*t);
+    for (const Range &x : in) {
+      if (r.meets(x)) bad_value("kv_cache_write: k, v or slots shares memory with the cache");
     }
-    for (const Tensor *other : parts) {
-      if (other != nullptr && other != t && overlap(*t, *other)) {
-        bad_value("kv_cache_write: the cache's tensors share memory with one another");
-      }
+    for (int i = 0; i < n; ++i) {
+      if (r.meets(parts[i])) bad_value("kv_cache_write: the cache's tensors share memory with one another");
     }
+    parts[n++] = r;
   }
   on_one_device("kv_cache_write", {&k, &v, &slots, &c.k});
   const Here here(k);
