@@ -92,8 +92,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     whose rows become zeros and have no gradient; one past the table makes its token's rows NaN.
 
     Differentiable once (``create_graph`` and forward-mode derivatives are refused) with respect to ``q``, ``k`` and
-    both weights; the weights' gradients are the same in every run. A ``table`` that requires a gradient is refused. A backward pass can be captured into a CUDA graph with its forward pass; while
-    an eager graph of the same leaves is alive, the captured forward pass is refused."""
+    both weights; the weights' gradients are the same in every run. A ``table`` that requires a gradient is refused. A
+    backward pass can be captured into a CUDA graph with its forward pass; while an eager graph of the same leaves is
+    alive, the captured forward pass is refused."""
     if stream is not None:
         with _On(stream, q, k, q_weight, k_weight, positions, table):
             return qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved)
@@ -173,11 +174,12 @@ def token_slots(block_table: torch.Tensor, sequences: torch.Tensor, positions: t
     row ``sequences[i]`` of ``block_table``. -1 for a sequence that the table does not have, a negative position, one
     past the table or one without a page. Plain PyTorch, any device, no synchronisation."""
     at, row = positions.long(), sequences.long()
-    known = (at >= 0) & (at < block_table.shape[1] * page_size) & (row >= 0) & (row < block_table.shape[0])
     if block_table.numel() == 0:
         return torch.full_like(at, -1)
-    page = block_table[torch.where(known, row, 0), torch.where(known, at, 0) // page_size].long()
-    return torch.where(known & (page >= 0), page * page_size + at % page_size, -1)
+    # Clamped, an index is one of the table's; where that changed it, there is no slot.
+    at_in, row_in = at.clamp(0, block_table.shape[1] * page_size - 1), row.clamp(0, block_table.shape[0] - 1)
+    page = block_table[row_in, at_in // page_size].long()
+    return torch.where((at == at_in) & (row == row_in) & (page >= 0), page * page_size + at % page_size, -1)
 
 
 def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, stream=None) -> None:
