@@ -107,14 +107,13 @@ struct Side {
 };
 
 // 16384 tokens x (32 + 8) heads of 128, bf16: 61.5 us for 344 MB (5.6 TB/s; a device copy: 6.4), with two thirds of the
-// issue slots and half of the integer pipe busy; fp32, 8192 tokens: 57 us for 340 MB (5.9). Four rows in flight and five
-// blocks an SM, for which the 16-bit form with pairs of halves spills 16 - 20 bytes a thread; without spills, with four
-// blocks, it takes 70 us, with three 69, with six, which spill more, 90; two rows 73, eight 65. One rounding: that of
-// the result.
+// issue slots and half of the integer pipe busy; fp32, 8192 tokens: 57 us for 340 MB (5.9). Four rows in flight and
+// five blocks an SM, for which the 16-bit form with pairs of halves spills 16 - 20 bytes a thread; without spills, with
+// four blocks, it takes 70 us, with three 69, with six, which spill more, 90; two rows 73, eight 65. One rounding: that
+// of the result.
 template <typename T, typename W, int LANES, int ROWS, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5) norm_rope_kernel(NormRope<T, W> a,
-    unsigned q_items, unsigned items,
-                                                                                       Divisor q_chunks, Divisor k_chunks, T *q_out, T *k_out) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5) norm_rope_kernel(NormRope<T, W> a, unsigned q_items,
+    unsigned items, Divisor q_chunks, Divisor k_chunks, T *q_out, T *k_out) {
   const int lane = threadIdx.x % LANES;
   const Place<INTERLEAVED> at(lane, a.dim, a.rotary);
   // All lanes of a warp take part in every shuffle: groups past the last item have no rows.
@@ -168,15 +167,13 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5) norm_rope_ke
 // adds those up in a fixed order, and norm_rope_weights_kernel adds the blocks' sums, so that the gradients are the
 // same in every run.
 //
-// The case above: 101 us for 512 MB (5.1 TB/s), both kernels, without the host. 61 % of the issue slots; what is left is the latency of
-// an item's position, then its angles. Two rows in flight and three blocks an SM: four rows 113, four blocks (spilling)
-// 114, one row in four blocks 138; positions looked up an item ahead 115; items of eight heads 104; more blocks than
-// fit at once 106 - 121.
+// The case above: 101 us for 512 MB (5.1 TB/s), both kernels, without the host. 61 % of the issue slots; what is left
+// is the latency of an item's position, then its angles. Two rows in flight and three blocks an SM: four rows 113, four
+// blocks (spilling) 114, one row in four blocks 138; positions looked up an item ahead 115; items of eight heads 104;
+// more blocks than fit at once 106 - 121.
 template <typename T, typename W, int LANES, int ROWS, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads, 3) norm_rope_backward_kernel(NormRope<T, W> a, unsigned q_items,
-    unsigned items,
-                                                                         int q_blocks, const T *gq, const T *gk, T *dq,
-                                                                         T *dk, float *partial) {
+    unsigned items, int q_blocks, const T *gq, const T *gk, T *dq, T *dk, float *partial) {
   extern __shared__ float sums[];  // [groups][dim]
   // The sum over the blocks may be set up from here on; it waits for the end of this grid before it reads.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -274,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 3) norm_rope_backward_kernel(NormRop
 // Adds the blocks' sums: a block has 32 columns of one weight, its warps take the rows in turn.
 template <typename W>
 __global__ void __launch_bounds__(1024) norm_rope_weights_kernel(const float *partial, int q_rows, int rows, int dim,
-                                                                 W *dq_weight, W *dk_weight) {
+    W *dq_weight, W *dk_weight) {
   __shared__ float s[32][33];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int col = blockIdx.x * 32 + threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -343,10 +340,9 @@ __device__ __forceinline__ void look_up_rows(const C &c, const Row &w, const voi
 // a lane looked up a token's row for the others and divisions became multiplications, 42 us); to bf16 43 us for 269 MB
 // (6.2 TB/s).
 template <typename T, typename C, int LANES, int ROWS>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 6) kv_write_kernel(Cache<C> c, const T *k,
-    const T *v, long long k_token,
-                                                            long long k_head, long long v_token, long long v_head,
-                                                            const void *slots, int wide_slots, int tokens) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 6) kv_write_kernel(Cache<C> c, const T *k, const T *v,
+    long long k_token, long long k_head, long long v_token, long long v_head, const void *slots, int wide_slots,
+    int tokens) {
   constexpr bool kQuantize = sizeof(C) == 1;
   const int lane = threadIdx.x % LANES;
   const bool in_row = 8 * lane < c.dim;
@@ -394,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 6) kv_write_ker
 // 16381 tokens x 8 heads of 128, e4m3 to bf16: 18.5 us for 102 MB; 65536 tokens: 66 us for 407 MB (6.2 TB/s).
 template <typename T, typename C, int LANES, int ROWS>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(Cache<C> c, T *k_out, T *v_out, const void *slots,
-                                                           int wide_slots, int tokens) {
+    int wide_slots, int tokens) {
   const int lane = threadIdx.x % LANES;
   const bool in_row = 8 * lane < c.dim;
   const Row w = row_of(blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES, ROWS, c.each);
@@ -438,8 +434,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(Cache<C> c, T *k_out,
 // the memory's latency; the first parts' loads are on their way while the maximum is found.
 template <typename T, typename O, int LANES>
 __global__ void __launch_bounds__(kThreads) join_kernel(const T *outs, const float *lses, long long out_part,
-                                                        long long lse_part, int parts, long long rows, int dim, O *out,
-                                                        float *lse) {
+    long long lse_part, int parts, long long rows, int dim, O *out, float *lse) {
   constexpr int kAhead = sizeof(T) == 4 ? 4 : 8;  // parts whose loads are in flight
   const int lane = threadIdx.x % LANES;
   const long long row = static_cast<long long>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
@@ -539,10 +534,8 @@ int backward_blocks() { return device_sm_count() * 3; }
 template <typename T, typename W>
 NormRope<T, W> norm_rope_args(const NormRopeArgs &a) {
   return NormRope<T, W>{static_cast<const T *>(a.q), static_cast<const T *>(a.k), a.q_token, a.q_head, a.k_token,
-      a.k_head,
-                        static_cast<const W *>(a.q_weight), static_cast<const W *>(a.k_weight), a.positions, a.table,
-                        a.tokens, a.q_heads, a.k_heads, a.dim, a.rotary, a.table_rows, a.eps, 1.f / static_cast<float>(a.dim),
-                        a.wide_positions};
+      a.k_head, static_cast<const W *>(a.q_weight), static_cast<const W *>(a.k_weight), a.positions, a.table, a.tokens,
+      a.q_heads, a.k_heads, a.dim, a.rotary, a.table_rows, a.eps, 1.f / static_cast<float>(a.dim), a.wide_positions};
 }
 
 // The weights have the rows' type or fp32.
@@ -564,9 +557,8 @@ template <typename F>
 int with_cache(const KvCacheArgs &c, F f) {
   auto args = [&](auto tag) {
     using C = typename decltype(tag)::type;
-    return Cache<C>{static_cast<C *>(c.k), static_cast<C *>(c.v), c.k_scale, c.v_scale,
-                    c.pages << c.page_shift, c.kv_heads, c.page_shift, c.dim,
-                    divisor(2 * static_cast<uint32_t>(c.kv_heads))};
+    return Cache<C>{static_cast<C *>(c.k), static_cast<C *>(c.v), c.k_scale, c.v_scale, c.pages << c.page_shift,
+        c.kv_heads, c.page_shift, c.dim, divisor(2 * static_cast<uint32_t>(c.kv_heads))};
   };
   switch (c.type) {
     case ATTN_BF16: return f(args(Tag<__nv_bfloat16>{}), Tag<__nv_bfloat16>{});
@@ -602,11 +594,10 @@ int qk_norm_rope(const NormRopeArgs &a, void *q_out, void *k_out, void *stream) 
         const unsigned blocks = blocks_for(items, kLanes);
         if (!blocks) return cudaErrorInvalidValue;
         norm_rope_kernel<T, W, kLanes, kRows, decltype(pairs)::value != 0>
-            <<<blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(norm_rope_args<T, W>(a),
-                static_cast<unsigned>(q_items),
-                                                                         static_cast<unsigned>(items), divisor((a.q_heads + kRows - 1) / kRows),
-                                                                         divisor((a.k_heads + kRows - 1) / kRows),
-                                                                         static_cast<T *>(q_out), static_cast<T *>(k_out));
+            <<<blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+                norm_rope_args<T, W>(a), static_cast<unsigned>(q_items), static_cast<unsigned>(items),
+                divisor((a.q_heads + kRows - 1) / kRows), divisor((a.k_heads + kRows - 1) / kRows),
+                static_cast<T *>(q_out), static_cast<T *>(k_out));
         return cudaGetLastError();
       };
       // One row a group while that leaves SMs without work, four rows in flight beyond.
@@ -620,7 +611,7 @@ int qk_norm_rope(const NormRopeArgs &a, void *q_out, void *k_out, void *stream) 
 size_t qk_norm_rope_workspace(int dim) { return static_cast<size_t>(backward_blocks()) * static_cast<size_t>(dim); }
 
 int qk_norm_rope_backward(const NormRopeArgs &a, const void *gq, const void *gk, void *dq, void *dk, void *dq_weight,
-                          void *dk_weight, float *workspace, void *stream) {
+    void *dk_weight, float *workspace, void *stream) {
   if (refuse(a)) return cudaErrorInvalidValue;
   return with_row_and_weight(a, [&](auto t, auto w) -> int {
     using T = typename decltype(t)::type;
@@ -642,21 +633,20 @@ int qk_norm_rope_backward(const NormRopeArgs &a, const void *gq, const void *gk,
         norm_rope_backward_kernel<T, W, kLanes, kRows, decltype(pairs)::value != 0>
             <<<blocks, kThreads, kThreads / kLanes * a.dim * sizeof(float), s>>>(
                 norm_rope_args<T, W>(a), static_cast<unsigned>(q_items), static_cast<unsigned>(items), q_blocks,
-                static_cast<const T *>(gq), static_cast<const T *>(gk), static_cast<T *>(dq), static_cast<T *>(dk), workspace);
+                static_cast<const T *>(gq), static_cast<const T *>(gk), static_cast<T *>(dq), static_cast<T *>(dk),
+                workspace);
         return cudaGetLastError();
       };
       const int e = a.interleaved ? launch(Int<1>{}) : launch(Int<0>{});
       if (e != cudaSuccess) return e;
-      return launch_after(norm_rope_weights_kernel<W>, dim3((a.dim + 31) / 32, 2), 1024, s, workspace, q_blocks,
-          blocks, a.dim,
-                          static_cast<W *>(dq_weight), static_cast<W *>(dk_weight));
+      return launch_after(norm_rope_weights_kernel<W>, dim3((a.dim + 31) / 32, 2), 1024, s, workspace, q_blocks, blocks,
+          a.dim, static_cast<W *>(dq_weight), static_cast<W *>(dk_weight));
     });
   });
 }
 
 int kv_cache_write(const KvCacheArgs &c, const void *k, const void *v, long long k_token, long long k_head,
-                   long long v_token, long long v_head, const void *slots, int wide_slots, int tokens, int type,
-                   void *stream) {
+    long long v_token, long long v_head, const void *slots, int wide_slots, int tokens, int type, void *stream) {
   if (refuse(c) || tokens < 0) return cudaErrorInvalidValue;
   if (tokens == 0) return 0;
   return with_type(type, [&](auto t) -> int {
@@ -684,7 +674,7 @@ int kv_cache_write(const KvCacheArgs &c, const void *k, const void *v, long long
 }
 
 int kv_cache_read(const KvCacheArgs &c, void *k_out, void *v_out, const void *slots, int wide_slots, int tokens,
-                  int type, void *stream) {
+    int type, void *stream) {
   if (refuse(c) || tokens < 0) return cudaErrorInvalidValue;
   if (tokens == 0) return 0;
   return with_type(type, [&](auto t) -> int {
@@ -701,7 +691,7 @@ int kv_cache_read(const KvCacheArgs &c, void *k_out, void *v_out, const void *sl
               kLanes);
           if (!blocks) return cudaErrorInvalidValue;
           kv_read_kernel<T, C, kLanes, kRows><<<blocks, kThreads, 0, s>>>(cache, static_cast<T *>(k_out),
-                                                                         static_cast<T *>(v_out), slots, wide_slots, tokens);
+              static_cast<T *>(v_out), slots, wide_slots, tokens);
           return cudaGetLastError();
         };
         return rows <= groups_at_once(kLanes) ? launch(Int<1>{}) : launch(Int<4>{});
@@ -711,7 +701,7 @@ int kv_cache_read(const KvCacheArgs &c, void *k_out, void *v_out, const void *sl
 }
 
 int attention_join(const void *outs, const float *lses, long long out_part, long long lse_part, int parts,
-                   long long rows, int dim, int in_type, int out_type, void *out, float *lse, void *stream) {
+    long long rows, int dim, int in_type, int out_type, void *out, float *lse, void *stream) {
   if (bad_rows(dim) || parts < 1 || rows < 0) return cudaErrorInvalidValue;
   if (rows == 0) return 0;
   return with_type(in_type, [&](auto t) -> int {

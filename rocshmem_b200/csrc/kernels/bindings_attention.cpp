@@ -112,7 +112,8 @@ void no_grad(const char *what, std::initializer_list<const Tensor *> tensors) {
   }
 }
 
-// A dual tensor (forward-mode differentiation) does not require a gradient: its tangent would be dropped without a word.
+// A dual tensor (forward-mode differentiation) does not require a gradient: its tangent would be dropped without a
+// word.
 void no_tangent(const char *what, std::initializer_list<const Tensor *> tensors) {
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
   for (const Tensor *t : tensors) {
@@ -132,7 +133,8 @@ void on_one_device(const char *what, std::initializer_list<const Tensor *> tenso
 
 // The inputs' device for the duration of a call, and its current stream.
 struct Here {
-  explicit Here(const Tensor &t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+  explicit Here(const Tensor &t)
+      : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
   c10::cuda::CUDAGuard guard;
   void *stream;
 };
@@ -176,7 +178,7 @@ void result(const Tensor &t, const char *name, at::IntArrayRef shape, std::initi
 // ---- norm and rotation --------------------------------------------------------------------------------------------
 
 NormRopeArgs norm_rope_args(const Tensor &q, const Tensor &k, const Tensor &q_weight, const Tensor &k_weight,
-                            const Tensor &positions, const Tensor &table, double eps, bool interleaved) {
+    const Tensor &positions, const Tensor &table, double eps, bool interleaved) {
   no_transform("qk_norm_rope", {&q, &k, &q_weight, &k_weight, &positions, &table});
   if (!is_float(q.scalar_type()) || k.scalar_type() != q.scalar_type()) {
     bad_type("q and k must both be bf16, fp16 or fp32, got ", q.scalar_type(), " and ", k.scalar_type());
@@ -241,8 +243,7 @@ NormRopeArgs norm_rope_args(const Tensor &q, const Tensor &k, const Tensor &q_we
 }
 
 std::pair<Tensor, Tensor> py_qk_norm_rope(const Tensor &q, const Tensor &k, const Tensor &q_weight,
-    const Tensor &k_weight,
-                                          const Tensor &positions, const Tensor &table, double eps, bool interleaved) {
+    const Tensor &k_weight, const Tensor &positions, const Tensor &table, double eps, bool interleaved) {
   const NormRopeArgs a = norm_rope_args(q, k, q_weight, k_weight, positions, table, eps, interleaved);
   const Here here(q);
   Tensor q_out = at::empty(q.sizes(), q.options()), k_out = at::empty(k.sizes(), k.options());
@@ -263,16 +264,16 @@ void check_capture(void *stream, int device, std::initializer_list<const Tensor 
     if (!node) continue;
     const auto of_node = node->stream();
     if (of_node.has_value() && *of_node != c10::cuda::getCurrentCUDAStream(device).unwrap()) {
-      throw std::runtime_error("qk_norm_rope: a graph of the same leaves from outside the capture is alive; drop it (its outputs "
-                               "and losses) before a backward pass is captured");
+      throw std::runtime_error("qk_norm_rope: a graph of the same leaves from outside the capture is alive; drop it "
+                               "(its outputs and losses) before a backward pass is captured");
     }
   }
 }
 
 struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k,
-                                                const Tensor &q_weight, const Tensor &k_weight, const Tensor &positions,
-                                                const Tensor &table, double eps, bool interleaved) {
+      const Tensor &q_weight, const Tensor &k_weight, const Tensor &positions, const Tensor &table, double eps,
+      bool interleaved) {
     ctx->save_for_backward({q, k, q_weight, k_weight, positions, table});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["interleaved"] = interleaved;
@@ -288,7 +289,7 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &q = saved[0], &k = saved[1], &q_weight = saved[2], &k_weight = saved[3], &table = saved[5];
     const NormRopeArgs a = norm_rope_args(q, k, q_weight, k_weight, saved[4], table, ctx->saved_data["eps"].toDouble(),
-                                          ctx->saved_data["interleaved"].toBool());
+        ctx->saved_data["interleaved"].toBool());
     const Here here(q);
     // Gradients come in any layout (an expanded one behind a sum, for instance); the kernel reads plain rows.
     auto plain = [](const Tensor &g) {
@@ -299,14 +300,13 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
     Tensor dwq = at::empty(q_weight.sizes(), q_weight.options()), dwk = at::empty(k_weight.sizes(), k_weight.options());
     Tensor workspace = at::empty({static_cast<int64_t>(qk_norm_rope_workspace(a.dim))}, table.options());
     check(qk_norm_rope_backward(a, data(gq), data(gk), data(dq), data(dk), data(dwq), data(dwk),
-                                static_cast<float *>(data(workspace)), here.stream), "qk_norm_rope_backward");
+        static_cast<float *>(data(workspace)), here.stream), "qk_norm_rope_backward");
     return {dq, dk, dwq, dwk, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
 std::pair<Tensor, Tensor> py_qk_norm_rope_any(const Tensor &q, const Tensor &k, const Tensor &q_weight,
-    const Tensor &k_weight,
-                                              const Tensor &positions, const Tensor &table, double eps, bool interleaved) {
+    const Tensor &k_weight, const Tensor &positions, const Tensor &table, double eps, bool interleaved) {
   if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || q_weight.requires_grad() ||
       k_weight.requires_grad())) {
     return py_qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved);
@@ -357,14 +357,16 @@ KvCacheArgs cache_args(const Cache &c) {
     }
   }
   for (const Tensor *t : {&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)}) {
-    if (t != nullptr && t->requires_grad()) bad_value("KvCache: the cache is written in place and cannot require a gradient");
+    if (t != nullptr && t->requires_grad()) {
+      bad_value("KvCache: the cache is written in place and cannot require a gradient");
+    }
   }
   no_tangent("KvCache", {&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)});
   int shift = 0;
   while ((int64_t{1} << shift) < size) ++shift;
   return KvCacheArgs{data(k), data(v), scaled ? static_cast<float *>(data(*c.k_scale)) : nullptr,
-                     scaled ? static_cast<float *>(data(*c.v_scale)) : nullptr, static_cast<int>(pages),
-                     static_cast<int>(heads), shift, static_cast<int>(dim), code(k.scalar_type())};
+      scaled ? static_cast<float *>(data(*c.v_scale)) : nullptr, static_cast<int>(pages), static_cast<int>(heads),
+      shift, static_cast<int>(dim), code(k.scalar_type())};
 }
 
 void py_kv_cache_write(const Cache &c, const Tensor &k, const Tensor &v, const Tensor &slots) {
@@ -395,7 +397,7 @@ void py_kv_cache_write(const Cache &c, const Tensor &k, const Tensor &v, const T
   on_one_device("kv_cache_write", {&k, &v, &slots, &c.k});
   const Here here(k);
   check(kv_cache_write(a, data(k), data(v), sk.token, sk.head, sv.token, sv.head, data(slots), wide,
-                       static_cast<int>(k.size(0)), code(k.scalar_type()), here.stream), "kv_cache_write");
+      static_cast<int>(k.size(0)), code(k.scalar_type()), here.stream), "kv_cache_write");
   written({&c.k, &c.v, or_null(c.k_scale), or_null(c.v_scale)});
 }
 
@@ -426,7 +428,7 @@ struct Paged {
 
 // Everything that does not depend on a device.
 Paged check_paged(const Tensor &q, const Cache &c, const Tensor &block_table, const Tensor &lengths,
-                  std::optional<double> scale, double softcap, int64_t window) {
+    std::optional<double> scale, double softcap, int64_t window) {
   Paged p{cache_args(c), {}};
   no_transform("paged_attention", {&q, &block_table, &lengths});
   if (!is_half(q.scalar_type()) || (p.cache.type != ATTN_E4M3 && p.cache.type != code(q.scalar_type()))) {
@@ -454,8 +456,8 @@ Paged check_paged(const Tensor &q, const Cache &c, const Tensor &block_table, co
   if (!(f > 0 && f < 1e30) || !(softcap >= 0 && softcap < 1e30) || window < 0) {
     bad_value("scale must be positive, softcap and window not negative");
   }
-  // The kernels take both as fp32 and the cap's reciprocal: what would become zero there, no cap at all, or lose digits is
-  // refused.
+  // The kernels take both as fp32 and the cap's reciprocal: what would become zero there, no cap at all, or lose digits
+  // is refused.
   if (f < kSmallest || (softcap > 0 && softcap < kSmallest)) {
     bad_value("scale and softcap (unless it is 0) must be at least ", kSmallest, ", got ", f, " and ", softcap);
   }
@@ -481,9 +483,8 @@ Paged check_paged(const Tensor &q, const Cache &c, const Tensor &block_table, co
 }
 
 std::pair<Tensor, OptTensor> py_paged_attention(const Tensor &q, const Cache &c, const Tensor &block_table,
-                                                const Tensor &lengths, std::optional<double> scale, double softcap,
-                                                int64_t window, const OptTensor &out_given, const OptTensor &lse_given,
-                                                bool want_lse) {
+    const Tensor &lengths, std::optional<double> scale, double softcap, int64_t window, const OptTensor &out_given,
+    const OptTensor &lse_given, bool want_lse) {
   Paged p = check_paged(q, c, block_table, lengths, scale, softcap, window);
   const std::initializer_list<const Tensor *> inputs = {&q, &block_table, &lengths, &c.k, &c.v, or_null(c.k_scale),
       or_null(c.v_scale)};
@@ -513,8 +514,7 @@ std::pair<Tensor, OptTensor> py_paged_attention(const Tensor &q, const Cache &c,
 }
 
 std::pair<Tensor, Tensor> py_attention_join(const Tensor &outs, const Tensor &lses,
-    std::optional<at::ScalarType> dtype_given,
-                                            const OptTensor &out_given) {
+    std::optional<at::ScalarType> dtype_given, const OptTensor &out_given) {
   no_transform("attention_join", {&outs, &lses, or_null(out_given)});
   if (!is_float(outs.scalar_type()) || lses.scalar_type() != at::kFloat) {
     bad_type("outs must be bf16, fp16 or fp32, lses fp32");
@@ -547,9 +547,8 @@ std::pair<Tensor, Tensor> py_attention_join(const Tensor &outs, const Tensor &ls
   Tensor out = out_given ? *out_given : at::empty(outs.sizes().slice(1), outs.options().dtype(dtype));
   Tensor lse = at::empty(lses.sizes().slice(1), lses.options());
   check(attention_join(data(outs), static_cast<const float *>(data(lses)), outs_part, lse_part, static_cast<int>(n),
-      B * H,
-                       static_cast<int>(D), code(outs.scalar_type()), code(dtype), data(out),
-                       static_cast<float *>(data(lse)), here.stream), "attention_join");
+      B * H, static_cast<int>(D), code(outs.scalar_type()), code(dtype), data(out), static_cast<float *>(data(lse)),
+      here.stream), "attention_join");
   written({or_null(out_given)});
   return {out, lse};
 }
@@ -574,7 +573,7 @@ PYBIND11_MODULE(_A, m) {
   m.def("kv_cache_write", &py_kv_cache_write);
   m.def("kv_cache_read", &py_kv_cache_read);
   m.def("check_paged", [](const Tensor &q, const Cache &c, const Tensor &table, const Tensor &lengths,
-                          std::optional<double> scale, double softcap, int64_t window) {
+      std::optional<double> scale, double softcap, int64_t window) {
     check_paged(q, c, table, lengths, scale, softcap, window);
   });
   m.def("paged_attention", &py_paged_attention);

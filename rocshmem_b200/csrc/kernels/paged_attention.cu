@@ -1,6 +1,7 @@
 // Attention of one new token per sequence over a paged cache, split over the cache's length and joined.
 //
-//   s_j = scale q.k_j  (capped: c tanh(s_j / c)),   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   lse = m + log sum
+//   s_j = scale q.k_j  (capped: c tanh(s_j / c))
+//   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   lse = m + log sum_j exp(s_j - m)
 //
 // A key and a value are read once and used by the 1 - 16 query heads that share them, so memory bounds the kernel:
 // about 23 bytes a cycle and SM have to arrive, and the arithmetic only has to keep up. The products run on warp-level
@@ -50,7 +51,9 @@ constexpr float kF16Shift = 14.f;
 
 enum Mode : int { MODE_BF16 = 0, MODE_F16 = 1, MODE_E4M3 = 2 };
 
-__device__ __forceinline__ uint32_t smem_addr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ uint32_t smem_addr(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -77,11 +80,13 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 template <bool BF16>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (BF16) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+                 "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   } else {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+                 "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
@@ -221,8 +226,7 @@ __device__ __forceinline__ void store_out(const Params &p, long long at, float x
 // the lse.
 template <int NT>
 __device__ __forceinline__ void finish(const Params &p, long long row0, int n_heads, int j, int lane,
-    const float (&m)[2],
-                                       const float (&l)[2], float (&inv)[2]) {
+    const float (&m)[2], const float (&l)[2], float (&inv)[2]) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const int col = 8 * j + 2 * (lane % 4) + c;
@@ -235,7 +239,7 @@ __device__ __forceinline__ void finish(const Params &p, long long row0, int n_he
 // Fragment (d, j) of O^T times the heads' factors, to the result. All lanes of the warp call it.
 template <int D, int MODE>
 __device__ __forceinline__ void store_fragment(const Params &p, long long row0, int n_heads, int j, int d, int lane,
-                                               const float (&o)[4], const float (&inv)[2]) {
+    const float (&o)[4], const float (&inv)[2]) {
   const int g = lane / 4, t = lane % 4;
   if (p.out_f32) {
 #pragma unroll
@@ -262,7 +266,8 @@ __device__ __forceinline__ void store_fragment(const Params &p, long long row0, 
     for (int r = 0; r < 2; ++r) {
       const uint32_t w = transpose8x8(pack2<MODE == MODE_BF16>(o[2 * r] * inv[0], o[2 * r + 1] * inv[1]));
       if (8 * j + g < n_heads) {
-        *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + (row0 + 8 * j + g) * D + 16 * d + 8 * r + 2 * t) = w;
+        uint16_t *const to = static_cast<uint16_t *>(p.out) + (row0 + 8 * j + g) * D;
+        *reinterpret_cast<uint32_t *>(to + 16 * d + 8 * r + 2 * t) = w;
       }
     }
   }
@@ -279,7 +284,7 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
   const int g = lane / 4, t = lane % 4;
   Cursor ahead = cur;
 
-  // ---- loads: `ahead` runs kStages - 1 tiles before `cur`; a tile's page is looked up one step before its rows are ----
+  // ---- loads: `ahead` runs kStages - 1 tiles before `cur`; a tile's page is looked up a step before its rows are ----
   const uint32_t stages = smem_addr(ring);
   struct Next {
     int page, pos, head;  // of the lane's key; pos < 0: none
@@ -310,7 +315,8 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
       const unsigned r = kEven ? i * kEach + my_row : at / kChunks, c = kEven ? 0 : at % kChunks;
       const int from = __shfl_sync(0xffffffffu, row, r);
       const uint32_t bytes = from < 0 ? 0 : 16;
-      const unsigned long long off = static_cast<unsigned long long>(static_cast<unsigned>(max(from, 0))) * S::kRowBytes;
+      const unsigned at_row = static_cast<unsigned>(max(from, 0));
+      const unsigned long long off = static_cast<unsigned long long>(at_row) * S::kRowBytes;
       const uint32_t to_k = kEven ? i * kEach * S::kPitchK : r * S::kPitchK + c * 16;
       const uint32_t to_v = kEven ? i * kEach * S::kPitchV : r * S::kPitchV + c * 16;
       copy16(my_to + at_stage + to_k, my_k + off + c * 16, bytes);
@@ -366,8 +372,8 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
         q_scale[j][0] = q_scale[j][1] = 1.f;
       } else {
         // A head's largest magnitude brought to [1, 2) by a power of two. bf16 values (8 bits) then fit fp16 exactly
-        // down to 2^-17, fp16 values (11 bits) down to 2^-14; what is smaller is rounded to steps of 2^-24, off by 2^-25
-        // at most, half of what fp32 would round off the largest element's product.
+        // down to 2^-17, fp16 values (11 bits) down to 2^-14; what is smaller is rounded to steps of 2^-24, off by
+        // 2^-25 at most, half of what fp32 would round off the largest element's product.
         uint4 raw[D / 32];
         uint32_t top = 0;
 #pragma unroll
@@ -533,9 +539,9 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
         }
         if constexpr (MODE == MODE_E4M3) v_unit = 1.f / cv;
         // P^T, as a value rounded to the operand's type and the rounded rest: of one part alone the rounding of
-        // bf16 (2^-8) or fp16 (2^-11) would be as large as that of the result. Two are off by 2^-17 and 2^-23. The second
-        // costs nothing where memory bounds (one part, 64 sequences of 1024 - 4096 tokens: 117 us both), 8 % with 16
-        // heads a key head in e4m3 (54.0 against 49.7).
+        // bf16 (2^-8) or fp16 (2^-11) would be as large as that of the result. Two are off by 2^-17 and 2^-23. The
+        // second costs nothing where memory bounds (64 sequences of 1024 - 4096 tokens in bf16: 117 us both), 8 % with
+        // 16 heads a key head in e4m3 (54.0 us against 49.7).
         uint32_t pf[MT][NT][2], pr[MT][NT][2];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
@@ -642,8 +648,7 @@ __device__ __forceinline__ void run_share(const Params &p, char *ring, Cursor cu
 // A partial result: fragments as they lie in the lanes, then maxima and sums of the columns.
 template <int D, int NT, int MODE>
 __device__ __forceinline__ void store_part(float *part, int lane, const float (&o)[D / 16][NT][4],
-    const float (&m)[NT][2],
-                                           const float (&l)[NT][2], float cv) {
+    const float (&m)[NT][2], const float (&l)[NT][2], float cv) {
   using S = Shape<D, NT, MODE>;
   const float f = MODE == MODE_E4M3 ? cv : 1.f;
 #pragma unroll
@@ -675,7 +680,8 @@ __device__ __forceinline__ Joined nothing() {
 __device__ __forceinline__ void add(Joined &a, const Joined &x) {
   const float2 now = make_float2(fmaxf(a.m.x, x.m.x), fmaxf(a.m.y, x.m.y));
   const float bx = now.x == -INFINITY ? 0.f : now.x, by = now.y == -INFINITY ? 0.f : now.y;
-  const float kx = exp2_fast(a.m.x - bx), ky = exp2_fast(a.m.y - by), ax = exp2_fast(x.m.x - bx), ay = exp2_fast(x.m.y - by);
+  const float kx = exp2_fast(a.m.x - bx), ky = exp2_fast(a.m.y - by);
+  const float ax = exp2_fast(x.m.x - bx), ay = exp2_fast(x.m.y - by);
   a.o.x = fmaf(x.o.x, ax, a.o.x * kx);
   a.o.y = fmaf(x.o.y, ay, a.o.y * ky);
   a.o.z = fmaf(x.o.z, ax, a.o.z * kx);
@@ -762,7 +768,7 @@ __global__ void __launch_bounds__(32, Shape<D, NT, MODE>::kBlocks) paged_kernel(
   cur.tile = static_cast<int>(into - static_cast<long long>(cur.unit) * cur.n);
   cur.left = static_cast<int>(t1 - t0);
   run_share<D, NT, MODE>(p, ring, cur, lane, [&](const Cursor &pair, bool begins, bool ends, int h0, int n_heads,
-                                                 float (&o)[DK][NT][4], float (&m)[NT][2], float (&l)[NT][2], float cv) {
+      float (&o)[DK][NT][4], float (&m)[NT][2], float (&l)[NT][2], float cv) {
     if (begins && lane == 0) {
       const int share = blockIdx.x;
       p.spans[static_cast<long long>(pair.b) * units + pair.unit] =
@@ -803,9 +809,8 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, MODE>::kTeam) paged_short_ke
   float *const part = reinterpret_cast<float *>(ring);
   static_assert(S::kPart * 4 <= S::kSmem, "a part fits the ring");
   if (cur.left > 0) {
-    run_share<D, NT, MODE>(p, ring, cur, lane,
-        [&](const Cursor &, bool, bool, int, int, float (&o)[DK][NT][4], float (&m)[NT][2],
-                                                   float (&l)[NT][2], float cv) {
+    run_share<D, NT, MODE>(p, ring, cur, lane, [&](const Cursor &, bool, bool, int, int, float (&o)[DK][NT][4],
+        float (&m)[NT][2], float (&l)[NT][2], float cv) {
       copies_wait<0>();
       __syncwarp();
       store_part<D, NT, MODE>(part, lane, o, m, l, cv);
@@ -871,11 +876,11 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const Params p) {
 // elements, bf16, 32 pairs, one launch against two: 128 keys 6.2 us against 9.8, 512 keys 10.3 and 10.3, 1024 keys 14.4
 // and 11.1.
 //
-// Over a grid of 1 - 32 sequences of 16 - 2048 keys, 64, 128 and 256 elements, bf16 and e4m3, 4 and 16 heads a key head,
-// the rule takes the faster form, or one within 8 % of it, in 308 of 336 cases. It is off most for more pairs than SMs
-// of 64 elements, of which an SM holds several blocks (256 pairs of 128 keys: two launches 9.8 us, one would take 6.2),
-// and at its upper end for few pairs that two launches would split further (4 pairs of 512 keys with 16 heads: one
-// launch 12.3 us, two 8.8; 8 pairs with 4 heads 10.3 and 8.2; 256 elements in e4m3 14.9 and 11.1).
+// Over a grid of 1 - 32 sequences of 16 - 2048 keys, 64, 128 and 256 elements, bf16 and e4m3, 4 and 16 heads a key
+// head, the rule takes the faster form, or one within 8 % of it, in 308 of 336 cases. It is off most for more pairs
+// than SMs of 64 elements, of which an SM holds several blocks (256 pairs of 128 keys: two launches 9.8 us, one would
+// take 6.2), and at its upper end for few pairs that two launches would split further (4 pairs of 512 keys with 16
+// heads: one launch 12.3 us, two 8.8; 8 pairs with 4 heads 10.3 and 8.2; 256 elements in e4m3 14.9 and 11.1).
 constexpr int kShortKeys = 64;
 // Keys that a share has at least: below that its fixed costs weigh more than the loads that another warp would take
 // over.
@@ -894,8 +899,9 @@ auto with_shape(int dim, int group, int cache_type, F f) {
     return f(Int<D>{}, Int<1>{}, Int<M>{});
   };
   auto modes = [&](auto d) {
-    return cache_type == ATTN_BF16 ? heads(d, Int<MODE_BF16>{}) : cache_type == ATTN_F16 ? heads(d, Int<MODE_F16>{})
-                                                                                       : heads(d, Int<MODE_E4M3>{});
+    return cache_type == ATTN_BF16  ? heads(d, Int<MODE_BF16>{})
+           : cache_type == ATTN_F16 ? heads(d, Int<MODE_F16>{})
+                                    : heads(d, Int<MODE_E4M3>{});
   };
   return dim == 64 ? modes(Int<64>{}) : dim == 96 ? modes(Int<96>{}) : dim == 128 ? modes(Int<128>{})
       : modes(Int<256>{});
@@ -950,9 +956,10 @@ int launch(Params p, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   if (longest_of(p) <= S::kKeys) return 0;  // no pair has two tiles: nothing to join
   // Many parts of each of a few pairs are shared by eight sets of threads (8 pairs of 32768 keys, 148 parts: 35 us the
-  // whole call, with one set 56); few parts of many pairs are not worth the exchange (512 pairs of 2048 keys: 68 us with
-  // one set, 76 with eight). The two are level at 128 pairs for 128 elements (2048 keys: 26.8 and 26.5), so that between
-  // 50 and 128 pairs, which have one set, eight would be up to a quarter faster (64 pairs of 2048 keys: 20.4 and 16.4).
+  // whole call, with one set 56); few parts of many pairs are not worth the exchange (512 pairs of 2048 keys: 68 us
+  // with one set, 76 with eight). The two are level at 128 pairs for 128 elements (2048 keys: 26.8 and 26.5), so that
+  // between 50 and 128 pairs, which have one set, eight would be up to a quarter faster (64 pairs of 2048 keys: 20.4
+  // and 16.4).
   const int shares = p.blocks;
   return pairs > shares / 24 ? launch_join<D, NT, MODE, 1>(p, s) : launch_join<D, NT, MODE, 8>(p, s);
 }
@@ -1014,7 +1021,7 @@ size_t paged_attention_workspace(const KvCacheArgs &c, const PagedAttentionArgs 
 }
 
 int paged_attention(const KvCacheArgs &c, const PagedAttentionArgs &a, void *workspace, size_t workspace_bytes,
-                    void *stream) {
+    void *stream) {
   if (refuse_call(c, a) || (c.type == ATTN_E4M3 && c.pages > 0 && (!c.k_scale || !c.v_scale)) ||
       (a.q_type != ATTN_BF16 && a.q_type != ATTN_F16) || (c.type != ATTN_E4M3 && c.type != a.q_type) ||
       (a.out_type != a.q_type && a.out_type != ATTN_F32) || workspace_bytes < paged_attention_workspace(c, a)) {

@@ -136,7 +136,7 @@ class KvCache:
         if dtype != E4M3:
             return cls(zeros(shape, dtype), zeros(shape, dtype))
         return cls(zeros(shape, dtype), zeros(shape, dtype), zeros(shape[:3], torch.float32),
-            zeros(shape[:3], torch.float32))
+                   zeros(shape[:3], torch.float32))
 
     def free(self) -> None:
         """Collective: give a symmetric cache's memory back to the heap."""
@@ -238,9 +238,8 @@ def paged_attention(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor, 
     if stream is not None:
         with _On(stream, q, block_table, lengths, *cache._tensors(), out, lse):
             return paged_attention(q, cache, block_table, lengths, scale, softcap, window, out, lse, return_lse)
-    both = _native.load_attention().paged_attention(q, cache._cache, block_table, lengths, scale, softcap, window,
-        out, lse,
-                                                    return_lse)
+    both = _native.load_attention().paged_attention(q, cache._cache, block_table, lengths, scale, softcap, window, out,
+                                                    lse, return_lse)
     return both if return_lse else both[0]
 
 
@@ -260,8 +259,7 @@ def attention_join(outs: torch.Tensor, lses: torch.Tensor, dtype: Optional[torch
 # ---- references (plain PyTorch, any device) -------------------------------------------------------------------------
 
 def ref_norm_rope(x: torch.Tensor, weight: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
-    eps: float = 1e-6,
-                  interleaved: bool = False) -> torch.Tensor:
+                  eps: float = 1e-6, interleaved: bool = False) -> torch.Tensor:
     """PyTorch reference of :func:`qk_norm_rope` for one of the two tensors, in 64 bits, differentiable."""
     R = table.shape[1]
     x = x.double()
@@ -328,6 +326,6 @@ def ref_attention_join(outs: torch.Tensor, lses: torch.Tensor):
     top = l.amax(dim=0)
     w = torch.exp(l - torch.where(top == float("-inf"), 0.0, top))
     total = w.sum(dim=0)
-    out = torch.where(w[..., None] > 0, outs.double() * w[..., None], 0.0).sum(dim=0) / torch.where(total > 0, total,
-        1.0)[..., None]
+    out = torch.where(w[..., None] > 0, outs.double() * w[..., None], 0.0).sum(dim=0)
+    out = out / torch.where(total > 0, total, 1.0)[..., None]
     return out, torch.where(total > 0, top + total.clamp(min=1e-300).log(), float("-inf"))

@@ -69,15 +69,16 @@ class ContextParallelDecode:
         positions of the whole sequence its tokens have, and a block table can leave out whole pages only, while a
         window's edge mostly lies inside one."""
         if q.dim() != 3 or q.shape[1:] != (self.heads, self.head_dim) or q.shape[0] > self.max_batch:
-            raise ValueError(f"q must be [batch <= {self.max_batch}, {self.heads}, {self.head_dim}], got {tuple(q.shape)}")
+            raise ValueError(f"q must be [batch <= {self.max_batch}, {self.heads}, {self.head_dim}], "
+                             f"got {tuple(q.shape)}")
         if q.shape[0] == 0:
             return torch.empty_like(q)
         cuda = rt.is_cuda()
         if self.n == 1:
             if cuda:
                 return attention.paged_attention(q, cache, block_table, lengths, scale=scale, softcap=softcap)
-            return attention.ref_paged_attention(q, cache, block_table, lengths, scale=scale,
-                softcap=softcap)[0].to(q.dtype)
+            out = attention.ref_paged_attention(q, cache, block_table, lengths, scale=scale, softcap=softcap)[0]
+            return out.to(q.dtype)
         if self.mine is None:
             raise RuntimeError("ContextParallelDecode was destroyed")
         B = q.shape[0]
