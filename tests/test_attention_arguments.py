@@ -92,7 +92,7 @@ def test_primals_within_a_dual_level_pass():
     lambda: torch.func.jvp(lambda t: norm_rope(table=t)[0], (torch.zeros(8, 64),), (torch.ones(8, 64),)),
     lambda: torch.func.functionalize(lambda w: norm_rope(q_weight=w)[0])(torch.ones(64)),
     lambda: torch.func.vmap(lambda k: write(k=k) or k)(zeros(2, 3, 2, 64)),
-    lambda: torch.func.vmap(lambda slots: at.kv_cache_read(cache(), slots)[0])(torch.zeros(2, 3, dtype=torch.int64)),
+    lambda: torch.func.vmap(lambda at_: at.kv_cache_read(cache(), at_)[0])(torch.zeros(2, 3, dtype=torch.int64)),
     lambda: torch.func.vmap(lambda k: at.KvCache(k, zeros(4, 2, 16, 64)) and k)(zeros(2, 4, 2, 16, 64)),
     lambda: torch.func.vmap(lambda q: attend(q=q))(zeros(3, 2, 4, 64)),
     lambda: torch.func.grad(lambda q: attend(q=q).float().sum())(zeros(2, 4, 64)),
@@ -110,7 +110,7 @@ def test_transforms_are_refused_by_the_operators_themselves(call):
 
 @pytest.mark.parametrize("leaves", [False, True])
 def test_a_table_that_requires_a_gradient_is_refused(leaves):
-    """Alone its gradient would be cut off, beside trained inputs it would be undefined: frequencies that never train."""
+    """Alone its gradient would be cut off, beside trained inputs undefined: frequencies that never train."""
     frequencies = torch.full((32,), 0.5, requires_grad=True)
     table = at.rope_table(8, 64, frequencies=frequencies)
     assert table.requires_grad

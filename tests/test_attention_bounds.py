@@ -1,22 +1,24 @@
 """Attention operators against 64 bits with bounds as narrow as their arithmetic: a probability that enters the second
-product with one rounding to 16 bits, or a token whose part of a weight's gradient is lost, is outside of them. That the
-bounds notice both is shown on the CPU, with the mistake in the oracle.
+product with one rounding to 16 bits, or a token whose part of a weight's gradient is lost, is outside of them. That
+the bounds notice both is shown on the CPU, with the mistake in the oracle.
 
 E = 2^-24 is the rounding of one fp32 operation, relative to its result.
 
-Paged attention, fp32 results. Queries, keys, factors of keys and the scale are small multiples of powers of two, so that
-a score q.k is exact. The score in base 2 then has the rounding of log2(e) and of one product (2 E of it), the
+Paged attention, fp32 results. Queries, keys, factors of keys and the scale are small multiples of powers of two, so
+that a score q.k is exact. The score in base 2 then has the rounding of log2(e) and of one product (2 E of it), the
 subtraction of the maximum one (E of score and maximum; fp16 and e4m3: the maximum is 14 less), its power of two 2^-22
 (4 E). A running result is multiplied by a power of two at every tile of 16 keys at most and at every part that is
 joined, each with 6 E; every tile adds to the sum of a lane (4 E, and 8 for the lanes). A weight is off by the sum of
 these, the normalised result by that of the weights and that of their sum. A matrix instruction adds 17 numbers, each
-cut off at E of the largest, two for a tile (34 E). In two parts a probability is off by 2^-17 of it in bf16: the rest of
-the first rounding is less than 2^-8 of its power of two, and 8 bits of it are kept; 2^-23 in fp16, and what is below the
-smallest number, 2^-25 where the largest probability is 2^14. A one-part probability would be off by up to 2^-8 or 2^-11.
+cut off at E of the largest, two for a tile (34 E). In two parts a probability is off by 2^-17 of it in bf16: the rest
+of the first rounding is less than 2^-8 of its power of two, and 8 bits of it are kept; 2^-23 in fp16, and what is
+below the smallest number, 2^-25 where the largest probability is 2^14. A one-part probability would be off by up to
+2^-8 or 2^-11.
 
-Weight gradients. A term g n has two roundings from the rotation, 11 from the norm (10 positive additions count half under
-the root, 4 for the reciprocal root, 2 products) and is 16 E off at most; sums have one rounding for each addition on the
-longest path: two rows a round and lane group, the groups of a block, a 32nd of the blocks, 5 within a warp."""
+Weight gradients. A term g n has two roundings from the rotation, 11 from the norm (10 positive additions count half
+under the root, 4 for the reciprocal root, 2 products) and is 16 E off at most; sums have one rounding for each
+addition on the longest path: two rows a round and lane group, the groups of a block, a 32nd of the blocks, 5 within a
+warp."""
 import math
 
 import pytest

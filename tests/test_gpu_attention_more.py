@@ -1,4 +1,4 @@
-"""Attention operators on a GPU, beside test_gpu_attention.py: tensors that are written in place."""
+"""Attention operators on a GPU, beside test_gpu_attention.py: tensors that are written in place, the range of sums."""
 import pytest
 import torch
 
@@ -69,3 +69,33 @@ def test_tensors_made_in_inference_mode_are_written_inside_and_outside_of_it():
     at.paged_attention(q, c, table, lengths, out=out, lse=lse)
     joined, _ = at.attention_join(out[None], lse[None], out=torch.empty_like(out))
     assert torch.equal(out, want) and torch.equal(joined, want)
+
+
+# ---- the range of sums ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+def test_values_whose_magnitudes_add_up_to_1e34(cache, wide):
+    """The largest that the documentation allows, in one launch and in two (partial results hold up to 2^14 times a
+    sum), with equal and with different weights. The bound: one rounding to bf16, and fp32 sums of 300 terms."""
+    from rocshmem_b200.ops import attention as at
+    g, n, D = gen(3), 300, 128
+    c = at.KvCache.allocate(19, 16, 1, D, cache)
+    size = 0.99e34 / n
+    signs = torch.randint(0, 2, c.v.shape, generator=g, device="cuda") * 2.0 - 1.0
+    if cache == E4M3:
+        c.k.copy_(randn(g, *c.k.shape).to(E4M3))
+        c.v.copy_((signs * 448).to(E4M3))
+        c.k_scale.fill_(1.0)
+        c.v_scale.fill_(size / 448)
+    else:
+        c.k.copy_(randn(g, *c.k.shape))
+        c.v.copy_(signs * size)
+    table = torch.full((1, 200 if wide else 19), -1, dtype=torch.int32, device="cuda")
+    table[0, :19] = torch.randperm(19, generator=g, device="cuda")
+    lengths = torch.tensor([n], dtype=torch.int32, device="cuda")
+    for q in (torch.zeros(1, 4, D, dtype=BF16, device="cuda"), randn(g, 1, 4, D, dtype=BF16)):
+        out = at.paged_attention(q, c, table, lengths)
+        want, _ = at.ref_paged_attention(q, c, table, lengths)
+        assert out.isfinite().all()
+        assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -13 * size).all()
