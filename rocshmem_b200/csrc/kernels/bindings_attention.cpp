@@ -68,7 +68,7 @@ void *data(const Tensor &t) { return const_cast<void *>(t.const_data_ptr()); }
 // Tensors inside a torch.func transform are wrappers without memory of their own. Called before an address is taken.
 void no_transform(const char *what, std::initializer_list<const Tensor *> tensors) {
   static const c10::DispatchKeySet wrappers({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
-      c10::DispatchKey::Functionalize});
+      c10::DispatchKey::Batched, c10::DispatchKey::Functionalize});
   for (const Tensor *t : tensors) {
     if (t != nullptr && t->key_set().has_any(wrappers)) {
       bad_value(what, " cannot be called inside a torch.func transform (vmap, grad, jvp and the like)");
@@ -286,6 +286,8 @@ struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
     if (at::GradMode::is_enabled()) {
       throw std::runtime_error("qk_norm_rope can be differentiated once: create_graph is refused");
     }
+    no_transform("qk_norm_rope's backward pass", {&grads[0], &grads[1]});
+    no_tangent("qk_norm_rope's backward pass", {&grads[0], &grads[1]});
     const auto saved = ctx->get_saved_variables();
     const Tensor &q = saved[0], &k = saved[1], &q_weight = saved[2], &k_weight = saved[3], &table = saved[5];
     const NormRopeArgs a = norm_rope_args(q, k, q_weight, k_weight, saved[4], table, ctx->saved_data["eps"].toDouble(),

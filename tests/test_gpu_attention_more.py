@@ -99,3 +99,27 @@ def test_values_whose_magnitudes_add_up_to_1e34(cache, wide):
         want, _ = at.ref_paged_attention(q, c, table, lengths)
         assert out.isfinite().all()
         assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -13 * size).all()
+
+
+# ---- derivatives of the backward pass -------------------------------------------------------------------------------
+
+def test_gradients_with_a_derivative_of_their_own_are_refused():
+    """A backward pass whose incoming gradient has a tangent (its result would have none), and one under vmap. The
+    engine turns the refusals into a RuntimeError, as it does that of a second derivative."""
+    import torch.autograd.forward_ad as fwd
+    from rocshmem_b200.ops import attention as at
+    g = gen(2)
+    leaves = [randn(g, 5, 2, 64).requires_grad_(), randn(g, 5, 1, 64).requires_grad_()]
+    w, positions = torch.ones(64, device="cuda"), torch.arange(5, device="cuda")
+    table = at.rope_table(8, 64, device="cuda")
+    out = at.qk_norm_rope(*leaves, w, w, positions, table)
+    grads = [randn(g, *x.shape) for x in out]
+    plain = torch.autograd.grad(out, leaves, grads, retain_graph=True)
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.autograd.grad(out, leaves, [grads[0], fwd.make_dual(grads[1], grads[1])], retain_graph=True)
+        within = torch.autograd.grad(out, leaves, grads, retain_graph=True)
+    with pytest.raises(RuntimeError, match="torch.func transform"):
+        torch.autograd.grad(out, leaves, [torch.stack([x, x]) for x in grads], retain_graph=True, is_grads_batched=True)
+    again = torch.autograd.grad(out, leaves, grads)
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(plain, within, again))
