@@ -17,6 +17,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as fwd
 
 from .. import runtime as rt
 from ..ops import attention
@@ -67,13 +68,20 @@ class ContextParallelDecode:
         tokens ``[B, heads, head_dim]`` in q's type, the same bits on every member. Arguments as in
         :func:`rocshmem_b200.ops.attention.paged_attention`. There is no sliding window: a member does not know which
         positions of the whole sequence its tokens have, and a block table can leave out whole pages only, while a
-        window's edge mostly lies inside one."""
+        window's edge mostly lies inside one. A ``q`` with a derivative is refused."""
         if q.dim() != 3 or q.shape[1:] != (self.heads, self.head_dim) or q.shape[0] > self.max_batch:
             raise ValueError(f"q must be [batch <= {self.max_batch}, {self.heads}, {self.head_dim}], "
                              f"got {tuple(q.shape)}")
         if q.shape[0] == 0:
             return torch.empty_like(q)
         cuda = rt.is_cuda()
+        if not cuda:
+            # What paged_attention refuses on GPUs; the reference that stands in for it would let autograd into the
+            # symmetric buffers.
+            if torch.is_grad_enabled() and q.requires_grad:
+                raise ValueError("ContextParallelDecode has no backward pass: call it under torch.no_grad(), or detach q")
+            if fwd.unpack_dual(q).tangent is not None:
+                raise ValueError("ContextParallelDecode has no forward-mode derivative: pass the primal of q")
         if self.n == 1:
             if cuda:
                 return attention.paged_attention(q, cache, block_table, lengths, scale=scale, softcap=softcap)
