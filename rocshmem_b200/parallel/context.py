@@ -79,7 +79,8 @@ class ContextParallelDecode:
             # What paged_attention refuses on GPUs; the reference that stands in for it would let autograd into the
             # symmetric buffers.
             if torch.is_grad_enabled() and q.requires_grad:
-                raise ValueError("ContextParallelDecode has no backward pass: call it under torch.no_grad(), or detach q")
+                raise ValueError("ContextParallelDecode has no backward pass: call it under torch.no_grad(), or detach "
+                                 "q")
             if fwd.unpack_dual(q).tangent is not None:
                 raise ValueError("ContextParallelDecode has no forward-mode derivative: pass the primal of q")
         if self.n == 1:

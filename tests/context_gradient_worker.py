@@ -1,4 +1,5 @@
-"""One PE of the test that decoding over a team refuses queries with a derivative (started by test_context_arguments.py)."""
+"""One PE of the test that decoding over a team refuses queries with a derivative (started by
+test_context_arguments.py)."""
 import torch
 import torch.autograd.forward_ad as fwd
 
